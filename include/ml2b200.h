@@ -40,7 +40,8 @@ extern "C" {
 #define ML2_E_INVALID (-1)   /* bad size, null or misaligned pointer, unsupported shape */
 #define ML2_E_CUDA (-2)      /* a CUDA runtime call failed; text in ml2_last_error() */
 #define ML2_E_STATE (-3)     /* call made in the wrong state (e.g. forward before bind) */
-#define ML2_E_DEVICE (-4)    /* a kernel's bounded wait ran out; status word in ml2_ctx_status() */
+#define ML2_E_DEVICE (-4)    /* a kernel's bounded wait ran out, or an operator met an invalid index in a device table;
+                              * status word in ml2_ctx_status() */
 #define ML2_E_NCCL (-5)      /* an NCCL call failed */
 
 typedef struct ml2_ctx ml2_ctx;
@@ -77,7 +78,8 @@ int ml2_ctx_synchronize(ml2_ctx* ctx);
  * runs to its end; the next synchronising call returns ML2_E_DEVICE. No counterpart in the reference
  * (its kernels never wait on one another). */
 int ml2_ctx_set_wait_limit(ml2_ctx* ctx, long long sm_cycles);
-/* Reads and clears the device error word written when a kernel's bounded wait expired. */
+/* Reads and clears the device error words: a kernel's bounded wait expired, or (codes from 0x101 on) one of the
+ * batched-decoding operators left out an element because its index in a device table was out of range. */
 int ml2_ctx_status(ml2_ctx* ctx, unsigned* error, unsigned* detail);
 /* Number of kernels this library has launched through `ctx` so far. */
 long long ml2_ctx_launch_count(ml2_ctx* ctx);
@@ -128,6 +130,63 @@ int ml2_embedding(ml2_ctx* ctx, void* out, const void* table, int size, const in
  * argmax(logits) when write_token != 0. Ties resolve to the LOWEST index (the reference's kernel
  * leaves ties to a race, :32-36; its CPU test expects the first maximum, test/ArgmaxTests.cs:33-46). */
 int ml2_argmax(ml2_ctx* ctx, const void* logits, int vocab_size, int* tokens, int next_pos, int write_token);
+
+/* ---- operator level: batched decoding over a paged cache --------------------------------------
+ * No counterpart in the reference, which decodes one sequence. A cache is rows of keys and values; a page is page_size
+ * (a power of two up to 1024) consecutive rows, and row `slot` = page * page_size + offset. One step of a batch is
+ * ml2_block_tables once, then per layer ml2_qk_norm_rope and ml2_prefix_attention. All three run on the context's stream
+ * without allocation or synchronisation and can be captured in CUDA graphs. Indices that they read on the device and
+ * find out of range are left out and reported by ml2_ctx_status. */
+#define ML2_F16 0
+#define ML2_BF16 1
+typedef struct ml2_kv {
+    void* key;            /* [rows][row_stride], a row holds n_kv_heads * head_size values */
+    void* value;
+    long long row_stride; /* elements from one row to the next, the same for both */
+    long long rows;
+} ml2_kv;
+#define ML2_REFUSED_LENGTH 1 /* a length is negative or needs more than table_stride pages */
+#define ML2_REFUSED_PAGES 2  /* the free pages do not suffice */
+#define ML2_REFUSED_TOKENS 3 /* the new tokens do not fit the slot map */
+/* Block tables and slot maps from request lengths (1..8192 requests). `lengths` are the tokens each request has in the
+ * cache, `new_lengths` what it shall have: growth takes pages, shrinking (0 ends a request) gives pages back. First the
+ * pages of requests that shrink are pushed on `free_pages` (a stack of *free_count entries with room for all n_pages pages of the cache) in the order
+ * of request and page, then requests that grow take pages from its top in request order and have them entered in
+ * table[request][table_stride]. A request is refused, and keeps its length and its pages, when a length is invalid, when
+ * the tokens of all requests up to it exceed max_tokens, or when it needs pages and the pages needed up to it (by
+ * requests not refused for the first two reasons) exceed the free ones; refused[request] is 0 or the reason.
+ * Row query_start[r] + i of the slot map is new token i of request r: slots[row] = its cache row, positions[row] =
+ * position_offset + its place in the request (position_offset: length of a prefix that is kept elsewhere). Rows from
+ * query_start[n_requests] to max_tokens are padding: slot -1, position 0. lengths_out and free_count_out may be the arrays
+ * lengths and free_count; where they are others, the call can be repeated with the same result. */
+int ml2_block_tables(ml2_ctx* ctx, const int* lengths, const int* new_lengths, int n_requests, int page_size, int* table, int table_stride,
+                     int* free_pages, const int* free_count, int n_pages, int* lengths_out, int* free_count_out, int* query_start,
+                     int* slots, int* positions, int max_tokens, int* refused, int position_offset);
+/* RMS norm of every query and key head (weights of head_size values; both null: no norm), rotation of the first
+ * rotary_size values of each head (pairs i, i + rotary_size / 2 as in ml2_rope; angle positions[t] *
+ * theta^(-2i / rotary_size), reduced in 64 bits), queries to query_out (may be query), keys and values to the cache rows
+ * slots[t], which must differ from one another. A token with a negative slot is padding: nothing of it is written.
+ * Arithmetic in fp32, one rounding to `dtype`. head_size and rotary_size are multiples of 16, head_size at most 256;
+ * strides in elements, multiples of 8; pointers 16-byte aligned. */
+int ml2_qk_norm_rope(ml2_ctx* ctx, int dtype, void* query_out, long long query_out_stride, const ml2_kv* cache, const void* query,
+                     long long query_stride, const void* key, long long key_stride, const void* value, long long value_stride,
+                     const void* query_weight, const void* key_weight, const int* positions, const int* slots, int n_tokens, int n_heads,
+                     int n_kv_heads, int head_size, int rotary_size, float theta, float eps);
+/* Attention of a batch that shares a prefix. Query rows query_start[r] .. query_start[r + 1] - 1 belong to request r, whose
+ * lengths[r] own tokens (the new ones included) lie in the pages table[r]; row i of `queries` sees all prefix->rows rows of
+ * the prefix and own tokens 0 .. lengths[r] - queries + i. out[row][head] = softmax(scale q.k) v; lse (may be null, fp32
+ * [n_rows][n_heads]) = log sum exp(scale q.k). A row that sees nothing, or whose scores are all -inf, gives zeros and
+ * -inf. Rows from query_start[n_requests] to n_rows stay as they are. Scores, softmax and sums are fp32; the weights are
+ * rounded to `dtype` before their product with the values. Prefix rows and cache rows that no query sees are not used,
+ * whatever they hold. max_length bounds lengths[]. head_size 64 or 128; strides in elements, multiples of 8; pointers
+ * 16-byte aligned. `workspace` (ml2_prefix_attention_workspace bytes for the same sizes, or for larger n_rows, n_requests,
+ * prefix and max_length) holds partial results: calls that may run at the same time need one each. */
+int ml2_prefix_attention_workspace(ml2_ctx* ctx, int n_rows, int n_requests, int prefix_length, int max_length, int n_heads,
+                                   int n_kv_heads, int head_size, size_t* bytes);
+int ml2_prefix_attention(ml2_ctx* ctx, int dtype, void* out, long long out_stride, float* lse, const void* query, long long query_stride,
+                         int n_rows, const ml2_kv* prefix, const ml2_kv* cache, int page_size, const int* table, int table_stride,
+                         const int* lengths, const int* query_start, int n_requests, int max_length, int n_heads, int n_kv_heads,
+                         int head_size, float scale, void* workspace, size_t workspace_bytes);
 
 /* ---- host-buffer convenience (the same operators with the copies inside the call) ---------- */
 /* Copies `in`/`inout` (host fp16) to scratch owned by the context, runs ml2_matvec_residual_int4 on

@@ -49,3 +49,15 @@ class ConfigStruct(ctypes.Structure):
     _fields_ = [("dim", ctypes.c_int32), ("hidden_dim", ctypes.c_int32), ("n_layers", ctypes.c_int32),
                 ("n_heads", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32), ("vocab_size", ctypes.c_int32),
                 ("seq_len", ctypes.c_int32), ("rope_theta", ctypes.c_float)]
+
+
+class KVStruct(ctypes.Structure):
+    _fields_ = [("key", ctypes.c_void_p), ("value", ctypes.c_void_p), ("row_stride", ctypes.c_longlong), ("rows", ctypes.c_longlong)]
+
+
+def declare(function, arguments):
+    """Sets the argument types of a C entry: p pointer, i int, l long long / size_t, f float (the context's p comes first)."""
+    kinds = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+    function.argtypes = [kinds[a] for a in arguments.replace(" ", "")]
+    function.restype = ctypes.c_int
+    return function

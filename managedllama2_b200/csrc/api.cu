@@ -223,8 +223,8 @@ int ml2_ctx_create(int device, ml2_ctx** out)
     c->sm_count = prop.multiProcessorCount;
     c->stream = nullptr;
     c->pdl = false;
-    if ((e = cudaMalloc(&c->status_dev, sizeof(DeviceStatus))) != cudaSuccess ||
-        (e = cudaMemset(c->status_dev, 0, sizeof(DeviceStatus))) != cudaSuccess) {
+    if ((e = cudaMalloc(&c->status_dev, 2 * sizeof(DeviceStatus))) != cudaSuccess ||
+        (e = cudaMemset(c->status_dev, 0, 2 * sizeof(DeviceStatus))) != cudaSuccess) {
         delete c;
         return fail(ML2_E_CUDA, "status word: %s", cudaGetErrorString(e));
     }
@@ -275,14 +275,24 @@ int ml2_ctx_status(ml2_ctx* h, unsigned* error, unsigned* detail)
     Ctx* c = reinterpret_cast<Ctx*>(h);
     if (!c) return fail(ML2_E_INVALID, "null context");
     if (int rc = use_device(c)) return rc;
-    DeviceStatus st{};
-    cudaError_t e = cudaMemcpyAsync(&st, c->status_dev, sizeof(st), cudaMemcpyDeviceToHost, c->stream);
+    DeviceStatus both[2] = {};
+    cudaError_t e = cudaMemcpyAsync(both, c->status_dev, sizeof(both), cudaMemcpyDeviceToHost, c->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
-    if (e == cudaSuccess && st.error) e = cudaMemsetAsync(c->status_dev, 0, sizeof(st), c->stream);
+    const DeviceStatus& st = both[0].error ? both[0] : both[1];
+    if (e == cudaSuccess && st.error) e = cudaMemsetAsync(c->status_dev, 0, sizeof(both), c->stream);
     if (e != cudaSuccess) return fail(ML2_E_CUDA, "status: %s", cudaGetErrorString(e));
     if (error) *error = st.error;
     if (detail) *detail = st.detail;
-    return st.error ? fail(ML2_E_DEVICE, "a kernel gave up waiting (code %u, tile %u)", st.error, st.detail) : ML2_OK;
+    if (both[0].error) return fail(ML2_E_DEVICE, "a kernel gave up waiting (code %u, tile %u)", st.error, st.detail);
+    switch (st.error) {
+    case 0: return ML2_OK;
+    case kInputFreeCount: return fail(ML2_E_DEVICE, "block_tables: the count of free pages was %d", (int)st.detail);
+    case kInputFreeOverflow: return fail(ML2_E_DEVICE, "block_tables: %u pages given back overflow the free stack", st.detail);
+    case kInputPage: return fail(ML2_E_DEVICE, "a page of request %u lies outside the cache", st.detail);
+    case kInputSlot: return fail(ML2_E_DEVICE, "the slot of token %u lies outside the cache", st.detail);
+    case kInputLength: return fail(ML2_E_DEVICE, "the length or the query rows of request %u are out of range", st.detail);
+    default: return fail(ML2_E_DEVICE, "input error %u (%u)", st.error, st.detail);
+    }
 }
 long long ml2_ctx_launch_count(ml2_ctx* h) { return h ? reinterpret_cast<Ctx*>(h)->launches : 0; }
 

@@ -17,10 +17,25 @@ struct DeviceStatus {
     unsigned int detail;
 };
 
+// What an operator that reads indices from device tables found wrong in them (second status word of the context). The
+// first finding is kept; the element is left out (its row, token or page counts as absent) and the kernel goes on.
+enum InputError : unsigned int {
+    kInputFreeCount = 0x101,     // count of the free pages outside 0..n_pages; detail = the count
+    kInputFreeOverflow = 0x102,  // more pages given back than the free stack holds; detail = pages given back
+    kInputPage = 0x103,          // page number outside the cache; detail = request
+    kInputSlot = 0x104,          // slot outside the cache; detail = token
+    kInputLength = 0x105,        // length above max_length or negative, or query rows out of order; detail = request
+};
+
 __host__ __device__ constexpr int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // ---- shared-memory addresses -------------------------------------------------------------
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void report_input_error(DeviceStatus* st, unsigned int code, int detail)
+{
+    if (atomicCAS(&st->error, 0u, code) == 0u) st->detail = (unsigned int)detail;
+}
 
 // ---- mbarrier ----------------------------------------------------------------------------
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count)

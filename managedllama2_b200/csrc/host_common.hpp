@@ -15,7 +15,7 @@ struct Ctx {
     int sm_count = 0;
     cudaStream_t stream = nullptr;
     bool pdl = false;
-    DeviceStatus* status_dev = nullptr;
+    DeviceStatus* status_dev = nullptr;   // [0] waits that ran out, [1] invalid indices met by an operator
     void* scratch = nullptr;          // host-buffer entry points stage their vectors here
     size_t scratch_bytes = 0;
     long long launches = 0;
@@ -40,6 +40,24 @@ int fail(int code, const char* fmt, ...);
 int use_device(const Ctx* ctx);
 int plan_matvec(const Ctx* ctx, Fmt fmt, Epi epi, int rows, int cols, int nmat, MatVecPlan* pl);
 int launch_matvec(Ctx* ctx, Fmt fmt, Epi epi, Pro pro, const MatVecPlan& pl, MatVecParams prm, bool pdl);
+
+// What an operator finds wrong in device tables goes here: apart from the waits' word, which stops the persistent kernel.
+inline DeviceStatus* input_status(const Ctx* ctx) { return ctx->status_dev + 1; }
+
+constexpr int kMaxPageSize = 1024;
+constexpr int kMaxRequests = 8192;
+// log2 of a page size, -1 when it is not a power of two in 1..kMaxPageSize
+inline int page_shift(int page_size)
+{
+    for (int s = 0; (1 << s) <= kMaxPageSize; ++s)
+        if (page_size == (1 << s)) return s;
+    return -1;
+}
+template <typename... P>
+inline bool aligned_to(size_t bytes, const P*... p)
+{
+    return ((reinterpret_cast<uintptr_t>(p) | ...) & (bytes - 1)) == 0;
+}
 
 // sampling chain (sampler.cu): Sampler.Sample for temperature != 0 on `st`; the logits are consumed in place
 int sampler_chain(cudaStream_t st, int device, void* logits, int* indices, int size, float temperature, float top_p, float coin, int* tokens,

@@ -266,3 +266,149 @@ class SampleTopP(Module):
     def Forward(self, logits, indices, size, threshold, tokens, nextPos):
         _lib.check(self.lib.ml2_sample_top_p(self.ctx.handle, _ptr(logits), _ptr(indices), size, ctypes.c_float(threshold),
                                              _ptr(tokens), nextPos))
+
+
+# ---- batched decoding over a paged cache: no counterpart in the reference, which decodes one sequence ------------------------
+
+_types = {}  # torch's own, fetched at the first call: importing this package does not import torch
+
+
+def _type(name):
+    if name not in _types:
+        import torch
+        _types[name] = getattr(torch, name)
+    return _types[name]
+
+
+def _dtype_code(t, what):
+    if t.dtype is _type("float16"):
+        return 0  # ML2_F16
+    if t.dtype is _type("bfloat16"):
+        return 1  # ML2_BF16
+    raise ValueError("%s: type %s is neither float16 nor bfloat16" % (what, t.dtype))
+
+
+def _rows(ctx, what, t, width, dtype):
+    """Checks a [rows][width] tensor whose rows may be apart (a slice of columns); returns the row stride in elements."""
+    if t.dtype is not dtype or t.get_device() != ctx.device:
+        raise ValueError("%s: expected %s on cuda:%d, got %s on %s" % (what, dtype, ctx.device, t.dtype, t.device))
+    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and width != 1):
+        raise ValueError("%s: expected [rows][%d] with neighbouring columns, got %s with strides %s" % (what, width, tuple(t.shape), t.stride()))
+    return t.stride(0) if t.shape[0] > 1 else max(width, t.stride(0))
+
+
+def _ints(ctx, what, t, count):
+    """Checks a contiguous int32 tensor of at least `count` entries; returns its device pointer."""
+    if t.dtype is not _type("int32") or t.get_device() != ctx.device or not t.is_contiguous() or t.numel() < count:
+        raise ValueError("%s: expected a contiguous int32 tensor of at least %d entries on cuda:%d, got %s %s on %s"
+                         % (what, count, ctx.device, tuple(t.shape), t.dtype, t.device))
+    return t.data_ptr()
+
+
+class BlockTables(Module):
+    """Block tables and slot maps of a batch from its request lengths (``ml2_block_tables``). All arrays are int32.
+
+    ``table`` is [requests][pages of the longest request], ``freePages`` the stack of free pages with room for every page of
+    the cache, ``slots`` and ``positions`` have one entry for every row of the step's token buffer."""
+
+    def __init__(self, cudaContext, pageSize):
+        super().__init__(cudaContext)
+        self.pageSize = pageSize
+        self._call = _lib.declare(self.lib.ml2_block_tables, "ppp ii pi ppi ppppp i p i")
+
+    def Forward(self, lengths, newLengths, table, freePages, freeCount, lengthsOut, freeCountOut, queryStart, slots, positions, refused,
+                positionOffset=0):
+        c, n = self.ctx, newLengths.numel()
+        if table.dim() != 2 or table.shape[0] != n:
+            raise ValueError("table: expected [%d][pages], got %s" % (n, tuple(table.shape)))
+        rows = slots.numel()
+        _lib.check(self._call(c.handle, _ints(c, "lengths", lengths, n), _ints(c, "newLengths", newLengths, n), n, self.pageSize,
+                              _ints(c, "table", table, 1), table.shape[1], _ints(c, "freePages", freePages, 1),
+                              _ints(c, "freeCount", freeCount, 1), freePages.numel(), _ints(c, "lengthsOut", lengthsOut, n),
+                              _ints(c, "freeCountOut", freeCountOut, 1), _ints(c, "queryStart", queryStart, n + 1),
+                              _ints(c, "slots", slots, rows), _ints(c, "positions", positions, rows), rows,
+                              _ints(c, "refused", refused, n), positionOffset))
+
+
+class QKNormRoPE(Module):
+    """Norm of query and key heads, rotation and cache write of a batch of tokens (``ml2_qk_norm_rope``).
+
+    ``query``, ``key`` and ``value`` are [tokens][heads * headSize] and may be columns of one tensor; the caches are
+    [rows][numKVHeads * headSize]. ``queryWeight`` and ``keyWeight`` are None for models without head norms."""
+
+    def __init__(self, cudaContext, config, rotarySize=None):
+        super().__init__(cudaContext)
+        self.numHeads, self.numKVHeads, self.theta = config.numHeads, config.numKVHeads, config.ropeTheta
+        self.headSize = config.dim // config.numHeads
+        self.rotarySize = self.headSize if rotarySize is None else rotarySize
+        self._call = _lib.declare(self.lib.ml2_qk_norm_rope, "p i pl p pl pl pl pp pp iiiii ff")
+
+    def Forward(self, queryOutput, keyCache, valueCache, query, key, value, queryWeight, keyWeight, positions, slots, eps=1e-5):
+        c, dtype, n = self.ctx, query.dtype, query.shape[0]
+        code, width, kvWidth = _dtype_code(query, "query"), self.numHeads * self.headSize, self.numKVHeads * self.headSize
+        qs, ks, vs = _rows(c, "query", query, width, dtype), _rows(c, "key", key, kvWidth, dtype), _rows(c, "value", value, kvWidth, dtype)
+        os, cs = _rows(c, "queryOutput", queryOutput, width, dtype), _rows(c, "keyCache", keyCache, kvWidth, dtype)
+        if _rows(c, "valueCache", valueCache, kvWidth, dtype) != cs or valueCache.shape[0] != keyCache.shape[0]:
+            raise ValueError("keyCache and valueCache must have the same rows and strides")
+        if key.shape[0] != n or value.shape[0] != n or queryOutput.shape[0] < n:
+            raise ValueError("query, key, value and queryOutput must have the same rows")
+        weights = [0, 0]
+        for i, (name, w) in enumerate((("queryWeight", queryWeight), ("keyWeight", keyWeight))):
+            if w is not None:
+                if w.dtype is not dtype or w.get_device() != c.device or not w.is_contiguous() or w.numel() != self.headSize:
+                    raise ValueError("%s: expected %d contiguous %s on cuda:%d" % (name, self.headSize, dtype, c.device))
+                weights[i] = w.data_ptr()
+        cache = _lib.KVStruct(keyCache.data_ptr(), valueCache.data_ptr(), cs, keyCache.shape[0])
+        _lib.check(self._call(c.handle, code, queryOutput.data_ptr(), os, ctypes.addressof(cache), query.data_ptr(), qs, key.data_ptr(), ks,
+                              value.data_ptr(), vs, weights[0], weights[1], _ints(c, "positions", positions, n), _ints(c, "slots", slots, n),
+                              n, self.numHeads, self.numKVHeads, self.headSize, self.rotarySize, self.theta, eps))
+
+
+class PrefixAttention(Module):
+    """Attention of a batch that shares a prefix (``ml2_prefix_attention``).
+
+    ``prefixKey`` and ``prefixValue`` are the shared rows, [length][numKVHeads * headSize] (a slice of a ``Transformer``'s own
+    caches will do; None: nothing is shared), ``keyCache`` and ``valueCache`` the pages of all requests."""
+
+    def __init__(self, cudaContext, config, pageSize):
+        super().__init__(cudaContext)
+        self.numHeads, self.numKVHeads, self.pageSize = config.numHeads, config.numKVHeads, pageSize
+        self.headSize = config.dim // config.numHeads
+        self._size = _lib.declare(self.lib.ml2_prefix_attention_workspace, "p iiiiiii p")
+        self._call = _lib.declare(self.lib.ml2_prefix_attention, "p i pl p pl i pp i pi pp ii iii f pl")
+
+    def WorkspaceBytes(self, rows, requests, prefixLength, maxLength):
+        """Size of the workspace for a call of these sizes or smaller ones; calls that may overlap need one each."""
+        n = ctypes.c_size_t()
+        _lib.check(self._size(self.ctx.handle, rows, requests, prefixLength, maxLength, self.numHeads, self.numKVHeads, self.headSize,
+                              ctypes.addressof(n)))
+        return n.value
+
+    def Forward(self, output, query, prefixKey, prefixValue, keyCache, valueCache, table, lengths, queryStart, workspace, maxLength,
+                lse=None, scale=None):
+        c, dtype, n = self.ctx, query.dtype, lengths.numel()
+        code, width, kvWidth, rows = _dtype_code(query, "query"), self.numHeads * self.headSize, self.numKVHeads * self.headSize, query.shape[0]
+        qs, os, cs = _rows(c, "query", query, width, dtype), _rows(c, "output", output, width, dtype), _rows(c, "keyCache", keyCache, kvWidth, dtype)
+        if _rows(c, "valueCache", valueCache, kvWidth, dtype) != cs or valueCache.shape[0] != keyCache.shape[0]:
+            raise ValueError("keyCache and valueCache must have the same rows and strides")
+        if output.shape[0] < rows or table.dim() != 2 or table.shape[0] != n:
+            raise ValueError("output needs %d rows and table %d; got %d and %s" % (rows, n, output.shape[0], tuple(table.shape)))
+        prefix = _lib.KVStruct(0, 0, kvWidth, 0)
+        if prefixKey is not None and prefixKey.shape[0] > 0:
+            ps = _rows(c, "prefixKey", prefixKey, kvWidth, dtype)
+            if _rows(c, "prefixValue", prefixValue, kvWidth, dtype) != ps or prefixValue.shape[0] != prefixKey.shape[0]:
+                raise ValueError("prefixKey and prefixValue must have the same rows and strides")
+            prefix = _lib.KVStruct(prefixKey.data_ptr(), prefixValue.data_ptr(), ps, prefixKey.shape[0])
+        lsePtr = 0
+        if lse is not None:
+            if lse.dtype is not _type("float32") or lse.get_device() != c.device or not lse.is_contiguous() or lse.numel() < rows * self.numHeads:
+                raise ValueError("lse: expected contiguous float32 [%d][%d] on cuda:%d" % (rows, self.numHeads, c.device))
+            lsePtr = lse.data_ptr()
+        if workspace.get_device() != c.device or not workspace.is_contiguous():
+            raise ValueError("workspace: expected a contiguous tensor on cuda:%d" % c.device)
+        cache = _lib.KVStruct(keyCache.data_ptr(), valueCache.data_ptr(), cs, keyCache.shape[0])
+        _lib.check(self._call(c.handle, code, output.data_ptr(), os, lsePtr, query.data_ptr(), qs, rows, ctypes.addressof(prefix),
+                              ctypes.addressof(cache), self.pageSize, _ints(c, "table", table, 1), table.shape[1],
+                              _ints(c, "lengths", lengths, n), _ints(c, "queryStart", queryStart, n + 1), n, maxLength, self.numHeads,
+                              self.numKVHeads, self.headSize, self.headSize ** -0.5 if scale is None else scale, workspace.data_ptr(),
+                              workspace.numel() * workspace.element_size()))
