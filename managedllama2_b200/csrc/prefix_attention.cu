@@ -19,65 +19,509 @@ struct AttnBatch {
     const void *q, *pk, *pv, *k, *v;
     const int *table, *lengths, *query_start;
     DeviceStatus* status;
+    float* part_o;      // [splits][n_rows][n_heads][head]: sum of exp2(score - m) v over the keys of one split
+    float2* part_ml;    // [splits][n_rows][n_heads]: m (largest score, in powers of two) and l = sum of exp2(score - m)
     long long out_stride, q_stride, prefix_stride, cache_stride;
-    int n_requests, n_rows, prefix, max_length, n_slots, table_stride, page_shift, n_heads, n_kv;
-    float scale;
+    int n_requests, n_rows, prefix, max_length, n_pages, table_stride, page_shift, n_heads, n_kv, group;
+    int prefix_chunk, prefix_splits, own_chunk, own_splits;  // keys of a split (multiples of 16) and the most of them
+    float scale_log2;   // scale * log2(e)
 };
 
-// One warp per (row, head): four dims per lane (head 128) or two (64), one key at a time.
+// Query rows [first, first + count) and own tokens of request r; a request whose entries cannot be has none of either.
+struct Span {
+    int first, count, length;
+    bool good;
+};
+__device__ __forceinline__ Span request_span(const AttnBatch& p, int r)
+{
+    const int a = p.query_start[r], b = p.query_start[r + 1], length = p.lengths[r];
+    const bool good = a >= 0 && b >= a && b <= p.n_rows && length >= 0 && length <= p.max_length;
+    return good ? Span{a, b - a, length, true} : Span{0, 0, 0, false};
+}
+
+constexpr int kTile = 16;      // keys of a tile: the k of one m16n8k16 product with the values
+constexpr int kStages = 3;     // tiles of a warp's ring
+constexpr int kAttnWarps = 4;
+constexpr int kAttnThreads = 32 * kAttnWarps;
+
+template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+// 16 bytes to shared memory without passing registers; `bytes` 0 writes zeros and reads nothing
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// One piece of work of a warp: up to 16 rows (query row, head of the group) of one key head against a run of keys.
+struct Unit {
+    int request;            // -1: the prefix
+    int kvh, row0, rows;    // rows: of the 16, counted over (query, head of the group); row0: first of them in the request
+    int first, count;       // the request's query rows
+    int length;             // own tokens (prefix rows)
+    int key0, key1;
+    int split;
+};
+
+// Rows of a request that has `count` queries, counted 16 at a time.
+__device__ __forceinline__ int row_tiles(const AttnBatch& p, int count) { return (count * p.group + 15) >> 4; }
+
+__device__ __forceinline__ Unit decode_unit(const AttnBatch& p, const int* s_units, int total_rows, int u)
+{
+    Unit w{};
+    const int own = s_units[p.n_requests];
+    int chunk;
+    if (u >= own) {
+        u -= own;
+        w.request = -1;
+        w.first = 0;
+        w.count = total_rows;
+        w.length = p.prefix;
+        chunk = p.prefix_chunk;
+    } else {
+        int lo = 0, hi = p.n_requests - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (s_units[mid + 1] > u) hi = mid;
+            else lo = mid + 1;
+        }
+        u -= s_units[lo];
+        const Span s = request_span(p, lo);
+        w.request = lo;
+        w.first = s.first;
+        w.count = s.count;
+        w.length = s.length;
+        chunk = p.own_chunk;
+    }
+    const int tiles = row_tiles(p, w.count);
+    // key heads next to one another in the cache go to neighbouring warps, then row tiles that read the same keys
+    w.kvh = u % p.n_kv;
+    u /= p.n_kv;
+    w.row0 = (u % tiles) * 16;
+    w.split = u / tiles;
+    w.rows = min(16, w.count * p.group - w.row0);
+    w.key0 = w.split * chunk;
+    w.key1 = min(w.key0 + chunk, w.length);
+    if (w.request >= 0) {
+        // the last row of the tile sees the most
+        const int last = (w.row0 + w.rows - 1) / p.group;
+        w.key1 = min(w.key1, w.length - w.count + last + 1);
+        w.split += p.prefix_splits;
+    }
+    return w;
+}
+
+// Every warp works for itself: it takes units at a fixed stride, streams their keys and values through a ring of its own
+// (cp.async, the next tiles of this or the following unit are under way while one is used) and leaves a partial result.
+// 16 rows are all the tensor core's m16 has, so a tile of 16 keys (8 KB at head 128) costs 32 products however few rows
+// are real; at one row HBM still bounds it.
 template <typename T, int kHead>
-__global__ void __launch_bounds__(128) prefix_attention_kernel(const AttnBatch p)
+__global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const __grid_constant__ AttnBatch p)
+{
+    constexpr int kRowBytes = kHead * 2, kChunks = kHead / 8, kTileBytes = kTile * kRowBytes, kSteps = kHead / 16;
+    extern __shared__ __align__(128) unsigned char s_mem[];
+    __shared__ unsigned s_valid[kAttnWarps][kStages];
+    __shared__ int s_sum[kAttnWarps + 1];
+    int* s_units = reinterpret_cast<int*>(s_mem + kAttnWarps * kStages * 2 * kTileBytes);  // units before request r
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    // ---- how many units every request has ---------------------------------------------------------------------------
+    {
+        const int per = ceil_div(p.n_requests, kAttnThreads), r0 = min((int)threadIdx.x * per, p.n_requests), r1 = min(r0 + per, p.n_requests);
+        int mine = 0;
+        for (int r = r0; r < r1; ++r) {
+            const Span s = request_span(p, r);
+            if (!s.good && blockIdx.x == 0) report_input_error(p.status, kInputLength, r);
+            s_units[r] = mine;
+            mine += row_tiles(p, s.count) * ceil_div(s.length, p.own_chunk) * p.n_kv;
+        }
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) s_sum[warp] = incl;
+        __syncthreads();
+        int base = incl - mine, all = 0;
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) {
+            if (w < warp) base += s_sum[w];
+            all += s_sum[w];
+        }
+        for (int r = r0; r < r1; ++r) s_units[r] += base;
+        if (threadIdx.x == 0) s_units[p.n_requests] = all;
+        __syncthreads();
+    }
+    const int total_rows = min(max(p.query_start[p.n_requests], 0), p.n_rows);
+    const int units = s_units[p.n_requests] + p.prefix_splits * row_tiles(p, total_rows) * p.n_kv;
+    const int stride = gridDim.x * kAttnWarps;
+
+    unsigned char* ring = s_mem + warp * kStages * 2 * kTileBytes;
+    const uint32_t ring_u32 = smem_u32(ring);
+    const int page_mask = (1 << p.page_shift) - 1;
+
+    // ---- where the loads stand: the next tile to ask for ----------------------------------------------------------------
+    int load_u = blockIdx.x * kAttnWarps + warp, load_key = 0;
+    Unit ld{};
+    long long row = -1;  // lanes 0..15: cache row of the tile's key `lane`, -1 for none
+    auto find_rows = [&]() {
+        const int key = load_key + (lane & 15);
+        row = -1;
+        if (key < ld.key1) {
+            if (ld.request < 0) row = key;
+            else {
+                const int page = p.table[(long long)ld.request * p.table_stride + (key >> p.page_shift)];
+                if (page >= 0 && page < p.n_pages) row = ((long long)page << p.page_shift) + (key & page_mask);
+                else report_input_error(p.status, kInputPage, ld.request);
+            }
+        }
+    };
+    auto open_unit = [&]() {
+        while (load_u < units) {
+            ld = decode_unit(p, s_units, total_rows, load_u);
+            if (ld.key0 < ld.key1) break;
+            load_u += stride;
+        }
+        load_key = ld.key0;
+        if (load_u < units) find_rows();
+    };
+    auto load_tile = [&](int stage) {
+        if (load_u < units) {
+            const T* kb = static_cast<const T*>(ld.request < 0 ? p.pk : p.k) + (long long)ld.kvh * kHead;
+            const T* vb = static_cast<const T*>(ld.request < 0 ? p.pv : p.v) + (long long)ld.kvh * kHead;
+            const long long step = ld.request < 0 ? p.prefix_stride : p.cache_stride;
+            const unsigned valid = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+            if (lane == 0) s_valid[warp][stage] = valid;
+            const uint32_t dst = ring_u32 + stage * 2 * kTileBytes;
+#pragma unroll
+            for (int i = 0; i < kChunks / 2; ++i) {
+                const int at = i * 32 + lane, key = at / kChunks, c = at % kChunks;
+                const long long r = __shfl_sync(0xffffffffu, row, key);
+                const long long off = r < 0 ? 0 : r * step + c * 8;
+                const uint32_t to = dst + key * kRowBytes + ((c ^ (key & 7)) << 4);
+                cp_async16(to, kb + off, r < 0 ? 0 : 16);
+                cp_async16(to + kTileBytes, vb + off, r < 0 ? 0 : 16);
+            }
+            load_key += kTile;
+            if (load_key < ld.key1) find_rows();
+            else {
+                load_u += stride;
+                open_unit();
+            }
+        }
+        cp_async_commit();
+    };
+
+    open_unit();
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) load_tile(i);
+
+    int stage = 0;
+    const int g = lane >> 2, t4 = lane & 3;
+    for (int u = blockIdx.x * kAttnWarps + warp; u < units; u += stride) {
+        const Unit w = decode_unit(p, s_units, total_rows, u);
+        if (w.key0 >= w.key1) continue;
+
+        // rows g and g + 8 of the tile: query row, head, and the keys they see
+        const int m0 = w.row0 + g, m1 = m0 + 8;
+        const bool live0 = g < w.rows, live1 = g + 8 < w.rows;
+        const int i0 = m0 / p.group, i1 = m1 / p.group;
+        const int h0 = w.kvh * p.group + m0 % p.group, h1 = w.kvh * p.group + m1 % p.group;
+        const int seen0 = w.request < 0 ? w.length : w.length - w.count + i0 + 1, seen1 = w.request < 0 ? w.length : w.length - w.count + i1 + 1;
+        const bool causal = w.request >= 0 && w.count > 1;
+
+        uint32_t qf[kSteps][4];
+        {
+            const T* q0 = static_cast<const T*>(p.q) + (long long)(w.first + i0) * p.q_stride + (long long)h0 * kHead + t4 * 2;
+            const T* q1 = static_cast<const T*>(p.q) + (long long)(w.first + i1) * p.q_stride + (long long)h1 * kHead + t4 * 2;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                qf[k][0] = live0 ? *reinterpret_cast<const uint32_t*>(q0 + k * 16) : 0u;
+                qf[k][1] = live1 ? *reinterpret_cast<const uint32_t*>(q1 + k * 16) : 0u;
+                qf[k][2] = live0 ? *reinterpret_cast<const uint32_t*>(q0 + k * 16 + 8) : 0u;
+                qf[k][3] = live1 ? *reinterpret_cast<const uint32_t*>(q1 + k * 16 + 8) : 0u;
+            }
+        }
+        float acc[kHead / 8][4];
+#pragma unroll
+        for (int n = 0; n < kHead / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        float mx0 = -INFINITY, mx1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+        for (int key = w.key0; key < w.key1; key += kTile) {
+            cp_async_wait<kStages - 2>();
+            __syncwarp();
+            const uint32_t kt = ring_u32 + stage * 2 * kTileBytes, vt = kt + kTileBytes;
+            const unsigned valid = s_valid[warp][stage];
+
+            float s[2][4] = {};
+            {
+                const int kr = (lane & 7) + ((lane >> 4) & 1) * 8, kc = (lane >> 3) & 1;
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    uint32_t b[4];
+                    ldsm4(b, kt + kr * kRowBytes + (((2 * k + kc) ^ (kr & 7)) << 4));
+                    mma16816<T>(s[0], qf[k], b[0], b[1]);
+                    mma16816<T>(s[1], qf[k], b[2], b[3]);
+                }
+            }
+            const bool masked = valid != 0xffffu || (causal && key + kTile > w.length - w.count + 1);
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[n][e] *= p.scale_log2;
+                    if (masked) {
+                        const int j = n * 8 + t4 * 2 + (e & 1);
+                        if (!((valid >> j) & 1u) || key + j >= (e < 2 ? seen0 : seen1)) s[n][e] = -INFINITY;
+                    }
+                }
+            float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+            float t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
+            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
+            const float n0 = fmaxf(mx0, t0), n1 = fmaxf(mx1, t1);
+            const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
+            if (__any_sync(0xffffffffu, n0 > mx0 || n1 > mx1)) {  // a larger score: what was summed shrinks
+                const float c0 = exp2_fast(mx0 - b0), c1 = exp2_fast(mx1 - b1);
+                l0 *= c0;
+                l1 *= c1;
+#pragma unroll
+                for (int n = 0; n < kHead / 8; ++n) {
+                    acc[n][0] *= c0;
+                    acc[n][1] *= c0;
+                    acc[n][2] *= c1;
+                    acc[n][3] *= c1;
+                }
+                mx0 = n0;
+                mx1 = n1;
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                s[n][0] = exp2_fast(s[n][0] - b0);
+                s[n][1] = exp2_fast(s[n][1] - b0);
+                s[n][2] = exp2_fast(s[n][2] - b1);
+                s[n][3] = exp2_fast(s[n][3] - b1);
+                l0 += s[n][0] + s[n][1];
+                l1 += s[n][2] + s[n][3];
+            }
+            if (masked && causal) {
+                // Weight 0 times a value that is not finite would be NaN in the rows that do not see its key. Such keys are
+                // taken out of the product and added to the rows that see them one by one.
+                unsigned odd = 0;
+                for (int j = 0; j < kTile; ++j) {
+                    bool bad = false;
+                    for (int c = lane; c < kHead / 2; c += 32) {
+                        const uint32_t at = vt + j * kRowBytes + ((((c >> 2) ^ (j & 7)) << 4) | ((c & 3) << 2));
+                        uint32_t v;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+                        const float2 f = unpack2<T>(v);
+                        bad |= !isfinite(f.x) || !isfinite(f.y);
+                    }
+                    if (__any_sync(0xffffffffu, bad)) odd |= 1u << j;
+                }
+                for (unsigned left = odd; left; left &= left - 1) {
+                    const int j = __ffs(left) - 1, n = j >> 3, src = (lane & ~3) | ((j & 7) >> 1);
+                    const float pa = (j & 1) ? s[n][1] : s[n][0], pb = (j & 1) ? s[n][3] : s[n][2];
+                    const float p0 = __shfl_sync(0xffffffffu, pa, src), p1 = __shfl_sync(0xffffffffu, pb, src);
+                    const bool in0 = key + j < seen0, in1 = key + j < seen1;
+#pragma unroll
+                    for (int d = 0; d < kHead / 8; ++d) {
+                        const uint32_t at = vt + j * kRowBytes + (((d ^ (j & 7)) << 4) | (t4 << 2));
+                        uint32_t v;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+                        const float2 f = unpack2<T>(v);
+                        if (in0) { acc[d][0] += p0 * f.x; acc[d][1] += p0 * f.y; }
+                        if (in1) { acc[d][2] += p1 * f.x; acc[d][3] += p1 * f.y; }
+                    }
+                }
+                if (odd) {
+                    __syncwarp();
+                    for (unsigned left = odd; left; left &= left - 1) {
+                        const int j = __ffs(left) - 1;
+                        for (int c = lane; c < kHead / 2; c += 32)
+                            asm volatile("st.shared.u32 [%0], %1;" ::"r"(vt + j * kRowBytes + c * 4), "r"(0u) : "memory");
+                    }
+                    __syncwarp();
+                }
+            }
+            // weights of at most 1, rounded to 16 bits for the product: the same half step the output's own rounding costs
+            const uint32_t pf[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]), pack2<T>(s[1][2], s[1][3])};
+            {
+                const int vr = (lane & 7) + ((lane >> 3) & 1) * 8, vc = lane >> 4;
+#pragma unroll
+                for (int d = 0; d < kHead / 16; ++d) {
+                    uint32_t b[4];
+                    ldsm4_t(b, vt + vr * kRowBytes + (((2 * d + vc) ^ (vr & 7)) << 4));
+                    mma16816<T>(acc[2 * d], pf, b[0], b[1]);
+                    mma16816<T>(acc[2 * d + 1], pf, b[2], b[3]);
+                }
+            }
+            __syncwarp();  // everybody has read the tile that the next load writes over one turn from now
+            load_tile(stage == 0 ? kStages - 1 : stage - 1);
+            stage = stage == kStages - 1 ? 0 : stage + 1;
+        }
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        const long long at0 = ((long long)w.split * p.n_rows + w.first + i0) * p.n_heads + h0;
+        const long long at1 = ((long long)w.split * p.n_rows + w.first + i1) * p.n_heads + h1;
+        if (live0) {
+            if (t4 == 0) p.part_ml[at0] = make_float2(mx0, l0);
+#pragma unroll
+            for (int n = 0; n < kHead / 8; ++n) *reinterpret_cast<float2*>(p.part_o + at0 * kHead + n * 8 + t4 * 2) = make_float2(acc[n][0], acc[n][1]);
+        }
+        if (live1) {
+            if (t4 == 0) p.part_ml[at1] = make_float2(mx1, l1);
+#pragma unroll
+            for (int n = 0; n < kHead / 8; ++n) *reinterpret_cast<float2*>(p.part_o + at1 * kHead + n * 8 + t4 * 2) = make_float2(acc[n][2], acc[n][3]);
+        }
+    }
+    cp_async_wait<0>();
+}
+
+// Joins the partial results of one row and head: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. One warp each.
+template <typename T, int kHead>
+__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttnBatch p)
 {
     constexpr int kPer = kHead / 32;
+    pdl_wait();
     const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    const int t = (int)(id / p.n_heads), h = (int)(id % p.n_heads), hk = h / (p.n_heads / p.n_kv);
+    const int t = (int)(id / p.n_heads), h = (int)(id % p.n_heads);
     if (t >= p.n_rows || t >= p.query_start[p.n_requests]) return;
-    int r = 0;
-    while (r < p.n_requests - 1 && p.query_start[r + 1] <= t) ++r;
-    const int queries = p.query_start[r + 1] - p.query_start[r];
-    int length = p.lengths[r];
-    if (lane == 0 && (length < 0 || length > p.max_length || p.query_start[r] < 0 || queries < 0 || queries > p.n_rows))
-        report_input_error(p.status, kInputLength, r);
-    length = min(length, p.max_length);
-    const int seen = max(0, min(length, length - queries + (t - p.query_start[r]) + 1));
-    const T* q = static_cast<const T*>(p.q) + t * p.q_stride + (long long)h * kHead + lane * kPer;
-    float qf[kPer], acc[kPer] = {};
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) qf[e] = (float)q[e] * p.scale;
-    float m = -INFINITY, l = 0.f;
-    for (long long j = -(long long)p.prefix; j < seen; ++j) {
-        const T *k, *v;
-        if (j < 0) {
-            const long long at = (j + p.prefix) * p.prefix_stride + (long long)hk * kHead + lane * kPer;
-            k = static_cast<const T*>(p.pk) + at;
-            v = static_cast<const T*>(p.pv) + at;
-        } else {
-            const int page = p.table[(long long)r * p.table_stride + (j >> p.page_shift)];
-            if (page < 0 || page >= (p.n_slots >> p.page_shift)) {
-                if (lane == 0) report_input_error(p.status, kInputPage, r);
-                continue;
-            }
-            const long long slot = ((long long)page << p.page_shift) + (j & ((1 << p.page_shift) - 1));
-            const long long at = slot * p.cache_stride + (long long)hk * kHead + lane * kPer;
-            k = static_cast<const T*>(p.k) + at;
-            v = static_cast<const T*>(p.v) + at;
-        }
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) s += qf[e] * (float)k[e];
-        s = warp_sum(s);
-        const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-        const float c = expf(m - base), w = expf(s - base);
-        l = l * c + w;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[e] = acc[e] * c + (w == 0.f ? 0.f : w * (float)v[e]);
-        m = mn;
+    int lo = 0, hi = p.n_requests - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (p.query_start[mid + 1] > t) hi = mid;
+        else lo = mid + 1;
     }
-    T* o = static_cast<T*>(p.out) + t * p.out_stride + (long long)h * kHead + lane * kPer;
+    const Span s = request_span(p, lo);
+    const int seen = s.good ? min(s.length, max(0, s.length - s.count + (t - s.first) + 1)) : 0;
+    const int own = ceil_div(seen, p.own_chunk), splits = p.prefix_splits + own;
+    const long long step = (long long)p.n_rows * p.n_heads;
+
+    float m = -INFINITY, l = 0.f, acc[kPer] = {};
+    for (int base = 0; base < splits; base += 32) {
+        const int mine = base + lane;
+        const float2 ml = mine < splits ? p.part_ml[mine * step + id] : make_float2(-INFINITY, 0.f);
+        const float mn = fmaxf(m, warp_max(ml.x)), to = mn == -INFINITY ? 0.f : mn;
+        const float c = exp2_fast(m - to), w = exp2_fast(ml.x - to);
+        l = l * c + warp_sum(ml.y * w);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) o[e] = (T)(l == 0.f ? 0.f : acc[e] / l);
-    if (p.lse && lane == 0) p.lse[(long long)t * p.n_heads + h] = l == 0.f ? -INFINITY : m + logf(l);
+        for (int e = 0; e < kPer; ++e) acc[e] *= c;
+        m = mn;
+        const int here = min(32, splits - base);
+        for (int i = 0; i < here; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float* o = p.part_o + ((base + i) * step + id) * kHead + lane * kPer;
+            if constexpr (kPer == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(o);
+                acc[0] += wi * v.x; acc[1] += wi * v.y; acc[2] += wi * v.z; acc[3] += wi * v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(o);
+                acc[0] += wi * v.x; acc[1] += wi * v.y;
+            }
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* o = static_cast<T*>(p.out) + t * p.out_stride + (long long)h * kHead + lane * kPer;
+    if constexpr (kPer == 4)
+        *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
+    else
+        *reinterpret_cast<uint32_t*>(o) = pack2<T>(acc[0] * inv, acc[1] * inv);
+    if (p.lse && lane == 0) p.lse[id] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+}
+
+// How the keys are cut. Own tokens: pieces of at most 256 keys, and smaller ones (32 at least) where whole requests would
+// not give every warp of the machine four pieces. The prefix likewise.
+struct AttnPlan {
+    int prefix_chunk, prefix_splits, own_chunk, own_splits, grid;
+    long long units;
+    size_t o_bytes, bytes;
+};
+static void cut(int length, long long pieces_of_one_split, int warps, int* chunk, int* splits)
+{
+    *chunk = kTile;
+    *splits = 0;
+    if (length == 0) return;
+    long long n = std::max<long long>(ceil_div(length, 256), (4ll * warps + pieces_of_one_split - 1) / pieces_of_one_split);
+    n = std::min<long long>(n, std::min(64, ceil_div(length, 32)));
+    *chunk = ceil_div(ceil_div(length, (int)n), kTile) * kTile;
+    *splits = ceil_div(length, *chunk);
+}
+static AttnPlan plan_attention(const Ctx* ctx, int n_rows, int n_requests, int prefix, int max_length, int n_heads, int n_kv, int head)
+{
+    AttnPlan pl{};
+    const int warps = 2 * ctx->sm_count * kAttnWarps, group = n_heads / n_kv;
+    const long long own_tiles = n_requests + (long long)n_rows * group / 16, prefix_tiles = ((long long)n_rows * group + 15) / 16;
+    cut(prefix, prefix_tiles * n_kv, warps, &pl.prefix_chunk, &pl.prefix_splits);
+    cut(max_length, own_tiles * n_kv, warps, &pl.own_chunk, &pl.own_splits);
+    pl.units = (own_tiles * pl.own_splits + prefix_tiles * pl.prefix_splits) * n_kv;
+    pl.grid = (int)std::min<long long>(2 * ctx->sm_count, std::max<long long>(1, (pl.units + kAttnWarps - 1) / kAttnWarps));
+    const size_t rows = (size_t)(pl.prefix_splits + pl.own_splits) * n_rows * n_heads;
+    pl.o_bytes = rows * head * sizeof(float);
+    pl.bytes = pl.o_bytes + rows * sizeof(float2);
+    return pl;
+}
+
+template <typename T, int kHead>
+static cudaError_t launch_attention(Ctx* ctx, const AttnBatch& p, const AttnPlan& pl)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(pl.grid);
+    cfg.blockDim = dim3(kAttnThreads);
+    cfg.dynamicSmemBytes = kAttnWarps * kStages * 2 * kTile * kHead * 2 + (p.n_requests + 1) * sizeof(int);
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctx->pdl ? 1 : 0;
+    cudaError_t e = cudaFuncSetAttribute(attention_units_kernel<T, kHead>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, attention_units_kernel<T, kHead>, p);
+    if (e != cudaSuccess) return e;
+    ++ctx->launches;
+    // the join starts while the last units finish and waits for them itself
+    cfg.gridDim = dim3((unsigned)(((long long)p.n_rows * p.n_heads + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, attention_join_kernel<T, kHead>, p);
+    if (e == cudaSuccess) ++ctx->launches;
+    return e;
 }
 
 static int check_sizes(const char* what, int n_rows, int n_requests, int prefix, int max_length, int n_heads, int n_kv, int head_size)
@@ -102,7 +546,7 @@ int ml2_prefix_attention_workspace(ml2_ctx* h, int n_rows, int n_requests, int p
 {
     if (!h || !bytes) return fail(ML2_E_INVALID, "prefix_attention_workspace: null argument");
     if (int rc = check_sizes("prefix_attention_workspace", n_rows, n_requests, prefix_length, max_length, n_heads, n_kv_heads, head_size)) return rc;
-    *bytes = 0;
+    *bytes = plan_attention(reinterpret_cast<Ctx*>(h), n_rows, n_requests, prefix_length, max_length, n_heads, n_kv_heads, head_size).bytes;
     return ML2_OK;
 }
 
@@ -134,21 +578,26 @@ int ml2_prefix_attention(ml2_ctx* h, int dtype, void* out, long long out_stride,
         !aligned_to(16, prefix->key, prefix->value, workspace))
         return fail(ML2_E_INVALID, "prefix_attention: pointers must be 16-byte aligned and row strides multiples of 8 elements");
     if (out == query) return fail(ML2_E_INVALID, "prefix_attention: out must not overlap the queries");
+    const AttnPlan pl = plan_attention(ctx, n_rows, n_requests, (int)prefix->rows, max_length, n_heads, n_kv_heads, head_size);
+    if (pl.units > INT32_MAX - (1 << 20) || (long long)n_rows * n_heads > INT32_MAX)
+        return fail(ML2_E_INVALID, "prefix_attention: n_rows=%d with %d heads is too much for one call", n_rows, n_heads);
+    if (workspace_bytes < pl.bytes || (pl.bytes && !workspace))
+        return fail(ML2_E_INVALID, "prefix_attention: the workspace has %zu bytes, %zu are needed", workspace_bytes, pl.bytes);
     if (int rc = use_device(ctx)) return rc;
     AttnBatch p{};
     p.out = out; p.lse = lse; p.q = query; p.pk = prefix->key; p.pv = prefix->value; p.k = cache->key; p.v = cache->value;
     p.table = table; p.lengths = lengths; p.query_start = query_start; p.status = input_status(ctx);
     p.out_stride = out_stride; p.q_stride = query_stride; p.prefix_stride = prefix->row_stride; p.cache_stride = cache->row_stride;
-    p.n_requests = n_requests; p.n_rows = n_rows; p.prefix = (int)prefix->rows; p.max_length = max_length; p.n_slots = (int)cache->rows;
-    p.table_stride = table_stride; p.page_shift = shift; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.scale = scale;
-    const unsigned grid = (unsigned)(((long long)n_rows * n_heads + 3) / 4);
-    if (dtype == ML2_F16 && head_size == 128) prefix_attention_kernel<__half, 128><<<grid, 128, 0, ctx->stream>>>(p);
-    if (dtype == ML2_F16 && head_size == 64) prefix_attention_kernel<__half, 64><<<grid, 128, 0, ctx->stream>>>(p);
-    if (dtype == ML2_BF16 && head_size == 128) prefix_attention_kernel<__nv_bfloat16, 128><<<grid, 128, 0, ctx->stream>>>(p);
-    if (dtype == ML2_BF16 && head_size == 64) prefix_attention_kernel<__nv_bfloat16, 64><<<grid, 128, 0, ctx->stream>>>(p);
-    const cudaError_t e = cudaGetLastError();
+    p.n_requests = n_requests; p.n_rows = n_rows; p.prefix = (int)prefix->rows; p.max_length = max_length; p.n_pages = (int)(cache->rows >> shift);
+    p.table_stride = table_stride; p.page_shift = shift; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.group = n_heads / n_kv_heads;
+    p.scale_log2 = scale * 1.44269504088896340736f;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + pl.o_bytes);
+    p.prefix_chunk = pl.prefix_chunk; p.prefix_splits = pl.prefix_splits; p.own_chunk = pl.own_chunk; p.own_splits = pl.own_splits;
+    cudaError_t e;
+    if (head_size == 128) e = dtype == ML2_F16 ? launch_attention<__half, 128>(ctx, p, pl) : launch_attention<__nv_bfloat16, 128>(ctx, p, pl);
+    else e = dtype == ML2_F16 ? launch_attention<__half, 64>(ctx, p, pl) : launch_attention<__nv_bfloat16, 64>(ctx, p, pl);
     if (e != cudaSuccess) return fail(ML2_E_CUDA, "prefix_attention: %s", cudaGetErrorString(e));
-    ++ctx->launches;
     return ML2_OK;
 }
 
