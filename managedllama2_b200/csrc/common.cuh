@@ -17,6 +17,8 @@ struct DeviceStatus {
     unsigned int detail;
 };
 
+constexpr unsigned int kAttentionGaveUp = 0x50;  // a wait inside the prefix kernel ran out (first status word)
+
 // What an operator that reads indices from device tables found wrong in them (second status word of the context). The
 // first finding is kept; the element is left out (its row, token or page counts as absent) and the kernel goes on.
 enum InputError : unsigned int {

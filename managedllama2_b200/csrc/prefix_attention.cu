@@ -8,8 +8,10 @@
 
 #include "batch_common.cuh"
 #include "host_common.hpp"
+#include "tcgen05.cuh"
 
 #include <cmath>
+#include <type_traits>
 
 namespace ml2 {
 
@@ -19,11 +21,17 @@ struct AttnBatch {
     const void *q, *pk, *pv, *k, *v;
     const int *table, *lengths, *query_start;
     DeviceStatus* status;
-    float* part_o;      // [splits][n_rows][n_heads][head]: sum of exp2(score - m) v over the keys of one split
-    float2* part_ml;    // [splits][n_rows][n_heads]: m (largest score, in powers of two) and l = sum of exp2(score - m)
+    DeviceStatus* waits;
+    // Partial results of the prefix, [splits][rows that are there][n_heads], and of the own tokens, [splits][n_rows][n_heads]:
+    // o = sum of exp2(score - m) v over the keys of one split [head], and (m, l): a reference near the largest score (in
+    // powers of two) and l = sum of exp2(score - m). A result without keys has m = -inf, l = 0 and an o that is not read.
+    float *pre_o, *own_o;
+    float2 *pre_ml, *own_ml;
+    long long wait_cycles;
     long long out_stride, q_stride, prefix_stride, cache_stride;
     int n_requests, n_rows, prefix, max_length, n_pages, table_stride, page_shift, n_heads, n_kv, group;
-    int prefix_chunk, prefix_splits, own_chunk, own_splits;  // keys of a split (multiples of 16) and the most of them
+    int prefix_chunk, prefix_splits, own_chunk;  // keys of a split (multiples of 16); prefix_splits 0: cut by blocks instead
+    int prefix_ctas;    // of the kernel that does the prefix by blocks, 0 without it
     float scale_log2;   // scale * log2(e)
 };
 
@@ -134,7 +142,6 @@ __device__ __forceinline__ Unit decode_unit(const AttnBatch& p, const int* s_uni
         // the last row of the tile sees the most
         const int last = (w.row0 + w.rows - 1) / p.group;
         w.key1 = min(w.key1, w.length - w.count + last + 1);
-        w.split += p.prefix_splits;
     }
     return w;
 }
@@ -153,7 +160,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const 
     int* s_units = reinterpret_cast<int*>(s_mem + kAttnWarps * kStages * 2 * kTileBytes);  // units before request r
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    pdl_wait();
+    // after the prefix kernel, which has waited for what comes before both, this one starts beside it
+    if (!p.prefix_ctas) pdl_wait();
     // ---- how many units every request has ---------------------------------------------------------------------------
     {
         const int per = ceil_div(p.n_requests, kAttnThreads), r0 = min((int)threadIdx.x * per, p.n_requests), r1 = min(r0 + per, p.n_requests);
@@ -396,20 +404,374 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const 
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        const long long at0 = ((long long)w.split * p.n_rows + w.first + i0) * p.n_heads + h0;
-        const long long at1 = ((long long)w.split * p.n_rows + w.first + i1) * p.n_heads + h1;
+        const long long step = w.request < 0 ? total_rows : p.n_rows;
+        float* part_o = w.request < 0 ? p.pre_o : p.own_o;
+        float2* part_ml = w.request < 0 ? p.pre_ml : p.own_ml;
+        const long long at0 = (w.split * step + w.first + i0) * p.n_heads + h0;
+        const long long at1 = (w.split * step + w.first + i1) * p.n_heads + h1;
         if (live0) {
-            if (t4 == 0) p.part_ml[at0] = make_float2(mx0, l0);
+            if (t4 == 0) part_ml[at0] = make_float2(mx0, l0);
 #pragma unroll
-            for (int n = 0; n < kHead / 8; ++n) *reinterpret_cast<float2*>(p.part_o + at0 * kHead + n * 8 + t4 * 2) = make_float2(acc[n][0], acc[n][1]);
+            for (int n = 0; n < kHead / 8; ++n) *reinterpret_cast<float2*>(part_o + at0 * kHead + n * 8 + t4 * 2) = make_float2(acc[n][0], acc[n][1]);
         }
         if (live1) {
-            if (t4 == 0) p.part_ml[at1] = make_float2(mx1, l1);
+            if (t4 == 0) part_ml[at1] = make_float2(mx1, l1);
 #pragma unroll
-            for (int n = 0; n < kHead / 8; ++n) *reinterpret_cast<float2*>(p.part_o + at1 * kHead + n * 8 + t4 * 2) = make_float2(acc[n][2], acc[n][3]);
+            for (int n = 0; n < kHead / 8; ++n) *reinterpret_cast<float2*>(part_o + at1 * kHead + n * 8 + t4 * 2) = make_float2(acc[n][2], acc[n][3]);
         }
     }
     cp_async_wait<0>();
+    if (p.prefix_ctas) pdl_wait();  // the join follows this kernel: it may start when the prefix is done too
+}
+
+// ---- the prefix, with many rows: fifth-generation tensor core ------------------------------------------------------------
+//
+// A block is 256 rows (query row, head of the group) of one key head, as two tiles of 128; blocks x key tiles of 128 keys
+// are cut into one contiguous run per CTA, so all CTAs do the same work within one tile and a block's runs ("segments") are
+// joined afterwards. Two streams of a CTA alternate on the tensor core:
+//   S = Q K^T (operands in shared memory, S in TMEM)      while the other stream's warps do their softmax,
+//   P = exp2(S - m), rounded to 16 bits, over S in TMEM   (128 threads, one row each: no exchange between threads)
+//   O += P V (P from TMEM, V as it lies: MN-major)
+// With more than 128 rows both streams use each key tile, the first with rows 0..127, the second with 128..255. With fewer,
+// both have the same rows and take the key tiles in turn: then HBM bounds the kernel and four tiles of 32 KB are under way.
+// The reference point m of a row moves only when a score exceeds it by more than 8 (weights up to 2^8 fit fp16 with room, and
+// sums are fp32): O is rescaled in TMEM a few times in all instead of at every tile.
+constexpr int kBlockRows = 256;
+constexpr int kKeyTile = 128;
+constexpr int kRing = 4;                 // key or value tiles in shared memory
+constexpr int kBlockThreads = 320;       // 2 x 4 softmax warps, tensor core warp, load warp
+constexpr float kSlack = 8.f;
+constexpr int kBlockPrefix = 512;        // from this length on the prefix is done by blocks
+
+struct PrefixMaps {
+    CUtensorMap k, v;
+};
+struct PrefixRuns {  // how blocks and key tiles are cut, from the rows that are there: the same in both kernels
+    int rows, blocks, key_tiles, per;    // rows of a key head, blocks of them, key tiles of one block, tiles of a CTA
+    long long tiles;
+};
+__host__ __device__ __forceinline__ PrefixRuns prefix_runs(int total_rows, int group, int n_kv, int prefix, int ctas)
+{
+    PrefixRuns r{};
+    r.rows = total_rows * group;
+    r.blocks = ceil_div(r.rows, kBlockRows);
+    r.key_tiles = ceil_div(prefix, kKeyTile);
+    r.tiles = (long long)n_kv * r.blocks * r.key_tiles;
+    r.per = (int)((r.tiles + ctas - 1) / ctas);
+    return r;
+}
+// Segments of a block: the CTAs first .. last have a part of it; two results each where the streams take turns.
+__device__ __forceinline__ void block_segments(const PrefixRuns& r, int kvh, int block, int* first, int* results)
+{
+    const long long a = ((long long)kvh * r.blocks + block) * r.key_tiles;
+    *first = (int)(a / r.per);
+    const int n = (int)((a + r.key_tiles - 1) / r.per) - *first + 1;
+    *results = r.rows - block * kBlockRows <= kBlockRows / 2 ? 2 * n : n;
+}
+
+template <int kHead> struct BlockSmem {
+    static constexpr int kHalf = kKeyTile * 128;              // 64 dims of 128 rows, 128-byte swizzle
+    static constexpr int kTileBytes = kHalf * (kHead / 64);   // a tile of Q, K or V
+    static constexpr int kBytes = 1024 + (2 + kRing) * kTileBytes;
+};
+
+template <typename T, int kHead>
+__global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(const __grid_constant__ AttnBatch p, const __grid_constant__ PrefixMaps maps)
+{
+    using S = BlockSmem<kHead>;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ unsigned char s_raw[];
+    __shared__ uint64_t b_full[kRing], b_empty[kRing], b_q[2], b_s[2], b_p[2], b_o[2], b_end;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    const uint32_t base = (smem_u32(s_raw) + 1023u) & ~1023u;  // Q tile of either stream, then the ring
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kRing; ++i) {
+            mbar_init(&b_full[i], 1);
+            mbar_init(&b_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&b_q[i], 128);
+            mbar_init(&b_s[i], 1);
+            mbar_init(&b_p[i], 128);
+            mbar_init(&b_o[i], 1);
+        }
+        mbar_init(&b_end, 1);
+        s_abort = 0;
+        mbar_fence_init();
+    }
+    if (warp == 8) tmem_alloc(&s_tmem, 512);
+    pdl_wait();
+    pdl_launch_dependents();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    const int total_rows = min(max(p.query_start[p.n_requests], 0), p.n_rows);
+    const PrefixRuns runs = prefix_runs(total_rows, p.group, p.n_kv, p.prefix, gridDim.x);
+    const long long begin = min((long long)blockIdx.x * runs.per, runs.tiles), end = min(begin + runs.per, runs.tiles);
+
+    // a CTA's run, block by block: f(kvh, block, first key tile, tiles)
+    auto for_segments = [&](auto&& f) {
+        for (long long at = begin; at < end;) {
+            const long long which = at / runs.key_tiles;
+            const int tile = (int)(at - which * runs.key_tiles), n = (int)min((long long)(runs.key_tiles - tile), end - at);
+            if (!f((int)(which / runs.blocks), (int)(which % runs.blocks), tile, n)) return false;
+            at += n;
+        }
+        return true;
+    };
+    // tiles of a stream in a segment
+    auto share = [](bool turns, int n, int stream) { return turns ? (n + 1 - stream) >> 1 : n; };
+
+    if (warp == 9) {
+        // ---- loads, in the order of their first use ------------------------------------------------------------------
+        if (lane == 0) {
+            tma_prefetch_map(&maps.k);
+            tma_prefetch_map(&maps.v);
+            unsigned count = 0;
+            auto load = [&](const CUtensorMap* map, int kvh, int tile) {
+                const unsigned slot = count % kRing, turn = count / kRing;
+                if (!mbar_wait_for(&b_empty[slot], (turn & 1) ^ 1, p.wait_cycles, &s_abort)) return false;
+                mbar_arrive_expect_tx(&b_full[slot], S::kTileBytes);
+#pragma unroll
+                for (int h = 0; h < kHead / 64; ++h)
+                    tma_load_2d(base + (2 + slot) * S::kTileBytes + h * S::kHalf, map, kvh * kHead + h * 64, tile * kKeyTile, &b_full[slot]);
+                ++count;
+                return true;
+            };
+            const bool done = for_segments([&](int kvh, int block, int tile, int n) {
+                const bool turns = runs.rows - block * kBlockRows <= kBlockRows / 2;
+                if (!load(&maps.k, kvh, tile)) return false;
+                if (turns && n > 1 && !load(&maps.k, kvh, tile + 1)) return false;
+                const int ahead = turns ? 2 : 1;
+                for (int j = 0; j < n; ++j) {
+                    if (!load(&maps.v, kvh, tile + j)) return false;
+                    if (j + ahead < n && !load(&maps.k, kvh, tile + j + ahead)) return false;
+                }
+                return true;
+            });
+            if (!done) {  // copies that are under way land before this CTA leaves
+                for (unsigned c = count > kRing ? count - kRing : 0; c < count; ++c)
+                    for (int i = 0; i < 1 << 20 && !mbar_try_wait(&b_full[c % kRing], (c / kRing) & 1); ++i) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp == 8) {
+        // ---- the tensor core's queue -----------------------------------------------------------------------------------
+        if (lane == 0) {
+            constexpr uint32_t kShapeS = tc_shape(128, kKeyTile, kBf16, false), kShapeO = tc_shape(128, kHead, kBf16, true);
+            unsigned count = 0;               // ring position of the next tile to be used
+            unsigned held[2][2] = {};         // [key, value]: the position that a stream's product reads
+            unsigned turn_p[2] = {0, 0};      // P tiles a stream has handed over
+            unsigned turn_q[2] = {0, 0};      // and Q tiles
+            auto take = [&](unsigned* pos) {
+                *pos = count++;
+                return mbar_wait_for(&b_full[*pos % kRing], (*pos / kRing) & 1, p.wait_cycles, &s_abort);
+            };
+            auto scores = [&](int s, unsigned pos, bool last_use) {
+                const uint32_t q = base + s * S::kTileBytes, k = base + (2 + pos % kRing) * S::kTileBytes;
+#pragma unroll
+                for (int i = 0; i < kHead / 16; ++i) {
+                    const uint32_t off = (i / 4) * S::kHalf + (i % 4) * 32;
+                    tc_mma_ss(tmem + s * 128, tc_operand(q + off, 16, 1024), tc_operand(k + off, 16, 1024), kShapeS, i > 0);
+                }
+                if (last_use) tc_commit(&b_empty[pos % kRing]);
+                tc_commit(&b_s[s]);
+            };
+            auto values = [&](int s, unsigned pos, bool first, bool last, bool last_use) {
+                if (!mbar_wait_for(&b_p[s], turn_p[s]++ & 1, p.wait_cycles, &s_abort)) return false;
+                tc_fence_after();
+                const uint32_t v = base + (2 + pos % kRing) * S::kTileBytes;
+#pragma unroll
+                for (int i = 0; i < kKeyTile / 16; ++i)
+                    tc_mma_ts(tmem + 256 + s * 128, tmem + s * 128 + i * 8, tc_operand(v + i * 2048, S::kHalf, 1024), kShapeO, !first || i > 0);
+                if (last_use) tc_commit(&b_empty[pos % kRing]);
+                if (last) tc_commit(&b_o[s]);
+                return true;
+            };
+            const bool done = for_segments([&](int, int block, int, int n) {
+                const bool turns = runs.rows - block * kBlockRows <= kBlockRows / 2;
+                const int n0 = share(turns, n, 0), n1 = share(turns, n, 1);
+                for (int s = 0; s < 2; ++s) {
+                    // a stream without tiles hands over no Q: it could be two phases ahead of this wait otherwise
+                    if (!(s ? n1 : n0)) continue;
+                    if (!mbar_wait_for(&b_q[s], turn_q[s]++ & 1, p.wait_cycles, &s_abort)) return false;
+                    if (s == 0 || turns) {
+                        if (!take(&held[s][0])) return false;
+                    } else held[1][0] = held[0][0];
+                    tc_fence_after();
+                    scores(s, held[s][0], turns || s == 1);
+                }
+                for (int j = 0; j < n0; ++j)
+                    for (int s = 0; s < 2; ++s) {
+                        const int ns = s ? n1 : n0;
+                        if (j >= ns) continue;
+                        if (s == 0 || turns) {
+                            if (!take(&held[s][1])) return false;
+                        } else held[1][1] = held[0][1];
+                        if (!values(s, held[s][1], j == 0, j == ns - 1, turns || s == 1)) return false;
+                        if (j + 1 < ns) {
+                            if (s == 0 || turns) {
+                                if (!take(&held[s][0])) return false;
+                            } else held[1][0] = held[0][0];
+                            scores(s, held[s][0], turns || s == 1);
+                        }
+                    }
+                return true;
+            });
+            if (!done) {  // products that are under way end before the TMEM is given back
+                tc_commit(&b_end);
+                for (int i = 0; i < 1 << 20 && !mbar_try_wait(&b_end, 0); ++i) {}
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: one row a thread -----------------------------------------------------------------------------------
+        const int s = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_s = tmem + s * 128 + lanes, t_o = tmem + 256 + s * 128 + lanes;
+        const uint32_t q_tile = base + s * S::kTileBytes;
+        unsigned turn_s = 0, turn_o = 0;
+        for_segments([&](int kvh, int block, int tile, int n) {
+            const bool turns = runs.rows - block * kBlockRows <= kBlockRows / 2;
+            const int ns = share(turns, n, s);
+            const int first_row = block * kBlockRows + (turns ? 0 : s * 128), rows = min(128, runs.rows - first_row);
+            // this warp's 32 rows of Q, sixteen bytes a lane: what the stream's earlier products read is done with
+            if (ns) {
+#pragma unroll 4
+                for (int i = 0; i < 32 * kHead / 8 / 32; ++i) {
+                    const int at = i * 32 + lane, r = (warp & 3) * 32 + at / (kHead / 8), c = at % (kHead / 8), m = first_row + r;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (r < rows)
+                        v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (long long)(m / p.group) * p.q_stride +
+                                                            (long long)(kvh * p.group + m % p.group) * kHead + c * 8);
+                    const uint32_t to = q_tile + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+                }
+                fence_async_shared();
+                mbar_arrive(&b_q[s]);
+            }
+
+            const bool busy = (warp & 3) * 32 < rows;  // warps without rows only keep step
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < ns; ++j) {
+                if (!__all_sync(0xffffffffu, mbar_wait_for(&b_s[s], turn_s++ & 1, p.wait_cycles, &s_abort))) return false;
+                tc_fence_after();
+                if (busy) {
+                    uint32_t x[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, x[c]);
+                    tmem_wait_ld();
+                    const int left = p.prefix - (tile + (turns ? 2 * j + s : j)) * kKeyTile;  // keys from this tile on
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[c][e] = __float_as_uint(__uint_as_float(x[c][e]) * p.scale_log2);
+                    if (left < kKeyTile) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (c * 32 + e >= left) x[c][e] = 0xff800000u;
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(x[c][e]));
+                    const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    const bool move = t > m + kSlack || m == -INFINITY;
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float to = move ? t : m, ref = to == -INFINITY ? 0.f : to, c = move ? exp2_fast(m - ref) : 1.f;
+                        m = to;
+                        l *= c;
+                        if (j > 0) {
+                            // the products before this S are done: S was queued behind them
+#pragma unroll 1
+                            for (int d = 0; d < kHead; d += 32) {
+                                uint32_t o[32];
+                                tmem_ld32(t_o + d, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
+                                tmem_st32(t_o + d, o);
+                            }
+                        }
+                    }
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const int c = 2 * h + e / 16, f = (e % 16) * 2;
+                            const float a = exp2_fast(__uint_as_float(x[c][f]) - ref), b = exp2_fast(__uint_as_float(x[c][f + 1]) - ref);
+                            sum[e & 3] += a + b;
+                            w[e] = pack2<T>(a, b);
+                        }
+                        tmem_st32(t_s + h * 32, w);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                mbar_arrive(&b_p[s]);
+            }
+
+            // ---- the segment's result --------------------------------------------------------------------------------------
+            int first, results;
+            block_segments(runs, kvh, block, &first, &results);
+            const int split = turns ? 2 * ((int)blockIdx.x - first) + s : (int)blockIdx.x - first;
+            if (ns) {
+                if (!__all_sync(0xffffffffu, mbar_wait_for(&b_o[s], turn_o++ & 1, p.wait_cycles, &s_abort))) return false;
+                tc_fence_after();
+            }
+            if (busy) {
+                const int mrow = first_row + row, t = mrow / p.group, h = kvh * p.group + mrow % p.group;
+                if (row < rows) p.pre_ml[((long long)split * total_rows + t) * p.n_heads + h] = make_float2(m, l);
+                if (ns) {
+                    // through this warp's own 32 rows of the Q tile (other warps may have the next segment's rows in theirs), 32
+                    // dims at a time, so that rows leave in whole lines
+                    const uint32_t mine = q_tile + (warp & 3) * 32 * 128;
+#pragma unroll 1
+                    for (int d = 0; d < kHead; d += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(t_o + d, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(mine + lane * 128 + (((e >> 2) ^ (lane & 7)) << 4)), "r"(o[e]),
+                                         "r"(o[e + 1]), "r"(o[e + 2]), "r"(o[e + 3])
+                                         : "memory");
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int r = i * 4 + (lane >> 3), c = lane & 7, mm = first_row + (warp & 3) * 32 + r;
+                            uint4 v;
+                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                         : "r"(mine + r * 128 + ((c ^ (r & 7)) << 4))
+                                         : "memory");
+                            if ((warp & 3) * 32 + r < rows)
+                                *reinterpret_cast<uint4*>(p.pre_o + (((long long)split * total_rows + mm / p.group) * p.n_heads + kvh * p.group + mm % p.group) * kHead +
+                                                          d + c * 4) = v;
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+            tc_fence_before();  // O has been read before the next segment's first product, which waits for this thread's P
+            return true;
+        });
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && s_abort) atomicCAS(&p.waits->error, 0u, kAttentionGaveUp);
+    tc_fence_after();
+    if (warp == 8) tmem_free(tmem, 512);
 }
 
 // Joins the partial results of one row and head: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. One warp each.
@@ -430,13 +792,22 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     }
     const Span s = request_span(p, lo);
     const int seen = s.good ? min(s.length, max(0, s.length - s.count + (t - s.first) + 1)) : 0;
-    const int own = ceil_div(seen, p.own_chunk), splits = p.prefix_splits + own;
-    const long long step = (long long)p.n_rows * p.n_heads;
+    const int total_rows = min(p.query_start[p.n_requests], p.n_rows);
+    int pre = p.prefix_splits;
+    if (p.prefix_ctas) {
+        int first;
+        const PrefixRuns runs = prefix_runs(total_rows, p.group, p.n_kv, p.prefix, p.prefix_ctas);
+        block_segments(runs, h / p.group, (t * p.group + h % p.group) / kBlockRows, &first, &pre);
+    }
+    const int splits = pre + ceil_div(seen, p.own_chunk);
+    const long long pre_step = (long long)total_rows * p.n_heads, own_step = (long long)p.n_rows * p.n_heads;
 
     float m = -INFINITY, l = 0.f, acc[kPer] = {};
     for (int base = 0; base < splits; base += 32) {
         const int mine = base + lane;
-        const float2 ml = mine < splits ? p.part_ml[mine * step + id] : make_float2(-INFINITY, 0.f);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (mine < pre) ml = p.pre_ml[mine * pre_step + id];
+        else if (mine < splits) ml = p.own_ml[(mine - pre) * own_step + id];
         const float mn = fmaxf(m, warp_max(ml.x)), to = mn == -INFINITY ? 0.f : mn;
         const float c = exp2_fast(m - to), w = exp2_fast(ml.x - to);
         l = l * c + warp_sum(ml.y * w);
@@ -446,7 +817,9 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
         const int here = min(32, splits - base);
         for (int i = 0; i < here; ++i) {
             const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float* o = p.part_o + ((base + i) * step + id) * kHead + lane * kPer;
+            if (wi == 0.f) continue;
+            const int at = base + i;
+            const float* o = (at < pre ? p.pre_o + (at * pre_step + id) * kHead : p.own_o + ((at - pre) * own_step + id) * kHead) + lane * kPer;
             if constexpr (kPer == 4) {
                 const float4 v = *reinterpret_cast<const float4*>(o);
                 acc[0] += wi * v.x; acc[1] += wi * v.y; acc[2] += wi * v.z; acc[3] += wi * v.w;
@@ -468,9 +841,9 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
 // How the keys are cut. Own tokens: pieces of at most 256 keys, and smaller ones (32 at least) where whole requests would
 // not give every warp of the machine four pieces. The prefix likewise.
 struct AttnPlan {
-    int prefix_chunk, prefix_splits, own_chunk, own_splits, grid;
+    int prefix_chunk, prefix_splits, own_chunk, own_splits, grid, prefix_ctas;
     long long units;
-    size_t o_bytes, bytes;
+    size_t pre_o, own_o, pre_ml, own_ml, bytes;  // offsets into the workspace, and its size
 };
 static void cut(int length, long long pieces_of_one_split, int warps, int* chunk, int* splits)
 {
@@ -487,40 +860,87 @@ static AttnPlan plan_attention(const Ctx* ctx, int n_rows, int n_requests, int p
     AttnPlan pl{};
     const int warps = 2 * ctx->sm_count * kAttnWarps, group = n_heads / n_kv;
     const long long own_tiles = n_requests + (long long)n_rows * group / 16, prefix_tiles = ((long long)n_rows * group + 15) / 16;
-    cut(prefix, prefix_tiles * n_kv, warps, &pl.prefix_chunk, &pl.prefix_splits);
+    long long pre_rows = 0;
+    if (prefix >= kBlockPrefix && n_rows) {
+        const long long blocks = ((long long)n_rows * group + kBlockRows - 1) / kBlockRows, key_tiles = ceil_div(prefix, kKeyTile);
+        pl.prefix_ctas = (int)std::min<long long>(std::max(1, ctx->sm_count), blocks * n_kv * key_tiles);
+        // Any number of rows up to n_rows may be there. With b blocks of a key head a CTA has at least n_kv b key_tiles / ctas
+        // tiles, a block at most ctas / (n_kv b) + 2 segments and never more than key tiles, and a segment two results.
+        pre_rows = std::min(512ll * pl.prefix_ctas + 1024ll * blocks * n_kv, 2ll * key_tiles * n_rows * n_heads);
+        pl.prefix_chunk = kTile;
+    } else {
+        cut(prefix, prefix_tiles * n_kv, warps, &pl.prefix_chunk, &pl.prefix_splits);
+        pre_rows = (long long)pl.prefix_splits * n_rows * n_heads;
+    }
     cut(max_length, own_tiles * n_kv, warps, &pl.own_chunk, &pl.own_splits);
     pl.units = (own_tiles * pl.own_splits + prefix_tiles * pl.prefix_splits) * n_kv;
-    pl.grid = (int)std::min<long long>(2 * ctx->sm_count, std::max<long long>(1, (pl.units + kAttnWarps - 1) / kAttnWarps));
-    const size_t rows = (size_t)(pl.prefix_splits + pl.own_splits) * n_rows * n_heads;
-    pl.o_bytes = rows * head * sizeof(float);
-    pl.bytes = pl.o_bytes + rows * sizeof(float2);
+    pl.grid = (int)std::min<long long>(2 * ctx->sm_count, (pl.units + kAttnWarps - 1) / kAttnWarps);
+    const size_t own_rows = (size_t)pl.own_splits * n_rows * n_heads;
+    pl.own_o = (size_t)pre_rows * head * sizeof(float);
+    pl.pre_ml = pl.own_o + own_rows * head * sizeof(float);
+    pl.own_ml = pl.pre_ml + (size_t)pre_rows * sizeof(float2);
+    pl.bytes = pl.own_ml + own_rows * sizeof(float2);
     return pl;
 }
 
-template <typename T, int kHead>
-static cudaError_t launch_attention(Ctx* ctx, const AttnBatch& p, const AttnPlan& pl)
+// Tensor map of the prefix's keys or values: boxes of 64 columns and kKeyTile rows in 128-byte swizzle, rows behind the end
+// read as zeros.
+static bool make_map(CUtensorMap* map, int dtype, const void* base, long long row_stride, int columns, int rows)
 {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(pl.grid);
-    cfg.blockDim = dim3(kAttnThreads);
-    cfg.dynamicSmemBytes = kAttnWarps * kStages * 2 * kTile * kHead * 2 + (p.n_requests + 1) * sizeof(int);
-    cfg.stream = ctx->stream;
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found);
+        return e == cudaSuccess && found == cudaDriverEntryPointSuccess ? reinterpret_cast<Encode>(f) : nullptr;
+    }();
+    if (!encode) return false;
+    const cuuint64_t size[2] = {(cuuint64_t)columns, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)row_stride * 2};
+    const cuuint32_t box[2] = {64, kKeyTile}, step[2] = {1, 1};
+    return encode(map, dtype == ML2_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), size, stride,
+                  box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int kHead>
+static cudaError_t launch_attention(Ctx* ctx, const AttnBatch& p, const AttnPlan& pl, const PrefixMaps& maps)
+{
+    static bool ready[16] = {};  // shared-memory limits are set once per device
+    cudaError_t e = cudaSuccess;
+    if (!ready[ctx->device & 15]) {
+        e = cudaFuncSetAttribute(attention_units_kernel<T, kHead>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_prefix_kernel<T, kHead>, cudaFuncAttributeMaxDynamicSharedMemorySize, BlockSmem<kHead>::kBytes);
+        if (e != cudaSuccess) return e;
+        ready[ctx->device & 15] = true;
+    }
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.stream = ctx->stream;
     cfg.attrs = attr;
     cfg.numAttrs = ctx->pdl ? 1 : 0;
-    cudaError_t e = cudaFuncSetAttribute(attention_units_kernel<T, kHead>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, attention_units_kernel<T, kHead>, p);
-    if (e != cudaSuccess) return e;
-    ++ctx->launches;
-    // the join starts while the last units finish and waits for them itself
+    if (pl.prefix_ctas) {
+        cfg.gridDim = dim3(pl.prefix_ctas);
+        cfg.blockDim = dim3(kBlockThreads);
+        cfg.dynamicSmemBytes = BlockSmem<kHead>::kBytes;
+        if ((e = cudaLaunchKernelEx(&cfg, attention_prefix_kernel<T, kHead>, p, maps)) != cudaSuccess) return e;
+        ++ctx->launches;
+        cfg.numAttrs = 1;  // what follows starts as this kernel's CTAs leave
+    }
+    if (pl.grid) {
+        cfg.gridDim = dim3(pl.grid);
+        cfg.blockDim = dim3(kAttnThreads);
+        cfg.dynamicSmemBytes = kAttnWarps * kStages * 2 * kTile * kHead * 2 + (p.n_requests + 1) * sizeof(int);
+        if ((e = cudaLaunchKernelEx(&cfg, attention_units_kernel<T, kHead>, p)) != cudaSuccess) return e;
+        ++ctx->launches;
+        cfg.numAttrs = 1;
+    }
     cfg.gridDim = dim3((unsigned)(((long long)p.n_rows * p.n_heads + 3) / 4));
     cfg.blockDim = dim3(128);
     cfg.dynamicSmemBytes = 0;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, attention_join_kernel<T, kHead>, p);
-    if (e == cudaSuccess) ++ctx->launches;
+    if ((e = cudaLaunchKernelEx(&cfg, attention_join_kernel<T, kHead>, p)) == cudaSuccess) ++ctx->launches;
     return e;
 }
 
@@ -591,12 +1011,18 @@ int ml2_prefix_attention(ml2_ctx* h, int dtype, void* out, long long out_stride,
     p.n_requests = n_requests; p.n_rows = n_rows; p.prefix = (int)prefix->rows; p.max_length = max_length; p.n_pages = (int)(cache->rows >> shift);
     p.table_stride = table_stride; p.page_shift = shift; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.group = n_heads / n_kv_heads;
     p.scale_log2 = scale * 1.44269504088896340736f;
-    p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + pl.o_bytes);
-    p.prefix_chunk = pl.prefix_chunk; p.prefix_splits = pl.prefix_splits; p.own_chunk = pl.own_chunk; p.own_splits = pl.own_splits;
+    char* ws = static_cast<char*>(workspace);
+    p.pre_o = reinterpret_cast<float*>(ws + pl.pre_o); p.own_o = reinterpret_cast<float*>(ws + pl.own_o);
+    p.pre_ml = reinterpret_cast<float2*>(ws + pl.pre_ml); p.own_ml = reinterpret_cast<float2*>(ws + pl.own_ml);
+    p.prefix_chunk = pl.prefix_chunk; p.prefix_splits = pl.prefix_splits; p.own_chunk = pl.own_chunk; p.prefix_ctas = pl.prefix_ctas;
+    p.waits = ctx->status_dev; p.wait_cycles = ctx->wait_cycles;
+    PrefixMaps maps{};
+    if (pl.prefix_ctas && (!make_map(&maps.k, dtype, prefix->key, prefix->row_stride, (int)kv_width, p.prefix) ||
+                           !make_map(&maps.v, dtype, prefix->value, prefix->row_stride, (int)kv_width, p.prefix)))
+        return fail(ML2_E_CUDA, "prefix_attention: no tensor map for a prefix of %d rows of %lld, stride %lld", p.prefix, kv_width, prefix->row_stride);
     cudaError_t e;
-    if (head_size == 128) e = dtype == ML2_F16 ? launch_attention<__half, 128>(ctx, p, pl) : launch_attention<__nv_bfloat16, 128>(ctx, p, pl);
-    else e = dtype == ML2_F16 ? launch_attention<__half, 64>(ctx, p, pl) : launch_attention<__nv_bfloat16, 64>(ctx, p, pl);
+    if (head_size == 128) e = dtype == ML2_F16 ? launch_attention<__half, 128>(ctx, p, pl, maps) : launch_attention<__nv_bfloat16, 128>(ctx, p, pl, maps);
+    else e = dtype == ML2_F16 ? launch_attention<__half, 64>(ctx, p, pl, maps) : launch_attention<__nv_bfloat16, 64>(ctx, p, pl, maps);
     if (e != cudaSuccess) return fail(ML2_E_CUDA, "prefix_attention: %s", cudaGetErrorString(e));
     return ML2_OK;
 }

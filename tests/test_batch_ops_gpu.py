@@ -24,6 +24,7 @@ def step(dtype):
 @pytest.fixture(scope="module")
 def ctx():
     c = ml2.CudaContext(0)
+    c.set_wait_limit(2 * 10**9)  # about a second: a wait that never ends is an error status, not ten seconds
     yield c
     c.close()
 
@@ -415,6 +416,22 @@ def test_attention_single_tokens(ctx, dtype, head, heads, kv, prefix):
 @pytest.mark.parametrize("prefix", [1, 15, 16, 17, 31, 32, 33, 64, 65, 127, 128, 129, 255, 256, 257, 511, 1025, 4032])
 def test_attention_prefix_lengths(ctx, prefix):
     Batch(prefix, "fp16", 4, 2, 128, 16, prefix, [3, 20], [1, 1]).check(ctx)
+
+
+@pytest.mark.parametrize("heads,kv,head,prefix,requests", [
+    (40, 40, 128, 4032, 1), (40, 40, 128, 4032, 64), (5, 5, 128, 513, 3), (37, 37, 64, 640, 2), (16, 2, 128, 2048, 16), (16, 2, 128, 2049, 17),
+    (24, 3, 64, 1111, 33), (8, 1, 64, 9000, 65), (64, 64, 64, 600, 130), (3, 1, 128, 700, 300), (12, 12, 128, 1500, 257)])
+def test_attention_prefix_in_blocks(ctx, heads, kv, head, prefix, requests):
+    """Runs of key tiles that begin and end anywhere in a head, blocks of up to 128, 129..256 and more rows; called twenty
+    times over without waiting."""
+    lengths, _ = ragged(prefix + requests, requests, 30, 1)
+    b = Batch(prefix + heads, "fp16" if heads % 2 else "bf16", heads, kv, head, 16, prefix, lengths, [1] * requests, extra_rows=2)
+    first, z = b.check(ctx)
+    op = ml2.PrefixAttention(ctx, b.cfg, 16)
+    ws = torch.full((op.WorkspaceBytes(b.q.shape[0], requests, prefix, 30),), 0xFF, dtype=torch.uint8, device="cuda")
+    results = [b.call(ctx, workspace=ws, max_length=30) for _ in range(20)]
+    for out, lse in results:
+        assert torch.equal(out, first) and torch.equal(lse, z)
 
 
 @pytest.mark.parametrize("page", [1, 2, 8, 16, 32, 64, 128, 1024])
