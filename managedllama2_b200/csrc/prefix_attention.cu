@@ -426,20 +426,20 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const 
 
 // ---- the prefix, with many rows: fifth-generation tensor core ------------------------------------------------------------
 //
-// A block is 256 rows (query row, head of the group) of one key head, as two tiles of 128; blocks x key tiles of 128 keys
-// are cut into one contiguous run per CTA, so all CTAs do the same work within one tile and a block's runs ("segments") are
+// A block is 256 rows (query row, head of the group) of one key head, as two tiles of 128; blocks x key tiles of 64 keys are
+// cut into one contiguous run per CTA, so all CTAs do the same work within one tile and a block's runs ("segments") are
 // joined afterwards. Two streams of a CTA alternate on the tensor core:
-//   S = Q K^T (operands in shared memory, S in TMEM)      while the other stream's warps do their softmax,
+//   S = Q K^T (operands in shared memory, S in TMEM, two of them a stream: one is filled while the other is used),
 //   P = exp2(S - m), rounded to 16 bits, over S in TMEM   (128 threads, one row each: no exchange between threads)
 //   O += P V (P from TMEM, V as it lies: MN-major)
 // With more than 128 rows both streams use each key tile, the first with rows 0..127, the second with 128..255. With fewer,
-// both have the same rows and take the key tiles in turn: then HBM bounds the kernel and four tiles of 32 KB are under way.
+// both have the same rows and take the key tiles in turn: then HBM bounds the kernel and eight tiles of 16 KB are under way.
 // The reference point m of a row moves only when a score exceeds it by more than 8 (weights up to 2^8 fit fp16 with room, and
 // sums are fp32): O is rescaled in TMEM a few times in all instead of at every tile.
 constexpr int kBlockRows = 256;
-constexpr int kKeyTile = 128;
-constexpr int kRing = 4;                 // key or value tiles in shared memory
-constexpr int kBlockThreads = 320;       // 2 x 4 softmax warps, tensor core warp, load warp
+constexpr int kKeyTile = 64;
+constexpr int kRing = 8;                 // key or value tiles in shared memory
+constexpr int kBlockThreads = 352;       // per stream 4 softmax warps and one that feeds the tensor core; load warp
 constexpr float kSlack = 8.f;
 constexpr int kBlockPrefix = 512;        // from this length on the prefix is done by blocks
 
@@ -470,10 +470,26 @@ __device__ __forceinline__ void block_segments(const PrefixRuns& r, int kvh, int
 }
 
 template <int kHead> struct BlockSmem {
-    static constexpr int kHalf = kKeyTile * 128;              // 64 dims of 128 rows, 128-byte swizzle
-    static constexpr int kTileBytes = kHalf * (kHead / 64);   // a tile of Q, K or V
-    static constexpr int kBytes = 1024 + (2 + kRing) * kTileBytes;
+    static constexpr int kQHalf = 128 * 128, kQBytes = kQHalf * (kHead / 64);            // 64 dims of 128 rows, 128-byte swizzle
+    static constexpr int kHalf = kKeyTile * 128, kTileBytes = kHalf * (kHead / 64);      // 64 dims of a key or value tile
+    static constexpr int kBytes = 1024 + 2 * kQBytes + kRing * kTileBytes;
 };
+
+// a * b + c, a + b on two fp32 values at once
+__device__ __forceinline__ uint64_t two(float x, float y) { return (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x); }
+__device__ __forceinline__ float2 apart(uint64_t v) { return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 
 template <typename T, int kHead>
 __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(const __grid_constant__ AttnBatch p, const __grid_constant__ PrefixMaps maps)
@@ -481,34 +497,40 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
     using S = BlockSmem<kHead>;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ unsigned char s_raw[];
-    __shared__ uint64_t b_full[kRing], b_empty[kRing], b_q[2], b_s[2], b_p[2], b_o[2], b_end;
+    __shared__ uint64_t b_full[kRing], b_empty[kRing], b_q[2], b_s[2][2], b_p[2][2], b_o[2][2], b_end[2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    const uint32_t base = (smem_u32(s_raw) + 1023u) & ~1023u;  // Q tile of either stream, then the ring
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t q_base = (smem_u32(s_raw) + 1023u) & ~1023u, ring = q_base + 2 * S::kQBytes;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // uniform, and known to be
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kRing; ++i) {
             mbar_init(&b_full[i], 1);
-            mbar_init(&b_empty[i], 1);
+            mbar_init(&b_empty[i], 2);  // one from each stream
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&b_q[i], 128);
-            mbar_init(&b_s[i], 1);
-            mbar_init(&b_p[i], 128);
-            mbar_init(&b_o[i], 1);
+            mbar_init(&b_end[i], 1);
+            mbar_init(&b_q[i], 4);  // one arrival a warp
+            for (int j = 0; j < 2; ++j) {
+                mbar_init(&b_o[i][j], 1);
+                mbar_init(&b_s[i][j], 1);
+                mbar_init(&b_p[i][j], 4);
+            }
         }
-        mbar_init(&b_end, 1);
         s_abort = 0;
         mbar_fence_init();
     }
     if (warp == 8) tmem_alloc(&s_tmem, 512);
+    if (warp == 10 && lane == 0) {
+        tma_prefetch_map(&maps.k);
+        tma_prefetch_map(&maps.v);
+    }
     pdl_wait();
     pdl_launch_dependents();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = s_tmem;  // columns: S of stream 0 (2 x 64), of stream 1, O of stream 0 (128), of stream 1
 
     const int total_rows = min(max(p.query_start[p.n_requests], 0), p.n_rows);
     const PrefixRuns runs = prefix_runs(total_rows, p.group, p.n_kv, p.prefix, gridDim.x);
@@ -527,11 +549,9 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
     // tiles of a stream in a segment
     auto share = [](bool turns, int n, int stream) { return turns ? (n + 1 - stream) >> 1 : n; };
 
-    if (warp == 9) {
+    if (warp == 10) {
         // ---- loads, in the order of their first use ------------------------------------------------------------------
         if (lane == 0) {
-            tma_prefetch_map(&maps.k);
-            tma_prefetch_map(&maps.v);
             unsigned count = 0;
             auto load = [&](const CUtensorMap* map, int kvh, int tile) {
                 const unsigned slot = count % kRing, turn = count / kRing;
@@ -539,19 +559,20 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                 mbar_arrive_expect_tx(&b_full[slot], S::kTileBytes);
 #pragma unroll
                 for (int h = 0; h < kHead / 64; ++h)
-                    tma_load_2d(base + (2 + slot) * S::kTileBytes + h * S::kHalf, map, kvh * kHead + h * 64, tile * kKeyTile, &b_full[slot]);
+                    tma_load_2d(ring + slot * S::kTileBytes + h * S::kHalf, map, kvh * kHead + h * 64, tile * kKeyTile, &b_full[slot]);
                 ++count;
                 return true;
             };
             const bool done = for_segments([&](int kvh, int block, int tile, int n) {
-                const bool turns = runs.rows - block * kBlockRows <= kBlockRows / 2;
-                if (!load(&maps.k, kvh, tile)) return false;
-                if (turns && n > 1 && !load(&maps.k, kvh, tile + 1)) return false;
-                const int ahead = turns ? 2 : 1;
-                for (int j = 0; j < n; ++j) {
-                    if (!load(&maps.v, kvh, tile + j)) return false;
-                    if (j + ahead < n && !load(&maps.k, kvh, tile + j + ahead)) return false;
-                }
+                const int step = runs.rows - block * kBlockRows <= kBlockRows / 2 ? 2 : 1;
+                auto loads = [&](const CUtensorMap* map, int j) {
+                    for (int t = j * step; t < min(n, (j + 1) * step); ++t)
+                        if (!load(map, kvh, tile + t)) return false;
+                    return true;
+                };
+                if (!loads(&maps.k, 0)) return false;
+                for (int j = 0; j * step < n; ++j)
+                    if (!loads(&maps.k, j + 1) || !loads(&maps.v, j)) return false;
                 return true;
             });
             if (!done) {  // copies that are under way land before this CTA leaves
@@ -560,136 +581,156 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
             }
         }
         __syncwarp();
-    } else if (warp == 8) {
-        // ---- the tensor core's queue -----------------------------------------------------------------------------------
+    } else if (warp >= 8) {
+        // ---- the tensor core's queue, one thread for each stream ------------------------------------------------------
+        // (One for both was slower than the products: its own instructions, some 700 cycles for the eight or four products of
+        // a tile, bounded the kernel.)
         if (lane == 0) {
             constexpr uint32_t kShapeS = tc_shape(128, kKeyTile, kBf16, false), kShapeO = tc_shape(128, kHead, kBf16, true);
-            unsigned count = 0;               // ring position of the next tile to be used
-            unsigned held[2][2] = {};         // [key, value]: the position that a stream's product reads
-            unsigned turn_p[2] = {0, 0};      // P tiles a stream has handed over
-            unsigned turn_q[2] = {0, 0};      // and Q tiles
-            auto take = [&](unsigned* pos) {
-                *pos = count++;
-                return mbar_wait_for(&b_full[*pos % kRing], (*pos / kRing) & 1, p.wait_cycles, &s_abort);
-            };
-            auto scores = [&](int s, unsigned pos, bool last_use) {
-                const uint32_t q = base + s * S::kTileBytes, k = base + (2 + pos % kRing) * S::kTileBytes;
-#pragma unroll
-                for (int i = 0; i < kHead / 16; ++i) {
-                    const uint32_t off = (i / 4) * S::kHalf + (i % 4) * 32;
-                    tc_mma_ss(tmem + s * 128, tc_operand(q + off, 16, 1024), tc_operand(k + off, 16, 1024), kShapeS, i > 0);
-                }
-                if (last_use) tc_commit(&b_empty[pos % kRing]);
-                tc_commit(&b_s[s]);
-            };
-            auto values = [&](int s, unsigned pos, bool first, bool last, bool last_use) {
-                if (!mbar_wait_for(&b_p[s], turn_p[s]++ & 1, p.wait_cycles, &s_abort)) return false;
-                tc_fence_after();
-                const uint32_t v = base + (2 + pos % kRing) * S::kTileBytes;
-#pragma unroll
-                for (int i = 0; i < kKeyTile / 16; ++i)
-                    tc_mma_ts(tmem + 256 + s * 128, tmem + s * 128 + i * 8, tc_operand(v + i * 2048, S::kHalf, 1024), kShapeO, !first || i > 0);
-                if (last_use) tc_commit(&b_empty[pos % kRing]);
-                if (last) tc_commit(&b_o[s]);
-                return true;
-            };
+            const int s = warp - 8;
+            const uint32_t q_op = tc_operand_low(q_base + s * S::kQBytes, 16), k_op = tc_operand_low(ring, 16), v_op = tc_operand_low(ring, S::kHalf);
+            const uint32_t t_s = tmem + s * 128, t_o = tmem + 256 + s * 128;
+            unsigned count = 0;               // ring position of the next tile
+            unsigned asked = 0, added = 0;    // S tiles queued since the start, and P tiles used
+            unsigned turn_q = 0;              // Q tiles taken
             const bool done = for_segments([&](int, int block, int, int n) {
                 const bool turns = runs.rows - block * kBlockRows <= kBlockRows / 2;
-                const int n0 = share(turns, n, 0), n1 = share(turns, n, 1);
-                for (int s = 0; s < 2; ++s) {
-                    // a stream without tiles hands over no Q: it could be two phases ahead of this wait otherwise
-                    if (!(s ? n1 : n0)) continue;
-                    if (!mbar_wait_for(&b_q[s], turn_q[s]++ & 1, p.wait_cycles, &s_abort)) return false;
-                    if (s == 0 || turns) {
-                        if (!take(&held[s][0])) return false;
-                    } else held[1][0] = held[0][0];
-                    tc_fence_after();
-                    scores(s, held[s][0], turns || s == 1);
-                }
-                for (int j = 0; j < n0; ++j)
-                    for (int s = 0; s < 2; ++s) {
-                        const int ns = s ? n1 : n0;
-                        if (j >= ns) continue;
-                        if (s == 0 || turns) {
-                            if (!take(&held[s][1])) return false;
-                        } else held[1][1] = held[0][1];
-                        if (!values(s, held[s][1], j == 0, j == ns - 1, turns || s == 1)) return false;
-                        if (j + 1 < ns) {
-                            if (s == 0 || turns) {
-                                if (!take(&held[s][0])) return false;
-                            } else held[1][0] = held[0][0];
-                            scores(s, held[s][0], turns || s == 1);
+                const int step = turns ? 2 : 1;
+                // Step j's key or value tiles, in the order of their loads. Each stream looks at every tile, and lets go at once
+                // of one that is the other's: who skipped a tile could take an earlier phase of its barrier for a later one.
+                auto visit = [&](int j, auto&& use) {
+                    for (int t = j * step; t < min(n, (j + 1) * step); ++t) {
+                        const unsigned slot = count % kRing, parity = (count / kRing) & 1;
+                        ++count;
+                        if (!mbar_wait_for(&b_full[slot], parity, p.wait_cycles, &s_abort)) return false;
+                        if (turns && (t & 1) != s) mbar_arrive(&b_empty[slot]);
+                        else {
+                            if (!use(slot)) return false;
+                            tc_commit(&b_empty[slot]);
                         }
                     }
+                    return true;
+                };
+                auto scores = [&](unsigned slot) {
+                    tc_fence_after();
+                    const uint32_t k = k_op + slot * (S::kTileBytes >> 4), to = t_s + (asked & 1) * 64;
+#pragma unroll
+                    for (int i = 0; i < kHead / 16; ++i)
+                        tc_mma_ss(to, tc_operand_at(q_op + (i / 4) * (S::kQHalf >> 4) + (i % 4) * 2), tc_operand_at(k + (i / 4) * (S::kHalf >> 4) + (i % 4) * 2),
+                                  kShapeS, i > 0);
+                    tc_commit(&b_s[s][asked++ & 1]);
+                    return true;
+                };
+                bool first = true;
+                auto values = [&](unsigned slot) {
+                    if (!mbar_wait_for(&b_p[s][added & 1], (added >> 1) & 1, p.wait_cycles, &s_abort)) return false;
+                    tc_fence_after();
+                    const uint32_t v = v_op + slot * (S::kTileBytes >> 4), from = t_s + (added & 1) * 64;
+                    tc_mma_ts(t_o, from, tc_operand_at(v), kShapeO, !first);
+#pragma unroll
+                    for (int k = 1; k < kKeyTile / 16; ++k) tc_mma_ts(t_o, from + k * 8, tc_operand_at(v + k * (2048 >> 4)), kShapeO, 1);
+                    tc_commit(&b_o[s][added++ & 1]);
+                    first = false;
+                    return true;
+                };
+                // a stream without tiles hands over no Q: it could be two phases ahead of this wait otherwise
+                if (share(turns, n, s) && !mbar_wait_for(&b_q[s], turn_q++ & 1, p.wait_cycles, &s_abort)) return false;
+                if (!visit(0, scores)) return false;
+                // S of the next step goes where P of the one before lay: behind the product that reads it
+                for (int j = 0; j * step < n; ++j)
+                    if (!visit(j + 1, scores) || !visit(j, values)) return false;
                 return true;
             });
             if (!done) {  // products that are under way end before the TMEM is given back
-                tc_commit(&b_end);
-                for (int i = 0; i < 1 << 20 && !mbar_try_wait(&b_end, 0); ++i) {}
+                tc_commit(&b_end[s]);
+                for (int i = 0; i < 1 << 20 && !mbar_try_wait(&b_end[s], 0); ++i) {}
             }
         }
         __syncwarp();
     } else {
         // ---- softmax: one row a thread -----------------------------------------------------------------------------------
         const int s = warp >> 2, row = threadIdx.x & 127;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_s = tmem + s * 128 + lanes, t_o = tmem + 256 + s * 128 + lanes;
-        const uint32_t q_tile = base + s * S::kTileBytes;
-        unsigned turn_s = 0, turn_o = 0;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_o = tmem + 256 + s * 128 + lanes;
+        const uint32_t q_tile = q_base + s * S::kQBytes;
+        // its sign goes into Q, so that the largest S is the largest score; never 0, so that -inf stays -inf
+        const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);
+        const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+        const uint64_t scale2 = two(scale, scale);
+        unsigned used = 0;  // S tiles of this stream since the start
+        // The product before the present S tile is done. Two barriers in turn, as for S and P: one of them never completes a
+        // second phase before this thread has seen the first.
+        auto o_done = [&]() { return mbar_wait_for(&b_o[s][(used - 1) & 1], ((used - 1) >> 1) & 1, p.wait_cycles, &s_abort); };
         for_segments([&](int kvh, int block, int tile, int n) {
             const bool turns = runs.rows - block * kBlockRows <= kBlockRows / 2;
             const int ns = share(turns, n, s);
             const int first_row = block * kBlockRows + (turns ? 0 : s * 128), rows = min(128, runs.rows - first_row);
+            // this thread's row, and what lies before it in the queries and in the results; others ask for theirs by shuffle
+            const int mrow = first_row + row, trow = mrow / p.group, hrow = kvh * p.group + mrow % p.group;
+            const long long q_at = trow * p.q_stride + (long long)hrow * kHead, at_row = (long long)trow * p.n_heads + hrow;
             // this warp's 32 rows of Q, sixteen bytes a lane: what the stream's earlier products read is done with
             if (ns) {
-#pragma unroll 4
-                for (int i = 0; i < 32 * kHead / 8 / 32; ++i) {
-                    const int at = i * 32 + lane, r = (warp & 3) * 32 + at / (kHead / 8), c = at % (kHead / 8), m = first_row + r;
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (r < rows)
-                        v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (long long)(m / p.group) * p.q_stride +
-                                                            (long long)(kvh * p.group + m % p.group) * kHead + c * 8);
-                    const uint32_t to = q_tile + (c >> 3) * S::kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+                constexpr int kVec = kHead / 8, kLoads = kVec;  // 16-byte vectors of a row; 32 rows of them are kVec a lane
+                uint4 v[kLoads];
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const int r = (i * 32 + lane) / kVec, c = lane % kVec;
+                    const long long at = __shfl_sync(0xffffffffu, q_at, r);
+                    v[i] = make_uint4(0, 0, 0, 0);
+                    if ((warp & 3) * 32 + r < rows) v[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + at + c * 8);
+                }
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const int r = (warp & 3) * 32 + (i * 32 + lane) / kVec, c = lane % kVec;
+                    const uint32_t to = q_tile + (c >> 3) * S::kQHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v[i].x ^ sign), "r"(v[i].y ^ sign), "r"(v[i].z ^ sign),
+                                 "r"(v[i].w ^ sign)
+                                 : "memory");
                 }
                 fence_async_shared();
-                mbar_arrive(&b_q[s]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b_q[s]);
             }
 
             const bool busy = (warp & 3) * 32 < rows;  // warps without rows only keep step
-            float m = -INFINITY, l = 0.f;
-            for (int j = 0; j < ns; ++j) {
-                if (!__all_sync(0xffffffffu, mbar_wait_for(&b_s[s], turn_s++ & 1, p.wait_cycles, &s_abort))) return false;
+            float m = -INFINITY;
+            uint64_t sum[2] = {0, 0};
+            for (int j = 0; j < ns; ++j, ++used) {
+                if (!__all_sync(0xffffffffu, mbar_wait_for(&b_s[s][used & 1], (used >> 1) & 1, p.wait_cycles, &s_abort))) return false;
                 tc_fence_after();
                 if (busy) {
-                    uint32_t x[4][32];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, x[c]);
+                    const uint32_t t_s = tmem + s * 128 + (used & 1) * 64 + lanes;
+                    uint32_t x[2][32];
+                    tmem_ld32(t_s, x[0]);
+                    tmem_ld32(t_s + 32, x[1]);
                     tmem_wait_ld();
                     const int left = p.prefix - (tile + (turns ? 2 * j + s : j)) * kKeyTile;  // keys from this tile on
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) x[c][e] = __float_as_uint(__uint_as_float(x[c][e]) * p.scale_log2);
                     if (left < kKeyTile) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
+                        for (int c = 0; c < 2; ++c)
 #pragma unroll
                             for (int e = 0; e < 32; ++e)
                                 if (c * 32 + e >= left) x[c][e] = 0xff800000u;
                     }
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(x[c][e]));
-                    const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                        for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) top[i] = fmaxf(fmaxf(top[i], __uint_as_float(x[c][e + 2 * i])), __uint_as_float(x[c][e + 2 * i + 1]));
+                    float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    t = t == -INFINITY ? t : t * scale;
                     const bool move = t > m + kSlack || m == -INFINITY;
                     if (__any_sync(0xffffffffu, move)) {
                         const float to = move ? t : m, ref = to == -INFINITY ? 0.f : to, c = move ? exp2_fast(m - ref) : 1.f;
                         m = to;
-                        l *= c;
+                        const uint64_t c2 = two(c, c);
+                        sum[0] = fma2(sum[0], c2, 0);
+                        sum[1] = fma2(sum[1], c2, 0);
                         if (j > 0) {
-                            // the products before this S are done: S was queued behind them
+                            // O is at rest between the product before (waited for here) and the one that waits for this P
+                            if (!__all_sync(0xffffffffu, o_done())) return false;
+                            tc_fence_after();
 #pragma unroll 1
                             for (int d = 0; d < kHead; d += 32) {
                                 uint32_t o[32];
@@ -701,25 +742,23 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                             }
                         }
                     }
-                    const float ref = m == -INFINITY ? 0.f : m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float ref = m == -INFINITY ? 0.f : -m;
+                    const uint64_t ref2 = two(ref, ref);
+                    uint32_t w[32];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int c = 2 * h + e / 16, f = (e % 16) * 2;
-                            const float a = exp2_fast(__uint_as_float(x[c][f]) - ref), b = exp2_fast(__uint_as_float(x[c][f + 1]) - ref);
-                            sum[e & 3] += a + b;
-                            w[e] = pack2<T>(a, b);
-                        }
-                        tmem_st32(t_s + h * 32, w);
+                    for (int e = 0; e < 32; ++e) {
+                        const int c = e / 16, f = (e % 16) * 2;
+                        const float2 y = apart(fma2((uint64_t)x[c][f + 1] << 32 | x[c][f], scale2, ref2));
+                        const float a = exp2_fast(y.x), b = exp2_fast(y.y);
+                        sum[e & 1] = add2(sum[e & 1], two(a, b));
+                        w[e] = pack2<T>(a, b);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_st32(t_s, w);
                     tmem_wait_st();
                 }
                 tc_fence_before();
-                mbar_arrive(&b_p[s]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b_p[s][used & 1]);
             }
 
             // ---- the segment's result --------------------------------------------------------------------------------------
@@ -727,12 +766,12 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
             block_segments(runs, kvh, block, &first, &results);
             const int split = turns ? 2 * ((int)blockIdx.x - first) + s : (int)blockIdx.x - first;
             if (ns) {
-                if (!__all_sync(0xffffffffu, mbar_wait_for(&b_o[s], turn_o++ & 1, p.wait_cycles, &s_abort))) return false;
+                if (!__all_sync(0xffffffffu, o_done())) return false;
                 tc_fence_after();
             }
             if (busy) {
-                const int mrow = first_row + row, t = mrow / p.group, h = kvh * p.group + mrow % p.group;
-                if (row < rows) p.pre_ml[((long long)split * total_rows + t) * p.n_heads + h] = make_float2(m, l);
+                const float2 l2 = apart(add2(sum[0], sum[1]));
+                if (row < rows) p.pre_ml[(long long)split * total_rows * p.n_heads + at_row] = make_float2(m, l2.x + l2.y);
                 if (ns) {
                     // through this warp's own 32 rows of the Q tile (other warps may have the next segment's rows in theirs), 32
                     // dims at a time, so that rows leave in whole lines
@@ -750,15 +789,15 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                         __syncwarp();
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const int r = i * 4 + (lane >> 3), c = lane & 7, mm = first_row + (warp & 3) * 32 + r;
+                            const int r = i * 4 + (lane >> 3), c = lane & 7;
+                            const long long at = __shfl_sync(0xffffffffu, at_row, r);
                             uint4 v;
                             asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                                          : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                                          : "r"(mine + r * 128 + ((c ^ (r & 7)) << 4))
                                          : "memory");
                             if ((warp & 3) * 32 + r < rows)
-                                *reinterpret_cast<uint4*>(p.pre_o + (((long long)split * total_rows + mm / p.group) * p.n_heads + kvh * p.group + mm % p.group) * kHead +
-                                                          d + c * 4) = v;
+                                *reinterpret_cast<uint4*>(p.pre_o + ((long long)split * total_rows * p.n_heads + at) * kHead + d + c * 4) = v;
                         }
                         __syncwarp();
                     }

@@ -8,6 +8,14 @@
 
 namespace ml2 {
 
+// true in one lane of a converged warp, always the same one
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 // ---- TMEM: 128 lanes x 512 columns of 32 bits; an address is lane << 16 | column -----------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t* s_addr, uint32_t columns)  // one whole warp
 {
@@ -53,9 +61,13 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 // K-major (the 128 bytes run along the summed index): `stride` = bytes from one group of eight rows to the next.
 // MN-major (they run along the other index): `lead` = bytes to the next 64 values of that index, `stride` = to the next eight
 // values of the summed one.
-__device__ __forceinline__ uint64_t tc_operand(uint32_t smem_addr, uint32_t lead, uint32_t stride)
+// All operands here have a stride of 1024, so the upper half is a constant; the address counts 16 bytes, and a step along the
+// summed index is added to the lower half.
+__device__ __forceinline__ uint32_t tc_operand_low(uint32_t smem_addr, uint32_t lead) { return (smem_addr & 0x3ffffu) >> 4 | (lead >> 4) << 16; }
+__device__ __forceinline__ uint64_t tc_operand_at(uint32_t low)
 {
-    return (uint64_t)((smem_addr & 0x3ffffu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
+    constexpr uint64_t kHigh = 1024 >> 4 | 1u << 14 | 2u << 29;  // stride, format of this generation, 128-byte swizzle
+    return kHigh << 32 | low;
 }
 // kind::f16 with fp32 accumulation: A and B both fp16 (bf16 = 0) or both bf16 (1)
 __host__ __device__ constexpr uint32_t tc_shape(int m, int n, int bf16, bool b_mn_major)
