@@ -22,16 +22,17 @@ struct AttnBatch {
     const int *table, *lengths, *query_start;
     DeviceStatus* status;
     DeviceStatus* waits;
-    // Partial results of the prefix, [splits][rows that are there][n_heads], and of the own tokens, [splits][n_rows][n_heads]:
-    // o = sum of exp2(score - m) v over the keys of one split [head], and (m, l): a reference near the largest score (in
-    // powers of two) and l = sum of exp2(score - m). A result without keys has m = -inf, l = 0 and an o that is not read.
-    float *pre_o, *own_o;
-    float2 *pre_ml, *own_ml;
+    // Partial results, for a row and head the sum o = sum of exp2(score - m) v over some of the keys [head], and (m, l): a
+    // reference near the largest score (in powers of two) and l = sum of exp2(score - m). One without keys has m = -inf, l = 0
+    // and an o that is not read. pre: of the prefix by blocks, [segments][rows that are there][n_heads]; run: of the warps' runs.
+    float *pre_o, *run_o;
+    float2 *pre_ml, *run_ml;
+    int* run_base;      // [n_requests + 1]: key tiles before request r, of all requests; then the tiles of a run
     long long wait_cycles;
     long long out_stride, q_stride, prefix_stride, cache_stride;
     int n_requests, n_rows, prefix, max_length, n_pages, table_stride, page_shift, n_heads, n_kv, group;
-    int prefix_chunk, prefix_splits, own_chunk;  // keys of a split (multiples of 16); prefix_splits 0: cut by blocks instead
-    int prefix_ctas;    // of the kernel that does the prefix by blocks, 0 without it
+    int prefix_ctas;    // of the kernel that does the prefix by blocks, 0 where the runs do it
+    int run_ctas;       // of the kernel of runs, 0 without it
     float scale_log2;   // scale * log2(e)
 };
 
@@ -89,88 +90,113 @@ __device__ __forceinline__ float exp2_fast(float x)
     return y;
 }
 
-// One piece of work of a warp: up to 16 rows (query row, head of the group) of one key head against a run of keys.
-struct Unit {
-    int request;            // -1: the prefix
-    int kvh, row0, rows;    // rows: of the 16, counted over (query, head of the group); row0: first of them in the request
-    int first, count;       // the request's query rows
-    int length;             // own tokens (prefix rows)
-    int key0, key1;
-    int split;
-};
-
-// Rows of a request that has `count` queries, counted 16 at a time.
+// Rows of a request that has `count` queries (or of the prefix, which all see), counted 16 at a time.
 __device__ __forceinline__ int row_tiles(const AttnBatch& p, int count) { return (count * p.group + 15) >> 4; }
-
-__device__ __forceinline__ Unit decode_unit(const AttnBatch& p, const int* s_units, int total_rows, int u)
+// Key tiles that the 16 rows from row0 on look at: as many as the last of them sees.
+__device__ __forceinline__ int tiles_seen(const AttnBatch& p, int count, int length, int row0, int rows)
 {
-    Unit w{};
-    const int own = s_units[p.n_requests];
-    int chunk;
-    if (u >= own) {
-        u -= own;
-        w.request = -1;
+    const int last = (row0 + rows - 1) / p.group, seen = min(length, length - count + last + 1);
+    return seen > 0 ? (seen + kTile - 1) / kTile : 0;
+}
+// Where the result of run `run` for the 16 rows from row0 on of a key head begins: runs and rows are numbered through, so that
+// no two results meet and all need no more than one entry per row and head, and 16 per run.
+__device__ __forceinline__ long long result_row(const AttnBatch& p, bool prefix, int first, int row0, int rows, int kvh, int run)
+{
+    return (prefix ? (long long)p.n_rows * p.n_heads : 0) + ((long long)first * p.group + row0) * p.n_kv + kvh * rows + 16ll * run;
+}
+
+// A walk over the key tiles of one run: 16 rows of one key head and request (a sequence), all its key tiles, then the next.
+struct Walk {
+    int pos, end;              // of all tiles
+    int request;               // n_requests: the prefix
+    int rt, kvh, k;            // row tile, key head, key tile
+    int first, count, length;  // query rows and keys of the request
+    int tiles, need, rows;     // key tiles of a sequence, those that its rows see, its rows
+};
+__device__ __forceinline__ void open_request(const AttnBatch& p, Walk& w, int total_rows)
+{
+    if (w.request == p.n_requests) {
         w.first = 0;
         w.count = total_rows;
         w.length = p.prefix;
-        chunk = p.prefix_chunk;
     } else {
-        int lo = 0, hi = p.n_requests - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (s_units[mid + 1] > u) hi = mid;
-            else lo = mid + 1;
-        }
-        u -= s_units[lo];
-        const Span s = request_span(p, lo);
-        w.request = lo;
+        const Span s = request_span(p, w.request);
         w.first = s.first;
         w.count = s.count;
         w.length = s.length;
-        chunk = p.own_chunk;
     }
-    const int tiles = row_tiles(p, w.count);
-    // key heads next to one another in the cache go to neighbouring warps, then row tiles that read the same keys
-    w.kvh = u % p.n_kv;
-    u /= p.n_kv;
-    w.row0 = (u % tiles) * 16;
-    w.split = u / tiles;
-    w.rows = min(16, w.count * p.group - w.row0);
-    w.key0 = w.split * chunk;
-    w.key1 = min(w.key0 + chunk, w.length);
-    if (w.request >= 0) {
-        // the last row of the tile sees the most
-        const int last = (w.row0 + w.rows - 1) / p.group;
-        w.key1 = min(w.key1, w.length - w.count + last + 1);
+    w.tiles = (w.length + kTile - 1) / kTile;
+}
+__device__ __forceinline__ void open_rows(const AttnBatch& p, Walk& w)
+{
+    w.rows = min(16, w.count * p.group - w.rt * 16);
+    w.need = w.request == p.n_requests ? w.tiles : tiles_seen(p, w.count, w.length, w.rt * 16, w.rows);
+}
+__device__ __forceinline__ void open_walk(const AttnBatch& p, const int* s_base, int total_rows, Walk& w)
+{
+    if (w.pos >= w.end) return;
+    int lo = 0, hi = p.n_requests;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s_base[mid + 1] > w.pos) hi = mid;
+        else lo = mid + 1;
     }
-    return w;
+    w.request = lo;
+    open_request(p, w, total_rows);
+    const int local = w.pos - s_base[lo], seq = local / w.tiles;
+    w.k = local - seq * w.tiles;
+    // key heads, next to one another in the cache, go to neighbouring runs
+    w.rt = seq / p.n_kv;
+    w.kvh = seq - w.rt * p.n_kv;
+    open_rows(p, w);
+}
+// Moves to the next key tile that somebody sees; false at the end of the run.
+__device__ __forceinline__ bool settle(const AttnBatch& p, const int* s_base, int total_rows, Walk& w)
+{
+    while (w.pos < w.end) {
+        if (w.k < w.need) return true;
+        w.pos += w.tiles - w.k;
+        w.k = 0;
+        if (w.pos >= w.end) return false;
+        if (++w.kvh < p.n_kv) continue;
+        w.kvh = 0;
+        if (++w.rt == row_tiles(p, w.count)) {
+            w.rt = 0;
+            do ++w.request;
+            while (s_base[w.request + 1] == s_base[w.request]);
+            open_request(p, w, total_rows);
+        }
+        open_rows(p, w);
+    }
+    return false;
 }
 
-// Every warp works for itself: it takes units at a fixed stride, streams their keys and values through a ring of its own
-// (cp.async, the next tiles of this or the following unit are under way while one is used) and leaves a partial result.
-// 16 rows are all the tensor core's m16 has, so a tile of 16 keys (8 KB at head 128) costs 32 products however few rows
-// are real; at one row HBM still bounds it.
+// Every warp works for itself: the key tiles of all requests, one after the other, are cut into runs of the same length, one
+// a warp. It streams its tiles through a ring of its own (cp.async; the next two are under way while one is used, across the
+// borders of sequences) and leaves a result for every sequence that it has a part of. 16 rows are all the tensor core's m16
+// has, so a tile of 16 keys (8 KB at head 128) costs 32 products however few rows are real; at one row HBM still bounds it.
 template <typename T, int kHead>
-__global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const __grid_constant__ AttnBatch p)
+__global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const __grid_constant__ AttnBatch p)
 {
     constexpr int kRowBytes = kHead * 2, kChunks = kHead / 8, kTileBytes = kTile * kRowBytes, kSteps = kHead / 16;
     extern __shared__ __align__(128) unsigned char s_mem[];
     __shared__ unsigned s_valid[kAttnWarps][kStages];
-    __shared__ int s_sum[kAttnWarps + 1];
-    int* s_units = reinterpret_cast<int*>(s_mem + kAttnWarps * kStages * 2 * kTileBytes);  // units before request r
+    __shared__ int s_sum[kAttnWarps];
+    int* s_base = reinterpret_cast<int*>(s_mem + kAttnWarps * kStages * 2 * kTileBytes);  // tiles before request r; the prefix last
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // after the prefix kernel, which has waited for what comes before both, this one starts beside it
     if (!p.prefix_ctas) pdl_wait();
-    // ---- how many units every request has ---------------------------------------------------------------------------
+    const int total_rows = min(max(p.query_start[p.n_requests], 0), p.n_rows);
+    // ---- how many tiles every request has -----------------------------------------------------------------------------
     {
         const int per = ceil_div(p.n_requests, kAttnThreads), r0 = min((int)threadIdx.x * per, p.n_requests), r1 = min(r0 + per, p.n_requests);
         int mine = 0;
         for (int r = r0; r < r1; ++r) {
             const Span s = request_span(p, r);
             if (!s.good && blockIdx.x == 0) report_input_error(p.status, kInputLength, r);
-            s_units[r] = mine;
-            mine += row_tiles(p, s.count) * ceil_div(s.length, p.own_chunk) * p.n_kv;
+            s_base[r] = mine;
+            mine += row_tiles(p, s.count) * p.n_kv * ((s.length + kTile - 1) / kTile);
         }
         int incl = mine;
 #pragma unroll
@@ -186,27 +212,36 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const 
             if (w < warp) base += s_sum[w];
             all += s_sum[w];
         }
-        for (int r = r0; r < r1; ++r) s_units[r] += base;
-        if (threadIdx.x == 0) s_units[p.n_requests] = all;
+        for (int r = r0; r < r1; ++r) s_base[r] += base;
+        if (threadIdx.x == 0) {
+            s_base[p.n_requests] = all;
+            s_base[p.n_requests + 1] = all + (p.prefix_ctas ? 0 : row_tiles(p, total_rows) * p.n_kv * ((p.prefix + kTile - 1) / kTile));
+        }
         __syncthreads();
     }
-    const int total_rows = min(max(p.query_start[p.n_requests], 0), p.n_rows);
-    const int units = s_units[p.n_requests] + p.prefix_splits * row_tiles(p, total_rows) * p.n_kv;
-    const int stride = gridDim.x * kAttnWarps;
+    const int all = s_base[p.n_requests + 1], per = (all + gridDim.x * kAttnWarps - 1) / (gridDim.x * kAttnWarps), run = blockIdx.x * kAttnWarps + warp;
+    if (blockIdx.x == 0) {  // the join finds the results by these
+        for (int r = threadIdx.x; r <= p.n_requests; r += kAttnThreads) p.run_base[r] = s_base[r];
+        if (threadIdx.x == 0) p.run_base[p.n_requests + 1] = per;
+    }
 
     unsigned char* ring = s_mem + warp * kStages * 2 * kTileBytes;
     const uint32_t ring_u32 = smem_u32(ring);
     const int page_mask = (1 << p.page_shift) - 1;
 
     // ---- where the loads stand: the next tile to ask for ----------------------------------------------------------------
-    int load_u = blockIdx.x * kAttnWarps + warp, load_key = 0;
-    Unit ld{};
+    Walk ld{};
+    ld.pos = min(run * per, all);
+    ld.end = min(ld.pos + per, all);
+    open_walk(p, s_base, total_rows, ld);
+    Walk w = ld;
+    bool more = settle(p, s_base, total_rows, ld);
     long long row = -1;  // lanes 0..15: cache row of the tile's key `lane`, -1 for none
     auto find_rows = [&]() {
-        const int key = load_key + (lane & 15);
+        const int key = ld.k * kTile + (lane & 15);
         row = -1;
-        if (key < ld.key1) {
-            if (ld.request < 0) row = key;
+        if (key < ld.length) {
+            if (ld.request == p.n_requests) row = key;
             else {
                 const int page = p.table[(long long)ld.request * p.table_stride + (key >> p.page_shift)];
                 if (page >= 0 && page < p.n_pages) row = ((long long)page << p.page_shift) + (key & page_mask);
@@ -214,20 +249,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const 
             }
         }
     };
-    auto open_unit = [&]() {
-        while (load_u < units) {
-            ld = decode_unit(p, s_units, total_rows, load_u);
-            if (ld.key0 < ld.key1) break;
-            load_u += stride;
-        }
-        load_key = ld.key0;
-        if (load_u < units) find_rows();
-    };
     auto load_tile = [&](int stage) {
-        if (load_u < units) {
-            const T* kb = static_cast<const T*>(ld.request < 0 ? p.pk : p.k) + (long long)ld.kvh * kHead;
-            const T* vb = static_cast<const T*>(ld.request < 0 ? p.pv : p.v) + (long long)ld.kvh * kHead;
-            const long long step = ld.request < 0 ? p.prefix_stride : p.cache_stride;
+        if (more) {
+            const bool prefix = ld.request == p.n_requests;
+            const T* kb = static_cast<const T*>(prefix ? p.pk : p.k) + (long long)ld.kvh * kHead;
+            const T* vb = static_cast<const T*>(prefix ? p.pv : p.v) + (long long)ld.kvh * kHead;
+            const long long step = prefix ? p.prefix_stride : p.cache_stride;
             const unsigned valid = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
             if (lane == 0) s_valid[warp][stage] = valid;
             const uint32_t dst = ring_u32 + stage * 2 * kTileBytes;
@@ -240,33 +267,33 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const 
                 cp_async16(to, kb + off, r < 0 ? 0 : 16);
                 cp_async16(to + kTileBytes, vb + off, r < 0 ? 0 : 16);
             }
-            load_key += kTile;
-            if (load_key < ld.key1) find_rows();
-            else {
-                load_u += stride;
-                open_unit();
-            }
+            ++ld.k;
+            ++ld.pos;
+            more = settle(p, s_base, total_rows, ld);
+            if (more) find_rows();  // the table is asked one tile ahead
         }
         cp_async_commit();
     };
 
-    open_unit();
+    if (more) find_rows();
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) load_tile(i);
 
     int stage = 0;
     const int g = lane >> 2, t4 = lane & 3;
-    for (int u = blockIdx.x * kAttnWarps + warp; u < units; u += stride) {
-        const Unit w = decode_unit(p, s_units, total_rows, u);
-        if (w.key0 >= w.key1) continue;
+    while (settle(p, s_base, total_rows, w)) {
+        const bool prefix = w.request == p.n_requests;
+        const int tile0 = w.k, tile1 = min(w.need, w.k + (w.end - w.pos)), row0 = w.rt * 16;
+        w.pos += tile1 - tile0;
+        w.k = tile1;
 
         // rows g and g + 8 of the tile: query row, head, and the keys they see
-        const int m0 = w.row0 + g, m1 = m0 + 8;
+        const int m0 = row0 + g, m1 = m0 + 8;
         const bool live0 = g < w.rows, live1 = g + 8 < w.rows;
         const int i0 = m0 / p.group, i1 = m1 / p.group;
         const int h0 = w.kvh * p.group + m0 % p.group, h1 = w.kvh * p.group + m1 % p.group;
-        const int seen0 = w.request < 0 ? w.length : w.length - w.count + i0 + 1, seen1 = w.request < 0 ? w.length : w.length - w.count + i1 + 1;
-        const bool causal = w.request >= 0 && w.count > 1;
+        const int seen0 = prefix ? w.length : w.length - w.count + i0 + 1, seen1 = prefix ? w.length : w.length - w.count + i1 + 1;
+        const int seen_by_all = prefix || w.count == 1 ? w.length : w.length - w.count + row0 / p.group + 1;
 
         uint32_t qf[kSteps][4];
         {
@@ -285,7 +312,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const 
         for (int n = 0; n < kHead / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
         float mx0 = -INFINITY, mx1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
-        for (int key = w.key0; key < w.key1; key += kTile) {
+        for (int key = tile0 * kTile; key < tile1 * kTile; key += kTile) {
             cp_async_wait<kStages - 2>();
             __syncwarp();
             const uint32_t kt = ring_u32 + stage * 2 * kTileBytes, vt = kt + kTileBytes;
@@ -302,7 +329,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const 
                     mma16816<T>(s[1], qf[k], b[2], b[3]);
                 }
             }
-            const bool masked = valid != 0xffffu || (causal && key + kTile > w.length - w.count + 1);
+            const bool causal = key + kTile > seen_by_all && seen_by_all < w.length, masked = valid != 0xffffu || causal;
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -344,21 +371,21 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const 
                 l0 += s[n][0] + s[n][1];
                 l1 += s[n][2] + s[n][3];
             }
-            if (masked && causal) {
+            if (causal) {
                 // Weight 0 times a value that is not finite would be NaN in the rows that do not see its key. Such keys are
                 // taken out of the product and added to the rows that see them one by one.
+                constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u, kOne = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
                 unsigned odd = 0;
-                for (int j = 0; j < kTile; ++j) {
+                for (int i = 0; i < kChunks / 2; ++i) {
+                    const int at = i * 32 + lane;  // 16 bytes of key at / kChunks
+                    uint32_t v[4];
+                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(vt + at * 16) : "memory");
                     bool bad = false;
-                    for (int c = lane; c < kHead / 2; c += 32) {
-                        const uint32_t at = vt + j * kRowBytes + ((((c >> 2) ^ (j & 7)) << 4) | ((c & 3) << 2));
-                        uint32_t v;
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-                        const float2 f = unpack2<T>(v);
-                        bad |= !isfinite(f.x) || !isfinite(f.y);
-                    }
-                    if (__any_sync(0xffffffffu, bad)) odd |= 1u << j;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) bad |= (((v[e] & kExp) + kOne) & 0x80008000u) != 0;  // an exponent of ones carries over
+                    if (bad) odd |= 1u << (at / kChunks);
                 }
+                odd = __reduce_or_sync(0xffffffffu, odd);
                 for (unsigned left = odd; left; left &= left - 1) {
                     const int j = __ffs(left) - 1, n = j >> 3, src = (lane & ~3) | ((j & 7) >> 1);
                     const float pa = (j & 1) ? s[n][1] : s[n][0], pb = (j & 1) ? s[n][3] : s[n][2];
@@ -404,20 +431,16 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_units_kernel(const 
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        const long long step = w.request < 0 ? total_rows : p.n_rows;
-        float* part_o = w.request < 0 ? p.pre_o : p.own_o;
-        float2* part_ml = w.request < 0 ? p.pre_ml : p.own_ml;
-        const long long at0 = (w.split * step + w.first + i0) * p.n_heads + h0;
-        const long long at1 = (w.split * step + w.first + i1) * p.n_heads + h1;
+        const long long at0 = result_row(p, prefix, w.first, row0, w.rows, w.kvh, run) + g, at1 = at0 + 8;
         if (live0) {
-            if (t4 == 0) part_ml[at0] = make_float2(mx0, l0);
+            if (t4 == 0) p.run_ml[at0] = make_float2(mx0, l0);
 #pragma unroll
-            for (int n = 0; n < kHead / 8; ++n) *reinterpret_cast<float2*>(part_o + at0 * kHead + n * 8 + t4 * 2) = make_float2(acc[n][0], acc[n][1]);
+            for (int n = 0; n < kHead / 8; ++n) *reinterpret_cast<float2*>(p.run_o + at0 * kHead + n * 8 + t4 * 2) = make_float2(acc[n][0], acc[n][1]);
         }
         if (live1) {
-            if (t4 == 0) part_ml[at1] = make_float2(mx1, l1);
+            if (t4 == 0) p.run_ml[at1] = make_float2(mx1, l1);
 #pragma unroll
-            for (int n = 0; n < kHead / 8; ++n) *reinterpret_cast<float2*>(part_o + at1 * kHead + n * 8 + t4 * 2) = make_float2(acc[n][2], acc[n][3]);
+            for (int n = 0; n < kHead / 8; ++n) *reinterpret_cast<float2*>(p.run_o + at1 * kHead + n * 8 + t4 * 2) = make_float2(acc[n][2], acc[n][3]);
         }
     }
     cp_async_wait<0>();
@@ -448,7 +471,7 @@ struct PrefixMaps {
 };
 struct PrefixRuns {  // how blocks and key tiles are cut, from the rows that are there: the same in both kernels
     int rows, blocks, key_tiles, per;    // rows of a key head, blocks of them, key tiles of one block, tiles of a CTA
-    long long tiles;
+    int tiles;                           // n_kv * blocks * key_tiles, below 2^31 (the host sees to it)
 };
 __host__ __device__ __forceinline__ PrefixRuns prefix_runs(int total_rows, int group, int n_kv, int prefix, int ctas)
 {
@@ -456,16 +479,16 @@ __host__ __device__ __forceinline__ PrefixRuns prefix_runs(int total_rows, int g
     r.rows = total_rows * group;
     r.blocks = ceil_div(r.rows, kBlockRows);
     r.key_tiles = ceil_div(prefix, kKeyTile);
-    r.tiles = (long long)n_kv * r.blocks * r.key_tiles;
-    r.per = (int)((r.tiles + ctas - 1) / ctas);
+    r.tiles = n_kv * r.blocks * r.key_tiles;
+    r.per = ceil_div(r.tiles, ctas);
     return r;
 }
 // Segments of a block: the CTAs first .. last have a part of it; two results each where the streams take turns.
 __device__ __forceinline__ void block_segments(const PrefixRuns& r, int kvh, int block, int* first, int* results)
 {
-    const long long a = ((long long)kvh * r.blocks + block) * r.key_tiles;
-    *first = (int)(a / r.per);
-    const int n = (int)((a + r.key_tiles - 1) / r.per) - *first + 1;
+    const unsigned a = (unsigned)(kvh * r.blocks + block) * r.key_tiles;
+    *first = (int)(a / (unsigned)r.per);
+    const int n = (int)((a + r.key_tiles - 1) / (unsigned)r.per) - *first + 1;
     *results = r.rows - block * kBlockRows <= kBlockRows / 2 ? 2 * n : n;
 }
 
@@ -534,15 +557,22 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
 
     const int total_rows = min(max(p.query_start[p.n_requests], 0), p.n_rows);
     const PrefixRuns runs = prefix_runs(total_rows, p.group, p.n_kv, p.prefix, gridDim.x);
-    const long long begin = min((long long)blockIdx.x * runs.per, runs.tiles), end = min(begin + runs.per, runs.tiles);
+    const int begin = min((int)blockIdx.x * runs.per, runs.tiles), end = min(begin + runs.per, runs.tiles);
 
     // a CTA's run, block by block: f(kvh, block, first key tile, tiles)
     auto for_segments = [&](auto&& f) {
-        for (long long at = begin; at < end;) {
-            const long long which = at / runs.key_tiles;
-            const int tile = (int)(at - which * runs.key_tiles), n = (int)min((long long)(runs.key_tiles - tile), end - at);
-            if (!f((int)(which / runs.blocks), (int)(which % runs.blocks), tile, n)) return false;
-            at += n;
+        if (begin >= end) return true;
+        int kvh = begin / runs.key_tiles, tile = begin - kvh * runs.key_tiles, block = kvh % runs.blocks;
+        kvh /= runs.blocks;
+        for (int left = end - begin; left > 0;) {
+            const int n = min(runs.key_tiles - tile, left);
+            if (!f(kvh, block, tile, n)) return false;
+            left -= n;
+            tile = 0;
+            if (++block == runs.blocks) {
+                block = 0;
+                ++kvh;
+            }
         }
         return true;
     };
@@ -823,30 +853,55 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     const int lane = threadIdx.x & 31;
     const int t = (int)(id / p.n_heads), h = (int)(id % p.n_heads);
     if (t >= p.n_rows || t >= p.query_start[p.n_requests]) return;
-    int lo = 0, hi = p.n_requests - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (p.query_start[mid + 1] > t) hi = mid;
-        else lo = mid + 1;
+    const int g = h % p.group, kvh = h / p.group, total_rows = min(p.query_start[p.n_requests], p.n_rows);
+    // the request of this row: the lanes look at 32 places at a time
+    int lo = 0;
+    for (int n = p.n_requests; n > 1;) {
+        const int step = (n + 31) >> 5, at = lo + lane * step;
+        const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && p.query_start[at] <= t);
+        const int k = below ? 31 - __clz(below) : 0;
+        lo += k * step;
+        n = min(step, n - k * step);
     }
-    const Span s = request_span(p, lo);
-    const int seen = s.good ? min(s.length, max(0, s.length - s.count + (t - s.first) + 1)) : 0;
-    const int total_rows = min(p.query_start[p.n_requests], p.n_rows);
-    int pre = p.prefix_splits;
+    // results: of the prefix (by blocks: `step` apart; by runs), then of the own tokens
+    long long pre_at = 0, pre_step = 0, own_at = 0;
+    int pre = 0, own = 0;
+    const float *pre_o = p.pre_o, *own_o = p.run_o;
+    const float2 *pre_ml = p.pre_ml, *own_ml = p.run_ml;
     if (p.prefix_ctas) {
         int first;
         const PrefixRuns runs = prefix_runs(total_rows, p.group, p.n_kv, p.prefix, p.prefix_ctas);
-        block_segments(runs, h / p.group, (t * p.group + h % p.group) / kBlockRows, &first, &pre);
+        block_segments(runs, kvh, (t * p.group + g) / kBlockRows, &first, &pre);
+        pre_at = id;
+        pre_step = (long long)total_rows * p.n_heads;
     }
-    const int splits = pre + ceil_div(seen, p.own_chunk);
-    const long long pre_step = (long long)total_rows * p.n_heads, own_step = (long long)p.n_rows * p.n_heads;
+    if (p.run_ctas) {
+        const int per = max(p.run_base[p.n_requests + 1], 1);
+        if (!p.prefix_ctas && p.prefix) {
+            const int m = t * p.group + g, row0 = m & ~15, rows = min(16, total_rows * p.group - row0), tiles = (p.prefix + kTile - 1) / kTile;
+            const int a = p.run_base[p.n_requests] + ((row0 >> 4) * p.n_kv + kvh) * tiles, first = a / per;
+            pre = (a + tiles - 1) / per - first + 1;
+            pre_at = result_row(p, true, 0, row0, rows, kvh, first) + (m & 15);
+            pre_step = 16;
+            pre_o = p.run_o;
+            pre_ml = p.run_ml;
+        }
+        const Span s = request_span(p, lo);
+        if (s.good && t >= s.first && t < s.first + s.count && s.length > 0) {
+            const int m = (t - s.first) * p.group + g, row0 = m & ~15, rows = min(16, s.count * p.group - row0), tiles = (s.length + kTile - 1) / kTile;
+            const int a = p.run_base[lo] + ((row0 >> 4) * p.n_kv + kvh) * tiles, first = a / per, need = tiles_seen(p, s.count, s.length, row0, rows);
+            own = need ? (a + need - 1) / per - first + 1 : 0;
+            own_at = result_row(p, false, s.first, row0, rows, kvh, first) + (m & 15);
+        }
+    }
+    const int splits = pre + own;
 
     float m = -INFINITY, l = 0.f, acc[kPer] = {};
     for (int base = 0; base < splits; base += 32) {
         const int mine = base + lane;
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (mine < pre) ml = p.pre_ml[mine * pre_step + id];
-        else if (mine < splits) ml = p.own_ml[(mine - pre) * own_step + id];
+        if (mine < pre) ml = pre_ml[pre_at + mine * pre_step];
+        else if (mine < splits) ml = own_ml[own_at + (mine - pre) * 16];
         const float mn = fmaxf(m, warp_max(ml.x)), to = mn == -INFINITY ? 0.f : mn;
         const float c = exp2_fast(m - to), w = exp2_fast(ml.x - to);
         l = l * c + warp_sum(ml.y * w);
@@ -854,18 +909,30 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
         for (int e = 0; e < kPer; ++e) acc[e] *= c;
         m = mn;
         const int here = min(32, splits - base);
-        for (int i = 0; i < here; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            if (wi == 0.f) continue;
-            const int at = base + i;
-            const float* o = (at < pre ? p.pre_o + (at * pre_step + id) * kHead : p.own_o + ((at - pre) * own_step + id) * kHead) + lane * kPer;
-            if constexpr (kPer == 4) {
-                const float4 v = *reinterpret_cast<const float4*>(o);
-                acc[0] += wi * v.x; acc[1] += wi * v.y; acc[2] += wi * v.z; acc[3] += wi * v.w;
-            } else {
-                const float2 v = *reinterpret_cast<const float2*>(o);
-                acc[0] += wi * v.x; acc[1] += wi * v.y;
+        for (int i = 0; i < here; i += 8) {  // eight at a time are under way
+            float v[8][kPer], wi[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int at = base + i + k;
+                wi[k] = __shfl_sync(0xffffffffu, w, (i + k) & 31);
+                if (i + k >= here) wi[k] = 0.f;
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) v[k][e] = 0.f;
+                if (wi[k] != 0.f) {
+                    const float* o = (at < pre ? pre_o + (pre_at + at * pre_step) * kHead : own_o + (own_at + (at - pre) * 16ll) * kHead) + lane * kPer;
+                    if constexpr (kPer == 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(o);
+                        v[k][0] = x.x; v[k][1] = x.y; v[k][2] = x.z; v[k][3] = x.w;
+                    } else {
+                        const float2 x = *reinterpret_cast<const float2*>(o);
+                        v[k][0] = x.x; v[k][1] = x.y;
+                    }
+                }
             }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) acc[e] += wi[k] * v[k][e];
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -877,48 +944,37 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     if (p.lse && lane == 0) p.lse[id] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
 }
 
-// How the keys are cut. Own tokens: pieces of at most 256 keys, and smaller ones (32 at least) where whole requests would
-// not give every warp of the machine four pieces. The prefix likewise.
+// Which kernels run, and the workspace's layout.
 struct AttnPlan {
-    int prefix_chunk, prefix_splits, own_chunk, own_splits, grid, prefix_ctas;
-    long long units;
-    size_t pre_o, own_o, pre_ml, own_ml, bytes;  // offsets into the workspace, and its size
+    int prefix_ctas, run_ctas;
+    long long tiles;   // key tiles of either kernel, at most
+    size_t run_o, pre_ml, run_ml, run_base, bytes;  // offsets into the workspace (pre_o comes first), and its size
 };
-static void cut(int length, long long pieces_of_one_split, int warps, int* chunk, int* splits)
-{
-    *chunk = kTile;
-    *splits = 0;
-    if (length == 0) return;
-    long long n = std::max<long long>(ceil_div(length, 256), (4ll * warps + pieces_of_one_split - 1) / pieces_of_one_split);
-    n = std::min<long long>(n, std::min(64, ceil_div(length, 32)));
-    *chunk = ceil_div(ceil_div(length, (int)n), kTile) * kTile;
-    *splits = ceil_div(length, *chunk);
-}
 static AttnPlan plan_attention(const Ctx* ctx, int n_rows, int n_requests, int prefix, int max_length, int n_heads, int n_kv, int head)
 {
     AttnPlan pl{};
-    const int warps = 2 * ctx->sm_count * kAttnWarps, group = n_heads / n_kv;
-    const long long own_tiles = n_requests + (long long)n_rows * group / 16, prefix_tiles = ((long long)n_rows * group + 15) / 16;
-    long long pre_rows = 0;
-    if (prefix >= kBlockPrefix && n_rows) {
-        const long long blocks = ((long long)n_rows * group + kBlockRows - 1) / kBlockRows, key_tiles = ceil_div(prefix, kKeyTile);
-        pl.prefix_ctas = (int)std::min<long long>(std::max(1, ctx->sm_count), blocks * n_kv * key_tiles);
+    if (!n_rows) return pl;
+    const int sms = std::max(1, ctx->sm_count);
+    const long long rows = (long long)n_rows * (n_heads / n_kv);  // of a key head
+    long long pre_rows = 0, run_rows = 0, run_tiles = (n_requests + rows / 16) * n_kv * ceil_div(max_length, kTile);
+    if (prefix >= kBlockPrefix) {
+        const long long blocks = (rows + kBlockRows - 1) / kBlockRows, key_tiles = ceil_div(prefix, kKeyTile);
+        pl.tiles = blocks * n_kv * key_tiles;
+        pl.prefix_ctas = (int)std::min<long long>(sms, pl.tiles);
         // Any number of rows up to n_rows may be there. With b blocks of a key head a CTA has at least n_kv b key_tiles / ctas
         // tiles, a block at most ctas / (n_kv b) + 2 segments and never more than key tiles, and a segment two results.
-        pre_rows = std::min(512ll * pl.prefix_ctas + 1024ll * blocks * n_kv, 2ll * key_tiles * n_rows * n_heads);
-        pl.prefix_chunk = kTile;
+        pre_rows = std::min(512ll * pl.prefix_ctas + 1024ll * blocks * n_kv, 2 * key_tiles * n_rows * n_heads);
     } else {
-        cut(prefix, prefix_tiles * n_kv, warps, &pl.prefix_chunk, &pl.prefix_splits);
-        pre_rows = (long long)pl.prefix_splits * n_rows * n_heads;
+        run_tiles += (rows + 15) / 16 * n_kv * ceil_div(prefix, kTile);
     }
-    cut(max_length, own_tiles * n_kv, warps, &pl.own_chunk, &pl.own_splits);
-    pl.units = (own_tiles * pl.own_splits + prefix_tiles * pl.prefix_splits) * n_kv;
-    pl.grid = (int)std::min<long long>(2 * ctx->sm_count, (pl.units + kAttnWarps - 1) / kAttnWarps);
-    const size_t own_rows = (size_t)pl.own_splits * n_rows * n_heads;
-    pl.own_o = (size_t)pre_rows * head * sizeof(float);
-    pl.pre_ml = pl.own_o + own_rows * head * sizeof(float);
-    pl.own_ml = pl.pre_ml + (size_t)pre_rows * sizeof(float2);
-    pl.bytes = pl.own_ml + own_rows * sizeof(float2);
+    pl.tiles = std::max(pl.tiles, run_tiles);
+    pl.run_ctas = (int)std::min<long long>(2 * sms, (run_tiles + kAttnWarps - 1) / kAttnWarps);
+    if (pl.run_ctas) run_rows = 2ll * n_rows * n_heads + 16ll * pl.run_ctas * kAttnWarps;
+    pl.run_o = (size_t)pre_rows * head * sizeof(float);
+    pl.pre_ml = pl.run_o + (size_t)run_rows * head * sizeof(float);
+    pl.run_ml = pl.pre_ml + (size_t)pre_rows * sizeof(float2);
+    pl.run_base = pl.run_ml + (size_t)run_rows * sizeof(float2);
+    pl.bytes = pl.run_base + (pl.run_ctas ? (n_requests + 2) * sizeof(int) : 0);
     return pl;
 }
 
@@ -948,7 +1004,7 @@ static cudaError_t launch_attention(Ctx* ctx, const AttnBatch& p, const AttnPlan
     static bool ready[16] = {};  // shared-memory limits are set once per device
     cudaError_t e = cudaSuccess;
     if (!ready[ctx->device & 15]) {
-        e = cudaFuncSetAttribute(attention_units_kernel<T, kHead>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        e = cudaFuncSetAttribute(attention_runs_kernel<T, kHead>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_prefix_kernel<T, kHead>, cudaFuncAttributeMaxDynamicSharedMemorySize, BlockSmem<kHead>::kBytes);
         if (e != cudaSuccess) return e;
         ready[ctx->device & 15] = true;
@@ -968,11 +1024,11 @@ static cudaError_t launch_attention(Ctx* ctx, const AttnBatch& p, const AttnPlan
         ++ctx->launches;
         cfg.numAttrs = 1;  // what follows starts as this kernel's CTAs leave
     }
-    if (pl.grid) {
-        cfg.gridDim = dim3(pl.grid);
+    if (pl.run_ctas) {
+        cfg.gridDim = dim3(pl.run_ctas);
         cfg.blockDim = dim3(kAttnThreads);
-        cfg.dynamicSmemBytes = kAttnWarps * kStages * 2 * kTile * kHead * 2 + (p.n_requests + 1) * sizeof(int);
-        if ((e = cudaLaunchKernelEx(&cfg, attention_units_kernel<T, kHead>, p)) != cudaSuccess) return e;
+        cfg.dynamicSmemBytes = kAttnWarps * kStages * 2 * kTile * kHead * 2 + (p.n_requests + 2) * sizeof(int);
+        if ((e = cudaLaunchKernelEx(&cfg, attention_runs_kernel<T, kHead>, p)) != cudaSuccess) return e;
         ++ctx->launches;
         cfg.numAttrs = 1;
     }
@@ -1038,7 +1094,7 @@ int ml2_prefix_attention(ml2_ctx* h, int dtype, void* out, long long out_stride,
         return fail(ML2_E_INVALID, "prefix_attention: pointers must be 16-byte aligned and row strides multiples of 8 elements");
     if (out == query) return fail(ML2_E_INVALID, "prefix_attention: out must not overlap the queries");
     const AttnPlan pl = plan_attention(ctx, n_rows, n_requests, (int)prefix->rows, max_length, n_heads, n_kv_heads, head_size);
-    if (pl.units > INT32_MAX - (1 << 20) || (long long)n_rows * n_heads > INT32_MAX)
+    if (pl.tiles > INT32_MAX / 2 || (long long)n_rows * (n_heads / n_kv_heads) > INT32_MAX / 2 || (long long)n_rows * n_heads > INT32_MAX)
         return fail(ML2_E_INVALID, "prefix_attention: n_rows=%d with %d heads is too much for one call", n_rows, n_heads);
     if (workspace_bytes < pl.bytes || (pl.bytes && !workspace))
         return fail(ML2_E_INVALID, "prefix_attention: the workspace has %zu bytes, %zu are needed", workspace_bytes, pl.bytes);
@@ -1051,9 +1107,10 @@ int ml2_prefix_attention(ml2_ctx* h, int dtype, void* out, long long out_stride,
     p.table_stride = table_stride; p.page_shift = shift; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.group = n_heads / n_kv_heads;
     p.scale_log2 = scale * 1.44269504088896340736f;
     char* ws = static_cast<char*>(workspace);
-    p.pre_o = reinterpret_cast<float*>(ws + pl.pre_o); p.own_o = reinterpret_cast<float*>(ws + pl.own_o);
-    p.pre_ml = reinterpret_cast<float2*>(ws + pl.pre_ml); p.own_ml = reinterpret_cast<float2*>(ws + pl.own_ml);
-    p.prefix_chunk = pl.prefix_chunk; p.prefix_splits = pl.prefix_splits; p.own_chunk = pl.own_chunk; p.prefix_ctas = pl.prefix_ctas;
+    p.pre_o = reinterpret_cast<float*>(ws); p.run_o = reinterpret_cast<float*>(ws + pl.run_o);
+    p.pre_ml = reinterpret_cast<float2*>(ws + pl.pre_ml); p.run_ml = reinterpret_cast<float2*>(ws + pl.run_ml);
+    p.run_base = reinterpret_cast<int*>(ws + pl.run_base);
+    p.prefix_ctas = pl.prefix_ctas; p.run_ctas = pl.run_ctas;
     p.waits = ctx->status_dev; p.wait_cycles = ctx->wait_cycles;
     PrefixMaps maps{};
     if (pl.prefix_ctas && (!make_map(&maps.k, dtype, prefix->key, prefix->row_stride, (int)kv_width, p.prefix) ||
