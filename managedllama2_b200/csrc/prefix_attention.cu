@@ -27,7 +27,7 @@ struct AttnBatch {
     // and an o that is not read. pre: of the prefix by blocks, [segments][rows that are there][n_heads]; run: of the warps' runs.
     float *pre_o, *run_o;
     float2 *pre_ml, *run_ml;
-    int* run_base;      // [n_requests + 1]: key tiles before request r, of all requests; then the tiles of a run
+    int* run_base;      // [n_requests + 1]: places before request r, of all requests; then the places of a run
     long long wait_cycles;
     long long out_stride, q_stride, prefix_stride, cache_stride;
     int n_requests, n_rows, prefix, max_length, n_pages, table_stride, page_shift, n_heads, n_kv, group;
@@ -52,6 +52,7 @@ constexpr int kTile = 16;      // keys of a tile: the k of one m16n8k16 product 
 constexpr int kStages = 3;     // tiles of a warp's ring
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
+constexpr int kOpen = 1;       // what it costs to begin a sequence (its queries, its result), in key tiles: 2300 cycles against 2200
 
 template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
@@ -98,6 +99,7 @@ __device__ __forceinline__ int tiles_seen(const AttnBatch& p, int count, int len
     const int last = (row0 + rows - 1) / p.group, seen = min(length, length - count + last + 1);
     return seen > 0 ? (seen + kTile - 1) / kTile : 0;
 }
+__device__ __forceinline__ int places(int length) { return length ? kOpen + (length + kTile - 1) / kTile : 0; }
 // Where the result of run `run` for the 16 rows from row0 on of a key head begins: runs and rows are numbered through, so that
 // no two results meet and all need no more than one entry per row and head, and 16 per run.
 __device__ __forceinline__ long long result_row(const AttnBatch& p, bool prefix, int first, int row0, int rows, int kvh, int run)
@@ -105,13 +107,14 @@ __device__ __forceinline__ long long result_row(const AttnBatch& p, bool prefix,
     return (prefix ? (long long)p.n_rows * p.n_heads : 0) + ((long long)first * p.group + row0) * p.n_kv + kvh * rows + 16ll * run;
 }
 
-// A walk over the key tiles of one run: 16 rows of one key head and request (a sequence), all its key tiles, then the next.
+// A walk over one run: 16 rows of one key head and request (a sequence), kOpen places for its beginning and one for each of its
+// key tiles, then the next sequence.
 struct Walk {
     int pos, end;              // of all tiles
     int request;               // n_requests: the prefix
-    int rt, kvh, k;            // row tile, key head, key tile
+    int rt, kvh, k;            // row tile, key head, place in the sequence
     int first, count, length;  // query rows and keys of the request
-    int tiles, need, rows;     // key tiles of a sequence, those that its rows see, its rows
+    int places, need, rows;    // places of a sequence, those up to the last key tile that its rows see, its rows
 };
 __device__ __forceinline__ void open_request(const AttnBatch& p, Walk& w, int total_rows)
 {
@@ -125,12 +128,12 @@ __device__ __forceinline__ void open_request(const AttnBatch& p, Walk& w, int to
         w.count = s.count;
         w.length = s.length;
     }
-    w.tiles = (w.length + kTile - 1) / kTile;
+    w.places = places(w.length);
 }
 __device__ __forceinline__ void open_rows(const AttnBatch& p, Walk& w)
 {
     w.rows = min(16, w.count * p.group - w.rt * 16);
-    w.need = w.request == p.n_requests ? w.tiles : tiles_seen(p, w.count, w.length, w.rt * 16, w.rows);
+    w.need = w.request == p.n_requests ? w.places : kOpen + tiles_seen(p, w.count, w.length, w.rt * 16, w.rows);
 }
 __device__ __forceinline__ void open_walk(const AttnBatch& p, const int* s_base, int total_rows, Walk& w)
 {
@@ -143,8 +146,8 @@ __device__ __forceinline__ void open_walk(const AttnBatch& p, const int* s_base,
     }
     w.request = lo;
     open_request(p, w, total_rows);
-    const int local = w.pos - s_base[lo], seq = local / w.tiles;
-    w.k = local - seq * w.tiles;
+    const int local = w.pos - s_base[lo], seq = local / w.places;
+    w.k = local - seq * w.places;
     // key heads, next to one another in the cache, go to neighbouring runs
     w.rt = seq / p.n_kv;
     w.kvh = seq - w.rt * p.n_kv;
@@ -154,8 +157,14 @@ __device__ __forceinline__ void open_walk(const AttnBatch& p, const int* s_base,
 __device__ __forceinline__ bool settle(const AttnBatch& p, const int* s_base, int total_rows, Walk& w)
 {
     while (w.pos < w.end) {
+        if (w.k < kOpen) {
+            const int n = min(kOpen - w.k, w.end - w.pos);
+            w.k += n;
+            w.pos += n;
+            continue;
+        }
         if (w.k < w.need) return true;
-        w.pos += w.tiles - w.k;
+        w.pos += w.places - w.k;
         w.k = 0;
         if (w.pos >= w.end) return false;
         if (++w.kvh < p.n_kv) continue;
@@ -171,8 +180,8 @@ __device__ __forceinline__ bool settle(const AttnBatch& p, const int* s_base, in
     return false;
 }
 
-// Every warp works for itself: the key tiles of all requests, one after the other, are cut into runs of the same length, one
-// a warp. It streams its tiles through a ring of its own (cp.async; the next two are under way while one is used, across the
+// Every warp works for itself: the key tiles of all requests, one after the other, and one place more for every sequence, are
+// cut into runs of the same length, one a warp (without that place runs through short requests took 1.5 times as long). It streams its tiles through a ring of its own (cp.async; the next two are under way while one is used, across the
 // borders of sequences) and leaves a result for every sequence that it has a part of. 16 rows are all the tensor core's m16
 // has, so a tile of 16 keys (8 KB at head 128) costs 32 products however few rows are real; at one row HBM still bounds it.
 template <typename T, int kHead>
@@ -182,13 +191,13 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
     extern __shared__ __align__(128) unsigned char s_mem[];
     __shared__ unsigned s_valid[kAttnWarps][kStages];
     __shared__ int s_sum[kAttnWarps];
-    int* s_base = reinterpret_cast<int*>(s_mem + kAttnWarps * kStages * 2 * kTileBytes);  // tiles before request r; the prefix last
+    int* s_base = reinterpret_cast<int*>(s_mem + kAttnWarps * kStages * 2 * kTileBytes);  // places before request r; the prefix last
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // after the prefix kernel, which has waited for what comes before both, this one starts beside it
     if (!p.prefix_ctas) pdl_wait();
     const int total_rows = min(max(p.query_start[p.n_requests], 0), p.n_rows);
-    // ---- how many tiles every request has -----------------------------------------------------------------------------
+    // ---- how many places every request has -----------------------------------------------------------------------------
     {
         const int per = ceil_div(p.n_requests, kAttnThreads), r0 = min((int)threadIdx.x * per, p.n_requests), r1 = min(r0 + per, p.n_requests);
         int mine = 0;
@@ -196,7 +205,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
             const Span s = request_span(p, r);
             if (!s.good && blockIdx.x == 0) report_input_error(p.status, kInputLength, r);
             s_base[r] = mine;
-            mine += row_tiles(p, s.count) * p.n_kv * ((s.length + kTile - 1) / kTile);
+            mine += row_tiles(p, s.count) * p.n_kv * places(s.length);
         }
         int incl = mine;
 #pragma unroll
@@ -215,7 +224,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
         for (int r = r0; r < r1; ++r) s_base[r] += base;
         if (threadIdx.x == 0) {
             s_base[p.n_requests] = all;
-            s_base[p.n_requests + 1] = all + (p.prefix_ctas ? 0 : row_tiles(p, total_rows) * p.n_kv * ((p.prefix + kTile - 1) / kTile));
+            s_base[p.n_requests + 1] = all + (p.prefix_ctas ? 0 : row_tiles(p, total_rows) * p.n_kv * places(p.prefix));
         }
         __syncthreads();
     }
@@ -238,7 +247,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
     bool more = settle(p, s_base, total_rows, ld);
     long long row = -1;  // lanes 0..15: cache row of the tile's key `lane`, -1 for none
     auto find_rows = [&]() {
-        const int key = ld.k * kTile + (lane & 15);
+        const int key = (ld.k - kOpen) * kTile + (lane & 15);
         row = -1;
         if (key < ld.length) {
             if (ld.request == p.n_requests) row = key;
@@ -283,9 +292,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
     const int g = lane >> 2, t4 = lane & 3;
     while (settle(p, s_base, total_rows, w)) {
         const bool prefix = w.request == p.n_requests;
-        const int tile0 = w.k, tile1 = min(w.need, w.k + (w.end - w.pos)), row0 = w.rt * 16;
-        w.pos += tile1 - tile0;
-        w.k = tile1;
+        const int n_tiles = min(w.need - w.k, w.end - w.pos), key0 = (w.k - kOpen) * kTile, row0 = w.rt * 16;
+        w.pos += n_tiles;
+        w.k += n_tiles;
 
         // rows g and g + 8 of the tile: query row, head, and the keys they see
         const int m0 = row0 + g, m1 = m0 + 8;
@@ -312,7 +321,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
         for (int n = 0; n < kHead / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
         float mx0 = -INFINITY, mx1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
-        for (int key = tile0 * kTile; key < tile1 * kTile; key += kTile) {
+        for (int key = key0; key < key0 + n_tiles * kTile; key += kTile) {
             cp_async_wait<kStages - 2>();
             __syncwarp();
             const uint32_t kt = ring_u32 + stage * 2 * kTileBytes, vt = kt + kTileBytes;
@@ -453,7 +462,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
 // cut into one contiguous run per CTA, so all CTAs do the same work within one tile and a block's runs ("segments") are
 // joined afterwards. Two streams of a CTA alternate on the tensor core:
 //   S = Q K^T (operands in shared memory, S in TMEM, two of them a stream: one is filled while the other is used),
-//   P = exp2(S - m), rounded to 16 bits, over S in TMEM   (128 threads, one row each: no exchange between threads)
+//   P = exp2(S - m), rounded to 16 bits, over S in TMEM   (256 threads, half a row each; with 128 the exponentials' latency
+//                                                          was open: 70 us instead of @@ for 1024 rows and 16384 keys of 8 heads)
 //   O += P V (P from TMEM, V as it lies: MN-major)
 // With more than 128 rows both streams use each key tile, the first with rows 0..127, the second with 128..255. With fewer,
 // both have the same rows and take the key tiles in turn: then HBM bounds the kernel and eight tiles of 16 KB are under way.
@@ -462,7 +472,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
 constexpr int kBlockRows = 256;
 constexpr int kKeyTile = 64;
 constexpr int kRing = 8;                 // key or value tiles in shared memory
-constexpr int kBlockThreads = 352;       // per stream 4 softmax warps and one that feeds the tensor core; load warp
+constexpr int kBlockThreads = 608;       // per stream 8 softmax warps and one that feeds the tensor core; load warp
 constexpr float kSlack = 8.f;
 constexpr int kBlockPrefix = 512;        // from this length on the prefix is done by blocks
 
@@ -514,6 +524,17 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
     return d;
 }
 
+// Barrier of the two warps `id`; true when `flag` is for any thread of them.
+__device__ __forceinline__ bool pair_any(int id, bool flag)
+{
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %3, 0;\n\tbar.red.or.pred p, %1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(any)
+                 : "r"(id), "r"(64), "r"((uint32_t)flag)
+                 : "memory");
+    return any != 0;
+}
+
 template <typename T, int kHead>
 __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(const __grid_constant__ AttnBatch p, const __grid_constant__ PrefixMaps maps)
 {
@@ -521,6 +542,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ unsigned char s_raw[];
     __shared__ uint64_t b_full[kRing], b_empty[kRing], b_q[2], b_s[2][2], b_p[2][2], b_o[2][2], b_end[2];
+    __shared__ float s_top[2][2][128];  // of a stream's half rows, when they have to agree on m, and their sums
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     const uint32_t q_base = (smem_u32(s_raw) + 1023u) & ~1023u, ring = q_base + 2 * S::kQBytes;
@@ -533,18 +555,18 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&b_end[i], 1);
-            mbar_init(&b_q[i], 4);  // one arrival a warp
+            mbar_init(&b_q[i], 8);  // one arrival a warp
             for (int j = 0; j < 2; ++j) {
                 mbar_init(&b_o[i][j], 1);
                 mbar_init(&b_s[i][j], 1);
-                mbar_init(&b_p[i][j], 4);
+                mbar_init(&b_p[i][j], 8);
             }
         }
         s_abort = 0;
         mbar_fence_init();
     }
-    if (warp == 8) tmem_alloc(&s_tmem, 512);
-    if (warp == 10 && lane == 0) {
+    if (warp == 16) tmem_alloc(&s_tmem, 512);
+    if (warp == 18 && lane == 0) {
         tma_prefetch_map(&maps.k);
         tma_prefetch_map(&maps.v);
     }
@@ -579,7 +601,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
     // tiles of a stream in a segment
     auto share = [](bool turns, int n, int stream) { return turns ? (n + 1 - stream) >> 1 : n; };
 
-    if (warp == 10) {
+    if (warp == 18) {
         // ---- loads, in the order of their first use ------------------------------------------------------------------
         if (lane == 0) {
             unsigned count = 0;
@@ -611,13 +633,13 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
             }
         }
         __syncwarp();
-    } else if (warp >= 8) {
+    } else if (warp >= 16) {
         // ---- the tensor core's queue, one thread for each stream ------------------------------------------------------
         // (One for both was slower than the products: its own instructions, some 700 cycles for the eight or four products of
         // a tile, bounded the kernel.)
         if (lane == 0) {
             constexpr uint32_t kShapeS = tc_shape(128, kKeyTile, kBf16, false), kShapeO = tc_shape(128, kHead, kBf16, true);
-            const int s = warp - 8;
+            const int s = warp - 16;
             const uint32_t q_op = tc_operand_low(q_base + s * S::kQBytes, 16), k_op = tc_operand_low(ring, 16), v_op = tc_operand_low(ring, S::kHalf);
             const uint32_t t_s = tmem + s * 128, t_o = tmem + 256 + s * 128;
             unsigned count = 0;               // ring position of the next tile
@@ -678,18 +700,24 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
         }
         __syncwarp();
     } else {
-        // ---- softmax: one row a thread -----------------------------------------------------------------------------------
-        const int s = warp >> 2, row = threadIdx.x & 127;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_o = tmem + 256 + s * 128 + lanes;
+        // ---- softmax: half a row a thread, two warps for 32 rows -----------------------------------------------------------
+        // These warps never leave early: after a wait that ran out they go through the rest without waiting and write nothing,
+        // so that nobody is missed at the barriers of two warps.
+        const int s = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane, pair = 1 + s * 4 + quarter;
+        const uint32_t lanes = (uint32_t)quarter << 21, t_o = tmem + 256 + s * 128 + half * (kHead / 2) + lanes;
         const uint32_t q_tile = q_base + s * S::kQBytes;
         // its sign goes into Q, so that the largest S is the largest score; never 0, so that -inf stays -inf
         const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);
         const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
         const uint64_t scale2 = two(scale, scale);
         unsigned used = 0;  // S tiles of this stream since the start
+        bool dead = false;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait_for(bar, parity, p.wait_cycles, &s_abort));
+        };
         // The product before the present S tile is done. Two barriers in turn, as for S and P: one of them never completes a
         // second phase before this thread has seen the first.
-        auto o_done = [&]() { return mbar_wait_for(&b_o[s][(used - 1) & 1], ((used - 1) >> 1) & 1, p.wait_cycles, &s_abort); };
+        auto o_done = [&]() { wait(&b_o[s][(used - 1) & 1], ((used - 1) >> 1) & 1); };
         for_segments([&](int kvh, int block, int tile, int n) {
             const bool turns = runs.rows - block * kBlockRows <= kBlockRows / 2;
             const int ns = share(turns, n, s);
@@ -697,20 +725,20 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
             // this thread's row, and what lies before it in the queries and in the results; others ask for theirs by shuffle
             const int mrow = first_row + row, trow = mrow / p.group, hrow = kvh * p.group + mrow % p.group;
             const long long q_at = trow * p.q_stride + (long long)hrow * kHead, at_row = (long long)trow * p.n_heads + hrow;
-            // this warp's 32 rows of Q, sixteen bytes a lane: what the stream's earlier products read is done with
+            // this warp's 16 rows of Q, sixteen bytes a lane: what the stream's earlier products read is done with
             if (ns) {
-                constexpr int kVec = kHead / 8, kLoads = kVec;  // 16-byte vectors of a row; 32 rows of them are kVec a lane
+                constexpr int kVec = kHead / 8, kLoads = kVec / 2;  // 16-byte vectors of a row; 16 rows of them are kVec / 2 a lane
                 uint4 v[kLoads];
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    const int r = (i * 32 + lane) / kVec, c = lane % kVec;
+                    const int r = half * 16 + (i * 32 + lane) / kVec, c = lane % kVec;
                     const long long at = __shfl_sync(0xffffffffu, q_at, r);
                     v[i] = make_uint4(0, 0, 0, 0);
-                    if ((warp & 3) * 32 + r < rows) v[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + at + c * 8);
+                    if (quarter * 32 + r < rows) v[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + at + c * 8);
                 }
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    const int r = (warp & 3) * 32 + (i * 32 + lane) / kVec, c = lane % kVec;
+                    const int r = quarter * 32 + half * 16 + (i * 32 + lane) / kVec, c = lane % kVec;
                     const uint32_t to = q_tile + (c >> 3) * S::kQHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
                     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v[i].x ^ sign), "r"(v[i].y ^ sign), "r"(v[i].z ^ sign),
                                  "r"(v[i].w ^ sign)
@@ -721,37 +749,36 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                 if (lane == 0) mbar_arrive(&b_q[s]);
             }
 
-            const bool busy = (warp & 3) * 32 < rows;  // warps without rows only keep step
+            const bool busy = quarter * 32 < rows;  // warps without rows only keep step
             float m = -INFINITY;
             uint64_t sum[2] = {0, 0};
             for (int j = 0; j < ns; ++j, ++used) {
-                if (!__all_sync(0xffffffffu, mbar_wait_for(&b_s[s][used & 1], (used >> 1) & 1, p.wait_cycles, &s_abort))) return false;
+                wait(&b_s[s][used & 1], (used >> 1) & 1);
                 tc_fence_after();
                 if (busy) {
                     const uint32_t t_s = tmem + s * 128 + (used & 1) * 64 + lanes;
-                    uint32_t x[2][32];
-                    tmem_ld32(t_s, x[0]);
-                    tmem_ld32(t_s + 32, x[1]);
+                    uint32_t x[32];
+                    tmem_ld32(t_s + half * 32, x);
                     tmem_wait_ld();
-                    const int left = p.prefix - (tile + (turns ? 2 * j + s : j)) * kKeyTile;  // keys from this tile on
-                    if (left < kKeyTile) {
+                    const int left = p.prefix - (tile + (turns ? 2 * j + s : j)) * kKeyTile - half * 32;  // keys from these on
+                    if (left < 32) {
 #pragma unroll
-                        for (int c = 0; c < 2; ++c)
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (c * 32 + e >= left) x[c][e] = 0xff800000u;
+                        for (int e = 0; e < 32; ++e)
+                            if (e >= left) x[e] = 0xff800000u;
                     }
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                    for (int e = 0; e < 32; e += 8)
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) top[i] = fmaxf(fmaxf(top[i], __uint_as_float(x[c][e + 2 * i])), __uint_as_float(x[c][e + 2 * i + 1]));
+                        for (int i = 0; i < 4; ++i) top[i] = fmaxf(fmaxf(top[i], __uint_as_float(x[e + 2 * i])), __uint_as_float(x[e + 2 * i + 1]));
                     float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                     t = t == -INFINITY ? t : t * scale;
-                    const bool move = t > m + kSlack || m == -INFINITY;
-                    if (__any_sync(0xffffffffu, move)) {
+                    // both halves have their S in registers after this barrier, so P may go over it
+                    if (pair_any(pair, t > m + kSlack || m == -INFINITY)) {
+                        s_top[s][half][row] = t;
+                        named_bar_sync(pair, 64);
+                        t = fmaxf(t, s_top[s][half ^ 1][row]);
+                        const bool move = t > m + kSlack || m == -INFINITY;
                         const float to = move ? t : m, ref = to == -INFINITY ? 0.f : to, c = move ? exp2_fast(m - ref) : 1.f;
                         m = to;
                         const uint64_t c2 = two(c, c);
@@ -759,10 +786,10 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                         sum[1] = fma2(sum[1], c2, 0);
                         if (j > 0) {
                             // O is at rest between the product before (waited for here) and the one that waits for this P
-                            if (!__all_sync(0xffffffffu, o_done())) return false;
+                            o_done();
                             tc_fence_after();
 #pragma unroll 1
-                            for (int d = 0; d < kHead; d += 32) {
+                            for (int d = 0; d < kHead / 2; d += 32) {
                                 uint32_t o[32];
                                 tmem_ld32(t_o + d, o);
                                 tmem_wait_ld();
@@ -774,16 +801,15 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                     }
                     const float ref = m == -INFINITY ? 0.f : -m;
                     const uint64_t ref2 = two(ref, ref);
-                    uint32_t w[32];
+                    uint32_t w[16];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int c = e / 16, f = (e % 16) * 2;
-                        const float2 y = apart(fma2((uint64_t)x[c][f + 1] << 32 | x[c][f], scale2, ref2));
+                    for (int e = 0; e < 16; ++e) {
+                        const float2 y = apart(fma2((uint64_t)x[2 * e + 1] << 32 | x[2 * e], scale2, ref2));
                         const float a = exp2_fast(y.x), b = exp2_fast(y.y);
                         sum[e & 1] = add2(sum[e & 1], two(a, b));
                         w[e] = pack2<T>(a, b);
                     }
-                    tmem_st32(t_s, w);
+                    tmem_st16(t_s + half * 16, w);
                     tmem_wait_st();
                 }
                 tc_fence_before();
@@ -796,38 +822,42 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
             block_segments(runs, kvh, block, &first, &results);
             const int split = turns ? 2 * ((int)blockIdx.x - first) + s : (int)blockIdx.x - first;
             if (ns) {
-                if (!__all_sync(0xffffffffu, o_done())) return false;
+                o_done();
                 tc_fence_after();
             }
             if (busy) {
+                const long long results_at = (long long)split * total_rows * p.n_heads;
                 const float2 l2 = apart(add2(sum[0], sum[1]));
-                if (row < rows) p.pre_ml[(long long)split * total_rows * p.n_heads + at_row] = make_float2(m, l2.x + l2.y);
+                if (half) s_top[s][1][row] = l2.x + l2.y;
+                named_bar_sync(pair, 64);
+                if (!half && row < rows && !dead) p.pre_ml[results_at + at_row] = make_float2(m, l2.x + l2.y + s_top[s][1][row]);
+                named_bar_sync(pair, 64);
                 if (ns) {
-                    // through this warp's own 32 rows of the Q tile (other warps may have the next segment's rows in theirs), 32
-                    // dims at a time, so that rows leave in whole lines
-                    const uint32_t mine = q_tile + (warp & 3) * 32 * 128;
+                    // through this warp's own 16 rows of the Q tile (others may have the next segment's rows in theirs), 16 dims
+                    // at a time, so that rows leave in pieces of 64 bytes
+                    const uint32_t mine = q_tile + quarter * 32 * 128 + half * 16 * 128;
 #pragma unroll 1
-                    for (int d = 0; d < kHead; d += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(t_o + d, o);
+                    for (int d = 0; d < kHead / 2; d += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(t_o + d, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(mine + lane * 128 + (((e >> 2) ^ (lane & 7)) << 4)), "r"(o[e]),
+                        for (int e = 0; e < 16; e += 4)
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(mine + lane * 64 + (((e >> 2) ^ ((lane >> 1) & 3)) << 4)), "r"(o[e]),
                                          "r"(o[e + 1]), "r"(o[e + 2]), "r"(o[e + 3])
                                          : "memory");
                         __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int r = i * 4 + (lane >> 3), c = lane & 7;
+                        for (int i = 0; i < 4; ++i) {
+                            const int r = i * 8 + (lane >> 2), c = lane & 3;
                             const long long at = __shfl_sync(0xffffffffu, at_row, r);
                             uint4 v;
                             asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                                          : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                         : "r"(mine + r * 128 + ((c ^ (r & 7)) << 4))
+                                         : "r"(mine + r * 64 + ((c ^ ((r >> 1) & 3)) << 4))
                                          : "memory");
-                            if ((warp & 3) * 32 + r < rows)
-                                *reinterpret_cast<uint4*>(p.pre_o + ((long long)split * total_rows * p.n_heads + at) * kHead + d + c * 4) = v;
+                            if (quarter * 32 + r < rows && !dead)
+                                *reinterpret_cast<uint4*>(p.pre_o + (results_at + at) * kHead + half * (kHead / 2) + d + c * 4) = v;
                         }
                         __syncwarp();
                     }
@@ -840,7 +870,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
     __syncthreads();
     if (threadIdx.x == 0 && s_abort) atomicCAS(&p.waits->error, 0u, kAttentionGaveUp);
     tc_fence_after();
-    if (warp == 8) tmem_free(tmem, 512);
+    if (warp == 16) tmem_free(tmem, 512);
 }
 
 // Joins the partial results of one row and head: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. One warp each.
@@ -878,9 +908,9 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     if (p.run_ctas) {
         const int per = max(p.run_base[p.n_requests + 1], 1);
         if (!p.prefix_ctas && p.prefix) {
-            const int m = t * p.group + g, row0 = m & ~15, rows = min(16, total_rows * p.group - row0), tiles = (p.prefix + kTile - 1) / kTile;
-            const int a = p.run_base[p.n_requests] + ((row0 >> 4) * p.n_kv + kvh) * tiles, first = a / per;
-            pre = (a + tiles - 1) / per - first + 1;
+            const int m = t * p.group + g, row0 = m & ~15, rows = min(16, total_rows * p.group - row0), n = places(p.prefix);
+            const int a = p.run_base[p.n_requests] + ((row0 >> 4) * p.n_kv + kvh) * n, first = (a + kOpen) / per;
+            pre = (a + n - 1) / per - first + 1;
             pre_at = result_row(p, true, 0, row0, rows, kvh, first) + (m & 15);
             pre_step = 16;
             pre_o = p.run_o;
@@ -888,8 +918,8 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
         }
         const Span s = request_span(p, lo);
         if (s.good && t >= s.first && t < s.first + s.count && s.length > 0) {
-            const int m = (t - s.first) * p.group + g, row0 = m & ~15, rows = min(16, s.count * p.group - row0), tiles = (s.length + kTile - 1) / kTile;
-            const int a = p.run_base[lo] + ((row0 >> 4) * p.n_kv + kvh) * tiles, first = a / per, need = tiles_seen(p, s.count, s.length, row0, rows);
+            const int m = (t - s.first) * p.group + g, row0 = m & ~15, rows = min(16, s.count * p.group - row0);
+            const int a = p.run_base[lo] + ((row0 >> 4) * p.n_kv + kvh) * places(s.length) + kOpen, first = a / per, need = tiles_seen(p, s.count, s.length, row0, rows);
             own = need ? (a + need - 1) / per - first + 1 : 0;
             own_at = result_row(p, false, s.first, row0, rows, kvh, first) + (m & 15);
         }
@@ -956,7 +986,7 @@ static AttnPlan plan_attention(const Ctx* ctx, int n_rows, int n_requests, int p
     if (!n_rows) return pl;
     const int sms = std::max(1, ctx->sm_count);
     const long long rows = (long long)n_rows * (n_heads / n_kv);  // of a key head
-    long long pre_rows = 0, run_rows = 0, run_tiles = (n_requests + rows / 16) * n_kv * ceil_div(max_length, kTile);
+    long long pre_rows = 0, run_rows = 0, run_tiles = (n_requests + rows / 16) * n_kv * (max_length ? kOpen + ceil_div(max_length, kTile) : 0);
     if (prefix >= kBlockPrefix) {
         const long long blocks = (rows + kBlockRows - 1) / kBlockRows, key_tiles = ceil_div(prefix, kKeyTile);
         pl.tiles = blocks * n_kv * key_tiles;
@@ -965,7 +995,7 @@ static AttnPlan plan_attention(const Ctx* ctx, int n_rows, int n_requests, int p
         // tiles, a block at most ctas / (n_kv b) + 2 segments and never more than key tiles, and a segment two results.
         pre_rows = std::min(512ll * pl.prefix_ctas + 1024ll * blocks * n_kv, 2 * key_tiles * n_rows * n_heads);
     } else {
-        run_tiles += (rows + 15) / 16 * n_kv * ceil_div(prefix, kTile);
+        run_tiles += (rows + 15) / 16 * n_kv * (prefix ? kOpen + ceil_div(prefix, kTile) : 0);
     }
     pl.tiles = std::max(pl.tiles, run_tiles);
     pl.run_ctas = (int)std::min<long long>(2 * sms, (run_tiles + kAttnWarps - 1) / kAttnWarps);
