@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
 // sums are fp32): O is rescaled in TMEM a few times in all instead of at every tile.
 constexpr int kBlockRows = 256;
 constexpr int kKeyTile = 64;
-constexpr int kRing = 8;                 // key or value tiles in shared memory
+constexpr int kRing = 4;                 // key tiles in shared memory, and value tiles
 constexpr int kBlockThreads = 608;       // per stream 8 softmax warps and one that feeds the tensor core; load warp
 constexpr float kSlack = 8.f;
 constexpr int kBlockPrefix = 512;        // from this length on the prefix is done by blocks
@@ -505,7 +505,7 @@ __device__ __forceinline__ void block_segments(const PrefixRuns& r, int kvh, int
 template <int kHead> struct BlockSmem {
     static constexpr int kQHalf = 128 * 128, kQBytes = kQHalf * (kHead / 64);            // 64 dims of 128 rows, 128-byte swizzle
     static constexpr int kHalf = kKeyTile * 128, kTileBytes = kHalf * (kHead / 64);      // 64 dims of a key or value tile
-    static constexpr int kBytes = 1024 + 2 * kQBytes + kRing * kTileBytes;
+    static constexpr int kBytes = 1024 + 2 * kQBytes + 2 * kRing * kTileBytes;
 };
 
 // a * b + c, a + b on two fp32 values at once
@@ -541,26 +541,30 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
     using S = BlockSmem<kHead>;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ unsigned char s_raw[];
-    __shared__ uint64_t b_full[kRing], b_empty[kRing], b_q[2], b_s[2][2], b_p[2][2], b_o[2][2], b_end[2];
+    // Tile g of the CTA's run (counted over all segments) has key and value slot g % kRing. b_k, b_v: it has landed. b_s, b_o, for
+    // each stream: its scores or its product with the values are done, which also frees the slot; a stream that does not use the
+    // tile arrives there as well. A commit costs the feeding thread 90 cycles, so each serves both ends.
+    __shared__ uint64_t b_k[kRing], b_v[kRing], b_s[2][kRing], b_o[2][kRing], b_q[2], b_p[2][2], b_end[2];
     __shared__ float s_top[2][2][128];  // of a stream's half rows, when they have to agree on m, and their sums
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    const uint32_t q_base = (smem_u32(s_raw) + 1023u) & ~1023u, ring = q_base + 2 * S::kQBytes;
+    const uint32_t q_base = (smem_u32(s_raw) + 1023u) & ~1023u, k_ring = q_base + 2 * S::kQBytes, v_ring = k_ring + kRing * S::kTileBytes;
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // uniform, and known to be
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kRing; ++i) {
-            mbar_init(&b_full[i], 1);
-            mbar_init(&b_empty[i], 2);  // one from each stream
+            mbar_init(&b_k[i], 1);
+            mbar_init(&b_v[i], 1);
+            for (int j = 0; j < 2; ++j) {
+                mbar_init(&b_s[j][i], 1);
+                mbar_init(&b_o[j][i], 1);
+            }
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&b_end[i], 1);
             mbar_init(&b_q[i], 8);  // one arrival a warp
-            for (int j = 0; j < 2; ++j) {
-                mbar_init(&b_o[i][j], 1);
-                mbar_init(&b_s[i][j], 1);
-                mbar_init(&b_p[i][j], 8);
-            }
+            mbar_init(&b_p[i][0], 8);
+            mbar_init(&b_p[i][1], 8);
+            mbar_init(&b_end[i], 1);
         }
         s_abort = 0;
         mbar_fence_init();
@@ -604,32 +608,40 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
     if (warp == 18) {
         // ---- loads, in the order of their first use ------------------------------------------------------------------
         if (lane == 0) {
-            unsigned count = 0;
-            auto load = [&](const CUtensorMap* map, int kvh, int tile) {
-                const unsigned slot = count % kRing, turn = count / kRing;
-                if (!mbar_wait_for(&b_empty[slot], (turn & 1) ^ 1, p.wait_cycles, &s_abort)) return false;
-                mbar_arrive_expect_tx(&b_full[slot], S::kTileBytes);
+            unsigned base = 0, keys = 0, vals = 0;  // first tile of the segment; tiles asked for
+            auto load = [&](bool key, int kvh, int tile, unsigned g) {
+                const unsigned slot = g % kRing, parity = (g / kRing & 1) ^ 1;
+                for (int s = 0; s < 2; ++s)
+                    if (!mbar_wait_for(key ? &b_s[s][slot] : &b_o[s][slot], parity, p.wait_cycles, &s_abort)) return false;
+                uint64_t* full = key ? &b_k[slot] : &b_v[slot];
+                mbar_arrive_expect_tx(full, S::kTileBytes);
 #pragma unroll
                 for (int h = 0; h < kHead / 64; ++h)
-                    tma_load_2d(ring + slot * S::kTileBytes + h * S::kHalf, map, kvh * kHead + h * 64, tile * kKeyTile, &b_full[slot]);
-                ++count;
+                    tma_load_2d((key ? k_ring : v_ring) + slot * S::kTileBytes + h * S::kHalf, key ? &maps.k : &maps.v, kvh * kHead + h * 64,
+                                tile * kKeyTile, full);
+                ++(key ? keys : vals);
                 return true;
             };
             const bool done = for_segments([&](int kvh, int block, int tile, int n) {
                 const int step = runs.rows - block * kBlockRows <= kBlockRows / 2 ? 2 : 1;
-                auto loads = [&](const CUtensorMap* map, int j) {
+                auto loads = [&](bool key, int j) {
                     for (int t = j * step; t < min(n, (j + 1) * step); ++t)
-                        if (!load(map, kvh, tile + t)) return false;
+                        if (!load(key, kvh, tile + t, base + t)) return false;
                     return true;
                 };
-                if (!loads(&maps.k, 0)) return false;
+                if (!loads(true, 0)) return false;
                 for (int j = 0; j * step < n; ++j)
-                    if (!loads(&maps.k, j + 1) || !loads(&maps.v, j)) return false;
+                    if (!loads(true, j + 1) || !loads(false, j)) return false;
+                base += n;
                 return true;
             });
             if (!done) {  // copies that are under way land before this CTA leaves
-                for (unsigned c = count > kRing ? count - kRing : 0; c < count; ++c)
-                    for (int i = 0; i < 1 << 20 && !mbar_try_wait(&b_full[c % kRing], (c / kRing) & 1); ++i) {}
+                auto land = [&](uint64_t* full, unsigned n) {
+                    for (unsigned g = n > kRing ? n - kRing : 0; g < n; ++g)
+                        for (int i = 0; i < 1 << 20 && !mbar_try_wait(&full[g % kRing], g / kRing & 1); ++i) {}
+                };
+                land(b_k, keys);
+                land(b_v, vals);
             }
         }
         __syncwarp();
@@ -640,57 +652,61 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
         if (lane == 0) {
             constexpr uint32_t kShapeS = tc_shape(128, kKeyTile, kBf16, false), kShapeO = tc_shape(128, kHead, kBf16, true);
             const int s = warp - 16;
-            const uint32_t q_op = tc_operand_low(q_base + s * S::kQBytes, 16), k_op = tc_operand_low(ring, 16), v_op = tc_operand_low(ring, S::kHalf);
+            const uint32_t q_op = tc_operand_low(q_base + s * S::kQBytes, 16), k_op = tc_operand_low(k_ring, 16), v_op = tc_operand_low(v_ring, S::kHalf);
             const uint32_t t_s = tmem + s * 128, t_o = tmem + 256 + s * 128;
-            unsigned count = 0;               // ring position of the next tile
+            unsigned base = 0;                // first tile of the segment
             unsigned asked = 0, added = 0;    // S tiles queued since the start, and P tiles used
             unsigned turn_q = 0;              // Q tiles taken
             const bool done = for_segments([&](int, int block, int, int n) {
                 const bool turns = runs.rows - block * kBlockRows <= kBlockRows / 2;
                 const int step = turns ? 2 : 1;
-                // Step j's key or value tiles, in the order of their loads. Each stream looks at every tile, and lets go at once
-                // of one that is the other's: who skipped a tile could take an earlier phase of its barrier for a later one.
-                auto visit = [&](int j, auto&& use) {
+                // Step j's key or value tiles. Each stream looks at every tile, and lets go at once of one that is the other's: who
+                // skipped a tile could take an earlier phase of its barrier for a later one.
+                auto scores = [&](int j) {
                     for (int t = j * step; t < min(n, (j + 1) * step); ++t) {
-                        const unsigned slot = count % kRing, parity = (count / kRing) & 1;
-                        ++count;
-                        if (!mbar_wait_for(&b_full[slot], parity, p.wait_cycles, &s_abort)) return false;
-                        if (turns && (t & 1) != s) mbar_arrive(&b_empty[slot]);
-                        else {
-                            if (!use(slot)) return false;
-                            tc_commit(&b_empty[slot]);
+                        const unsigned g = base + t, slot = g % kRing;
+                        if (!mbar_wait_for(&b_k[slot], g / kRing & 1, p.wait_cycles, &s_abort)) return false;
+                        if (turns && (t & 1) != s) {
+                            mbar_arrive(&b_s[s][slot]);
+                            continue;
                         }
+                        tc_fence_after();
+                        const uint32_t k = k_op + slot * (S::kTileBytes >> 4), to = t_s + (asked++ & 1) * 64;
+#pragma unroll
+                        for (int i = 0; i < kHead / 16; ++i)
+                            tc_mma_ss(to, tc_operand_at(q_op + (i / 4) * (S::kQHalf >> 4) + (i % 4) * 2),
+                                      tc_operand_at(k + (i / 4) * (S::kHalf >> 4) + (i % 4) * 2), kShapeS, i > 0);
+                        tc_commit(&b_s[s][slot]);
                     }
                     return true;
                 };
-                auto scores = [&](unsigned slot) {
-                    tc_fence_after();
-                    const uint32_t k = k_op + slot * (S::kTileBytes >> 4), to = t_s + (asked & 1) * 64;
+                uint32_t add = 0;
+                auto values = [&](int j) {
+                    for (int t = j * step; t < min(n, (j + 1) * step); ++t) {
+                        const unsigned g = base + t, slot = g % kRing;
+                        if (!mbar_wait_for(&b_v[slot], g / kRing & 1, p.wait_cycles, &s_abort)) return false;
+                        if (turns && (t & 1) != s) {
+                            mbar_arrive(&b_o[s][slot]);
+                            continue;
+                        }
+                        if (!mbar_wait_for(&b_p[s][added & 1], added >> 1 & 1, p.wait_cycles, &s_abort)) return false;
+                        tc_fence_after();
+                        const uint32_t v = v_op + slot * (S::kTileBytes >> 4), from = t_s + (added++ & 1) * 64;
+                        tc_mma_ts(t_o, from, tc_operand_at(v), kShapeO, add);
 #pragma unroll
-                    for (int i = 0; i < kHead / 16; ++i)
-                        tc_mma_ss(to, tc_operand_at(q_op + (i / 4) * (S::kQHalf >> 4) + (i % 4) * 2), tc_operand_at(k + (i / 4) * (S::kHalf >> 4) + (i % 4) * 2),
-                                  kShapeS, i > 0);
-                    tc_commit(&b_s[s][asked++ & 1]);
-                    return true;
-                };
-                bool first = true;
-                auto values = [&](unsigned slot) {
-                    if (!mbar_wait_for(&b_p[s][added & 1], (added >> 1) & 1, p.wait_cycles, &s_abort)) return false;
-                    tc_fence_after();
-                    const uint32_t v = v_op + slot * (S::kTileBytes >> 4), from = t_s + (added & 1) * 64;
-                    tc_mma_ts(t_o, from, tc_operand_at(v), kShapeO, !first);
-#pragma unroll
-                    for (int k = 1; k < kKeyTile / 16; ++k) tc_mma_ts(t_o, from + k * 8, tc_operand_at(v + k * (2048 >> 4)), kShapeO, 1);
-                    tc_commit(&b_o[s][added++ & 1]);
-                    first = false;
+                        for (int k = 1; k < kKeyTile / 16; ++k) tc_mma_ts(t_o, from + k * 8, tc_operand_at(v + k * (2048 >> 4)), kShapeO, 1);
+                        tc_commit(&b_o[s][slot]);
+                        add = 1;
+                    }
                     return true;
                 };
                 // a stream without tiles hands over no Q: it could be two phases ahead of this wait otherwise
                 if (share(turns, n, s) && !mbar_wait_for(&b_q[s], turn_q++ & 1, p.wait_cycles, &s_abort)) return false;
-                if (!visit(0, scores)) return false;
+                if (!scores(0)) return false;
                 // S of the next step goes where P of the one before lay: behind the product that reads it
                 for (int j = 0; j * step < n; ++j)
-                    if (!visit(j + 1, scores) || !visit(j, values)) return false;
+                    if (!scores(j + 1) || !values(j)) return false;
+                base += n;
                 return true;
             });
             if (!done) {  // products that are under way end before the TMEM is given back
@@ -715,9 +731,11 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait_for(bar, parity, p.wait_cycles, &s_abort));
         };
-        // The product before the present S tile is done. Two barriers in turn, as for S and P: one of them never completes a
-        // second phase before this thread has seen the first.
-        auto o_done = [&]() { wait(&b_o[s][(used - 1) & 1], ((used - 1) >> 1) & 1); };
+        unsigned base = 0;  // first tile of the segment
+        // The stream's product with the values of tile g is done. Not asked for before the one of tile g - 4 is seen to be done, and
+        // the slot is not used again before this: a block has at least eight tiles (kBlockPrefix), so that a stream has no tile only
+        // in a run's first or last segment.
+        auto o_done = [&](unsigned g) { wait(&b_o[s][g % kRing], g / kRing & 1); };
         for_segments([&](int kvh, int block, int tile, int n) {
             const bool turns = runs.rows - block * kBlockRows <= kBlockRows / 2;
             const int ns = share(turns, n, s);
@@ -753,7 +771,8 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
             float m = -INFINITY;
             uint64_t sum[2] = {0, 0};
             for (int j = 0; j < ns; ++j, ++used) {
-                wait(&b_s[s][used & 1], (used >> 1) & 1);
+                const unsigned g = base + (turns ? 2 * j + s : j);
+                wait(&b_s[s][g % kRing], g / kRing & 1);
                 tc_fence_after();
                 if (busy) {
                     const uint32_t t_s = tmem + s * 128 + (used & 1) * 64 + lanes;
@@ -786,7 +805,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                         sum[1] = fma2(sum[1], c2, 0);
                         if (j > 0) {
                             // O is at rest between the product before (waited for here) and the one that waits for this P
-                            o_done();
+                            o_done(g - (turns ? 2 : 1));
                             tc_fence_after();
 #pragma unroll 1
                             for (int d = 0; d < kHead / 2; d += 32) {
@@ -822,9 +841,10 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
             block_segments(runs, kvh, block, &first, &results);
             const int split = turns ? 2 * ((int)blockIdx.x - first) + s : (int)blockIdx.x - first;
             if (ns) {
-                o_done();
+                o_done(base + (turns ? 2 * (ns - 1) + s : ns - 1));
                 tc_fence_after();
             }
+            base += n;
             if (busy) {
                 const long long results_at = (long long)split * total_rows * p.n_heads;
                 const float2 l2 = apart(add2(sum[0], sum[1]));
