@@ -5,21 +5,19 @@
 //   pushes  pages(new) .. pages(old) - 1 of every request that shrinks go on top of the free stack,
 //   pops    every request that grows takes pages(new) - pages(old) pages off the top,
 //   tokens  token old[r] + j of a growing request gets row start[r] + j of the slot map.
-// The sums are done by every CTA for itself in shared memory (a few thousand additions, cheaper than a hand-off between
-// kernels); the lists are then cut evenly over all threads, each element finding its request by bisection of the sums.
-// What bounds it is latency: loads of the lengths, the scan's barriers, one dependent table load and the store.
+// One CTA does the sums in shared memory, then the lists, cut evenly over its threads, each element finding its request by
+// bisection of the sums. What bounds it is latency: loads of the lengths, the scan's barriers, dependent loads and the store.
+// Where the tokens are many (a step that brings prompts), a second kernel of many CTAs writes the slot map from the finished
+// table: 196000 tokens of 512 requests took the one CTA 150 us.
 #include "../../include/ml2b200.h"
-
-#include <cooperative_groups.h>
 
 #include "batch_common.cuh"
 #include "host_common.hpp"
 
 namespace ml2 {
 
-namespace cg = cooperative_groups;
-
 constexpr int kTablesThreads = 1024;
+constexpr int kTablesFill = 4096;  // up to here one CTA writes the slot map: @@
 
 struct TablesParams {
     const int* lengths;
@@ -35,6 +33,7 @@ struct TablesParams {
     int* refused;
     DeviceStatus* status;
     int n, page_shift, width, n_pages, max_tokens, offset;
+    int fill;  // rows of the slot map that the first kernel writes: all of them or none
 };
 
 struct Sums {
@@ -100,8 +99,6 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Tabl
     int* s_push = s_pop + p.n + 1;        // pages given back before request r
     int* s_old = s_push + p.n + 1;
 
-    cg::cluster_group cluster = cg::this_cluster();
-    const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
     pdl_wait();
 
     const int per = ceil_div(p.n, (int)blockDim.x), r0 = min((int)threadIdx.x * per, p.n), r1 = min(r0 + per, p.n);
@@ -125,10 +122,10 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Tabl
 
     int count = *p.free_count;
     if (count < 0 || count > p.n_pages) {
-        if (threadIdx.x == 0 && rank == 0) report_input_error(p.status, kInputFreeCount, count);
+        if (threadIdx.x == 0) report_input_error(p.status, kInputFreeCount, count);
         count = min(max(count, 0), p.n_pages);
     }
-    if (total.back > p.n_pages - count && threadIdx.x == 0 && rank == 0) report_input_error(p.status, kInputFreeOverflow, total.back);
+    if (total.back > p.n_pages - count && threadIdx.x == 0) report_input_error(p.status, kInputFreeOverflow, total.back);
     const int have = min(count + min(total.back, p.n_pages - count), p.n_pages);
     const bool all_fit = total.tokens <= p.max_tokens && total.need <= have;
 
@@ -148,7 +145,7 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Tabl
             s_start[r] = (int)before.tokens;
             s_pop[r] = before.need;
             before = before + v;
-            if (rank == 0) p.refused[r] = valid(s_old[r], p.new_lengths[r]) ? 0 : ML2_REFUSED_LENGTH;
+            p.refused[r] = valid(s_old[r], p.new_lengths[r]) ? 0 : ML2_REFUSED_LENGTH;
         }
     } else {
         const long long tokens_before = before.tokens;
@@ -190,7 +187,7 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Tabl
                 before.tokens += v.tokens;
                 before.need += v.need;
             }
-            if (rank == 0) p.refused[r] = code;
+            p.refused[r] = code;
         }
     }
     if (threadIdx.x == 0) {
@@ -200,7 +197,7 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Tabl
     }
     __syncthreads();
 
-    const int threads = ctas * (int)blockDim.x, me = rank * (int)blockDim.x + (int)threadIdx.x;
+    const int threads = (int)blockDim.x, me = (int)threadIdx.x;
     const int n_push = have - count, n_pop = total.need, n_tokens = (int)total.tokens;
     for (int x = me; x < n_push; x += threads) {
         const int r = bisect(s_push, p.n, x);
@@ -208,12 +205,12 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Tabl
     }
     // Pages given back are taken again below, and the lengths may be written over the ones read above: everybody is done
     // reading and pushing first.
-    cluster.sync();
+    __syncthreads();
     for (int x = me; x < n_pop; x += threads) {
         const int r = bisect(s_pop, p.n, x);
         p.table[(size_t)r * p.width + pages(s_old[r]) + (x - s_pop[r])] = p.free_pages[have - 1 - x];
     }
-    for (int t = me; t < p.max_tokens; t += threads) {
+    for (int t = me; t < p.fill; t += threads) {
         int slot = -1, position = 0;
         if (t < n_tokens) {
             const int r = bisect(s_start, p.n, t), old = s_old[r], at = old + (t - s_start[r]);
@@ -227,18 +224,42 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Tabl
         p.slots[t] = slot;
         p.positions[t] = position;
     }
-    if (rank == 0) {
-        for (int r = r0; r < r1; ++r) {
-            // a request that keeps its rows keeps its length: growth is seen in the served sums, all else in the lengths
-            const int a = s_old[r], b = p.new_lengths[r];
-            const bool grows = b > a, served = s_start[r + 1] > s_start[r];
-            p.query_start[r] = s_start[r];
-            p.lengths_out[r] = !valid(a, b) || (grows && !served) ? a : b;
+    for (int r = r0; r < r1; ++r) {
+        // a request that keeps its rows keeps its length: growth is seen in the served sums, all else in the lengths
+        const int a = s_old[r], b = p.new_lengths[r];
+        const bool grows = b > a, served = s_start[r + 1] > s_start[r];
+        p.query_start[r] = s_start[r];
+        p.lengths_out[r] = !valid(a, b) || (grows && !served) ? a : b;
+    }
+    if (threadIdx.x == 0) {
+        p.query_start[p.n] = n_tokens;
+        *p.free_count_out = have - n_pop;
+    }
+}
+
+// The slot map of many tokens, four a thread: request by bisection of query_start, its old length from the new one.
+__global__ void __launch_bounds__(256) slot_map_kernel(const TablesParams p)
+{
+    pdl_wait();
+    const int n_tokens = p.query_start[p.n], t0 = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (t0 >= p.max_tokens) return;
+    int r = 0, start = 0, end = 0, old = 0;
+    for (int t = t0; t < min(t0 + 4, p.max_tokens); ++t) {
+        int slot = -1, position = 0;
+        if (t < n_tokens) {
+            if (t >= end) {
+                r = bisect(p.query_start, p.n, t);
+                start = p.query_start[r];
+                end = p.query_start[r + 1];
+                old = p.new_lengths[r] - (end - start);
+            }
+            const int at = old + (t - start), id = p.table[(size_t)r * p.width + (at >> p.page_shift)];
+            if (id >= 0 && id < p.n_pages) slot = (id << p.page_shift) + (at & ((1 << p.page_shift) - 1));
+            else report_input_error(p.status, kInputPage, r);
+            position = p.offset + at;
         }
-        if (threadIdx.x == 0) {
-            p.query_start[p.n] = n_tokens;
-            *p.free_count_out = have - n_pop;
-        }
+        p.slots[t] = slot;
+        p.positions[t] = position;
     }
 }
 
@@ -275,10 +296,11 @@ extern "C" int ml2_block_tables(ml2_ctx* h, const int* lengths, const int* new_l
     p.lengths_out = lengths_out; p.free_count_out = free_count_out; p.query_start = query_start; p.slots = slots; p.positions = positions;
     p.refused = refused; p.status = input_status(ctx);
     p.n = n_requests; p.page_shift = shift; p.width = table_stride; p.n_pages = n_pages; p.max_tokens = max_tokens; p.offset = position_offset;
+    p.fill = max_tokens <= kTablesFill ? max_tokens : 0;
 
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(1);
-    cfg.blockDim = dim3(kTablesThreads);
+    cfg.blockDim = dim3(n_requests <= 256 && p.fill <= 1024 ? 256 : kTablesThreads);
     cfg.dynamicSmemBytes = (4 * (size_t)n_requests + 3) * sizeof(int);
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[1];
@@ -290,7 +312,16 @@ extern "C" int ml2_block_tables(ml2_ctx* h, const int* lengths, const int* new_l
     if (cfg.dynamicSmemBytes > 48 * 1024)
         e = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((4 * kMaxRequests + 3) * sizeof(int)));
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, block_tables_kernel, p);
+    if (e == cudaSuccess) {
+        ++ctx->launches;
+        if (p.fill < max_tokens) {
+            cfg.gridDim = dim3((unsigned)ceil_div(max_tokens, 1024));
+            cfg.blockDim = dim3(256);
+            cfg.dynamicSmemBytes = 0;
+            cfg.numAttrs = 1;  // is set up while the first kernel runs, and waits for it
+            if ((e = cudaLaunchKernelEx(&cfg, slot_map_kernel, p)) == cudaSuccess) ++ctx->launches;
+        }
+    }
     if (e != cudaSuccess) return fail(ML2_E_CUDA, "block_tables: %s", cudaGetErrorString(e));
-    ++ctx->launches;
     return ML2_OK;
 }

@@ -16,7 +16,7 @@
 
 namespace ml2 {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 640;  // of a block at most
 constexpr int kRopeMaxHead = 256;
 
 struct RopeParams {
@@ -33,54 +33,59 @@ struct RopeParams {
 };
 
 // A head of `head` elements is head / 16 lanes, 16 elements each: two 16-byte vectors that hold the two halves of eight
-// rotated pairs (lanes below rotary / 16), or two neighbouring vectors of the part that is not rotated.
+// rotated pairs (lanes below rotary / 16), or two neighbouring vectors of the part that is not rotated. A block takes one
+// token, all of it in one pass where the heads fit its threads; the first vectors are asked for before the angles are
+// computed, which hides most of either behind the other.
 template <typename T>
 __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid_constant__ RopeParams p)
 {
     __shared__ float2 s_unit[kRopeMaxHead / 2];
     const long long t = blockIdx.x;
+    const int lane = threadIdx.x % p.lanes, per_block = blockDim.x / p.lanes, units = p.head >> 4, turned = p.rotary >> 4, half = p.rotary >> 1;
+    const int at0 = lane < turned ? 8 * lane : 16 * lane, at1 = lane < turned ? 8 * lane + half : 16 * lane + 8;
+    const int heads = p.n_heads + 2 * p.n_kv;
+    auto source = [&](int h) {
+        if (h < p.n_heads) return static_cast<const T*>(p.q) + t * p.q_stride + (long long)h * p.head;
+        h -= p.n_heads;
+        if (h < p.n_kv) return static_cast<const T*>(p.k) + t * p.k_stride + (long long)h * p.head;
+        return static_cast<const T*>(p.v) + t * p.v_stride + (long long)(h - p.n_kv) * p.head;
+    };
     pdl_wait();
+    int h = blockIdx.y * per_block + threadIdx.x / p.lanes;
+    uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
+    if (lane < units && h < heads) {
+        const T* in = source(h);
+        x0 = *reinterpret_cast<const uint4*>(in + at0);
+        x1 = *reinterpret_cast<const uint4*>(in + at1);
+    }
     const int slot = p.slots[t];
     if (slot < 0) return;  // padding
     if (slot >= p.n_slots) {
         if (threadIdx.x == 0) report_input_error(p.status, kInputSlot, (int)t);
         return;
     }
-    const int half = p.rotary >> 1;
     const double pos = (double)p.positions[t];
-    for (int i = threadIdx.x; i < half; i += kRopeThreads) {
+    for (int i = threadIdx.x; i < half; i += blockDim.x) {
         const double a = pos * p.turns[i];
         const float r = 2.f * (float)(a - rint(a));
         s_unit[i] = make_float2(cospif(r), sinpif(r));
     }
     __syncthreads();
 
-    const int lane = threadIdx.x % p.lanes, per_block = kRopeThreads / p.lanes, units = p.head >> 4, turned = p.rotary >> 4;
-    const int at0 = lane < turned ? 8 * lane : 16 * lane, at1 = lane < turned ? 8 * lane + half : 16 * lane + 8;
-    const bool live = lane < units;
-    const int heads = p.n_heads + 2 * p.n_kv;
     for (int base = blockIdx.y * per_block; base < heads; base += gridDim.y * per_block) {
-        const int h = base + threadIdx.x / p.lanes;
-        const bool here = live && h < heads;
-        const T* in = nullptr;
-        T* out = nullptr;
-        const T* w = nullptr;
+        const bool here = lane < units && h < heads;
+        const int next = h + gridDim.y * per_block;
+        T* out;
+        const T* w;
         if (h < p.n_heads) {
-            in = static_cast<const T*>(p.q) + t * p.q_stride + (long long)h * p.head;
             out = static_cast<T*>(p.q_out) + t * p.q_out_stride + (long long)h * p.head;
             w = static_cast<const T*>(p.qw);
         } else if (h < p.n_heads + p.n_kv) {
-            in = static_cast<const T*>(p.k) + t * p.k_stride + (long long)(h - p.n_heads) * p.head;
             out = static_cast<T*>(p.k_cache) + (long long)slot * p.cache_stride + (long long)(h - p.n_heads) * p.head;
             w = static_cast<const T*>(p.kw);
         } else {
-            in = static_cast<const T*>(p.v) + t * p.v_stride + (long long)(h - p.n_heads - p.n_kv) * p.head;
             out = static_cast<T*>(p.v_cache) + (long long)slot * p.cache_stride + (long long)(h - p.n_heads - p.n_kv) * p.head;
-        }
-        uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
-        if (here) {
-            x0 = *reinterpret_cast<const uint4*>(in + at0);
-            x1 = *reinterpret_cast<const uint4*>(in + at1);
+            w = nullptr;
         }
         float a[8], b[8];
         unpack8<T>(x0, a);
@@ -102,22 +107,30 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid
                 }
             }
         }
-        if (!here) continue;
+        uint4 y0 = x0, y1 = x1;
         if (h < p.n_heads + p.n_kv) {
             if (lane < turned) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float2 u = s_unit[8 * lane + e];
-                    const float y0 = a[e] * u.x - b[e] * u.y, y1 = a[e] * u.y + b[e] * u.x;
-                    a[e] = y0;
-                    b[e] = y1;
+                    const float r0 = a[e] * u.x - b[e] * u.y, r1 = a[e] * u.y + b[e] * u.x;
+                    a[e] = r0;
+                    b[e] = r1;
                 }
             }
-            x0 = pack8<T>(a);
-            x1 = pack8<T>(b);
+            y0 = pack8<T>(a);
+            y1 = pack8<T>(b);
         }
-        *reinterpret_cast<uint4*>(out + at0) = x0;
-        *reinterpret_cast<uint4*>(out + at1) = x1;
+        if (lane < units && next < heads) {
+            const T* in = source(next);
+            x0 = *reinterpret_cast<const uint4*>(in + at0);
+            x1 = *reinterpret_cast<const uint4*>(in + at1);
+        }
+        if (here) {
+            *reinterpret_cast<uint4*>(out + at0) = y0;
+            *reinterpret_cast<uint4*>(out + at1) = y1;
+        }
+        h = next;
     }
 }
 
@@ -168,10 +181,13 @@ extern "C" int ml2_qk_norm_rope(ml2_ctx* h, int dtype, void* query_out, long lon
         double f = 0.15915494309189533577;  // 1 / (2 pi)
         for (int i = 0; i < rotary_size / 2; ++i, f *= ratio) p.turns[i] = f;
     }
-    const int heads = n_heads + 2 * n_kv_heads, passes = ceil_div(heads * p.lanes, kRopeThreads);
+    // one pass with up to kRopeThreads threads; a few tokens with many heads are cut over several blocks of 256
+    const int lanes = (n_heads + 2 * n_kv_heads) * p.lanes;
+    const bool few = n_tokens * 2 < ctx->sm_count;
+    const int threads = std::min(few ? 256 : kRopeThreads, ceil_div(lanes, 32) * 32);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)n_tokens, (unsigned)std::min(passes, std::max(1, 2 * ctx->sm_count / n_tokens)));
-    cfg.blockDim = dim3(kRopeThreads);
+    cfg.gridDim = dim3((unsigned)n_tokens, few ? (unsigned)std::min(ceil_div(lanes, threads), std::max(1, 2 * ctx->sm_count / n_tokens)) : 1u);
+    cfg.blockDim = dim3(threads);
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -270,20 +270,20 @@ class SampleTopP(Module):
 
 # ---- batched decoding over a paged cache: no counterpart in the reference, which decodes one sequence ------------------------
 
-_types = {}  # torch's own, fetched at the first call: importing this package does not import torch
+_torch = None  # fetched by the first operator that is made: importing this package does not import torch
 
 
-def _type(name):
-    if name not in _types:
+def _use_torch():
+    global _torch
+    if _torch is None:
         import torch
-        _types[name] = getattr(torch, name)
-    return _types[name]
+        _torch = torch
 
 
 def _dtype_code(t, what):
-    if t.dtype is _type("float16"):
+    if t.dtype is _torch.float16:
         return 0  # ML2_F16
-    if t.dtype is _type("bfloat16"):
+    if t.dtype is _torch.bfloat16:
         return 1  # ML2_BF16
     raise ValueError("%s: type %s is neither float16 nor bfloat16" % (what, t.dtype))
 
@@ -299,7 +299,7 @@ def _rows(ctx, what, t, width, dtype):
 
 def _ints(ctx, what, t, count):
     """Checks a contiguous int32 tensor of at least `count` entries; returns its device pointer."""
-    if t.dtype is not _type("int32") or t.get_device() != ctx.device or not t.is_contiguous() or t.numel() < count:
+    if t.dtype is not _torch.int32 or t.get_device() != ctx.device or not t.is_contiguous() or t.numel() < count:
         raise ValueError("%s: expected a contiguous int32 tensor of at least %d entries on cuda:%d, got %s %s on %s"
                          % (what, count, ctx.device, tuple(t.shape), t.dtype, t.device))
     return t.data_ptr()
@@ -313,6 +313,7 @@ class BlockTables(Module):
 
     def __init__(self, cudaContext, pageSize):
         super().__init__(cudaContext)
+        _use_torch()
         self.pageSize = pageSize
         self._call = _lib.declare(self.lib.ml2_block_tables, "ppp ii pi ppi ppppp i p i")
 
@@ -338,6 +339,7 @@ class QKNormRoPE(Module):
 
     def __init__(self, cudaContext, config, rotarySize=None):
         super().__init__(cudaContext)
+        _use_torch()
         self.numHeads, self.numKVHeads, self.theta = config.numHeads, config.numKVHeads, config.ropeTheta
         self.headSize = config.dim // config.numHeads
         self.rotarySize = self.headSize if rotarySize is None else rotarySize
@@ -372,6 +374,7 @@ class PrefixAttention(Module):
 
     def __init__(self, cudaContext, config, pageSize):
         super().__init__(cudaContext)
+        _use_torch()
         self.numHeads, self.numKVHeads, self.pageSize = config.numHeads, config.numKVHeads, pageSize
         self.headSize = config.dim // config.numHeads
         self._size = _lib.declare(self.lib.ml2_prefix_attention_workspace, "p iiiiiii p")
@@ -401,7 +404,7 @@ class PrefixAttention(Module):
             prefix = _lib.KVStruct(prefixKey.data_ptr(), prefixValue.data_ptr(), ps, prefixKey.shape[0])
         lsePtr = 0
         if lse is not None:
-            if lse.dtype is not _type("float32") or lse.get_device() != c.device or not lse.is_contiguous() or lse.numel() < rows * self.numHeads:
+            if lse.dtype is not _torch.float32 or lse.get_device() != c.device or not lse.is_contiguous() or lse.numel() < rows * self.numHeads:
                 raise ValueError("lse: expected contiguous float32 [%d][%d] on cuda:%d" % (rows, self.numHeads, c.device))
             lsePtr = lse.data_ptr()
         if workspace.get_device() != c.device or not workspace.is_contiguous():
