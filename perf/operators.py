@@ -341,7 +341,9 @@ def _operators(c):
 
 def _call(st):
     c = st["case"]
-    op = _operators(c)
+    if "operator" not in st:  # looked up once for the inputs, as a program holds it: not at every pass
+        st["operator"] = _operators(c)
+    op = st["operator"]
     if c["op"] == "tables":
         op.Forward(st["old"], st["new"], st["table"], st["free"], st["free_count"], st["lengths"], st["free_count_out"], st["start"],
                    st["slots"], st["positions"], st["refused"], st["offset"])
