@@ -139,12 +139,6 @@ int ml2_argmax(ml2_ctx* ctx, const void* logits, int vocab_size, int* tokens, in
  * find out of range are left out and reported by ml2_ctx_status. */
 #define ML2_F16 0
 #define ML2_BF16 1
-typedef struct ml2_kv {
-    void* key;            /* [rows][row_stride], a row holds n_kv_heads * head_size values */
-    void* value;
-    long long row_stride; /* elements from one row to the next, the same for both */
-    long long rows;
-} ml2_kv;
 #define ML2_REFUSED_LENGTH 1 /* a length is negative or needs more than table_stride pages */
 #define ML2_REFUSED_PAGES 2  /* the free pages do not suffice */
 #define ML2_REFUSED_TOKENS 3 /* the new tokens do not fit the slot map */
@@ -159,21 +153,35 @@ typedef struct ml2_kv {
  * position_offset + its place in the request (position_offset: length of a prefix that is kept elsewhere). Rows from
  * query_start[n_requests] to max_tokens are padding: slot -1, position 0. lengths_out and free_count_out may be the arrays
  * lengths and free_count; where they are others, the call can be repeated with the same result. */
-int ml2_block_tables(ml2_ctx* ctx, const int* lengths, const int* new_lengths, int n_requests, int page_size, int* table, int table_stride,
-                     int* free_pages, const int* free_count, int n_pages, int* lengths_out, int* free_count_out, int* query_start,
-                     int* slots, int* positions, int max_tokens, int* refused, int position_offset);
+typedef struct ml2_block_tables_args {
+    const int *lengths, *new_lengths; /* [n_requests] */
+    int *table, *free_pages;          /* [n_requests][table_stride], [n_pages] */
+    const int* free_count;
+    int *lengths_out, *free_count_out;
+    int* query_start;                 /* [n_requests + 1] */
+    int *slots, *positions;           /* [max_tokens] */
+    int* refused;                     /* [n_requests] */
+    int n_requests, page_size, table_stride, n_pages, max_tokens, position_offset;
+} ml2_block_tables_args;
+int ml2_block_tables(ml2_ctx* ctx, const ml2_block_tables_args* args);
 /* RMS norm of every query and key head (weights of head_size values; both null: no norm), rotation of the first
  * rotary_size values of each head (pairs i, i + rotary_size / 2 as in ml2_rope; angle positions[t] *
  * theta^(-2i / rotary_size), reduced in 64 bits), queries to query_out (may be query), keys and values to the cache rows
  * slots[t], which must differ from one another. A token with a negative slot is padding: nothing of it is written.
  * Arithmetic in fp32, one rounding to `dtype`. head_size and rotary_size are multiples of 16, head_size at most 256;
  * strides in elements, multiples of 8; pointers 16-byte aligned. */
-int ml2_qk_norm_rope(ml2_ctx* ctx, int dtype, void* query_out, long long query_out_stride, const ml2_kv* cache, const void* query,
-                     long long query_stride, const void* key, long long key_stride, const void* value, long long value_stride,
-                     const void* query_weight, const void* key_weight, const int* positions, const int* slots, int n_tokens, int n_heads,
-                     int n_kv_heads, int head_size, int rotary_size, float theta, float eps);
+typedef struct ml2_qk_norm_rope_args {
+    void *query_out, *key_cache, *value_cache;      /* [n_tokens][n_heads * head_size], [cache_rows][n_kv_heads * head_size] */
+    const void *query, *key, *value;                /* [n_tokens][...] */
+    const void *query_weight, *key_weight;          /* [head_size] */
+    const int *positions, *slots;                   /* [n_tokens] */
+    long long query_out_stride, cache_stride, cache_rows, query_stride, key_stride, value_stride;
+    int dtype, n_tokens, n_heads, n_kv_heads, head_size, rotary_size;
+    float theta, eps;
+} ml2_qk_norm_rope_args;
+int ml2_qk_norm_rope(ml2_ctx* ctx, const ml2_qk_norm_rope_args* args);
 /* Attention of a batch that shares a prefix. Query rows query_start[r] .. query_start[r + 1] - 1 belong to request r, whose
- * lengths[r] own tokens (the new ones included) lie in the pages table[r]; row i of `queries` sees all prefix->rows rows of
+ * lengths[r] own tokens (the new ones included) lie in the pages table[r]; row i of `queries` sees all prefix_length rows of
  * the prefix and own tokens 0 .. lengths[r] - queries + i. out[row][head] = softmax(scale q.k) v; lse (may be null, fp32
  * [n_rows][n_heads]) = log sum exp(scale q.k). A row that sees nothing, or whose scores are all -inf, gives zeros and
  * -inf. Rows from query_start[n_requests] to n_rows stay as they are. Scores, softmax and sums are fp32; the weights are
@@ -183,10 +191,20 @@ int ml2_qk_norm_rope(ml2_ctx* ctx, int dtype, void* query_out, long long query_o
  * prefix and max_length) holds partial results: calls that may run at the same time need one each. */
 int ml2_prefix_attention_workspace(ml2_ctx* ctx, int n_rows, int n_requests, int prefix_length, int max_length, int n_heads,
                                    int n_kv_heads, int head_size, size_t* bytes);
-int ml2_prefix_attention(ml2_ctx* ctx, int dtype, void* out, long long out_stride, float* lse, const void* query, long long query_stride,
-                         int n_rows, const ml2_kv* prefix, const ml2_kv* cache, int page_size, const int* table, int table_stride,
-                         const int* lengths, const int* query_start, int n_requests, int max_length, int n_heads, int n_kv_heads,
-                         int head_size, float scale, void* workspace, size_t workspace_bytes);
+typedef struct ml2_prefix_attention_args {
+    void* out;                                    /* [n_rows][n_heads * head_size] */
+    float* lse;                                   /* [n_rows][n_heads], or null */
+    const void* query;                            /* [n_rows][n_heads * head_size] */
+    const void *prefix_key, *prefix_value;        /* [prefix_length][n_kv_heads * head_size] */
+    const void *key_cache, *value_cache;          /* [cache_rows][n_kv_heads * head_size] */
+    const int *table, *lengths, *query_start;     /* [n_requests][table_stride], [n_requests], [n_requests + 1] */
+    void* workspace;
+    size_t workspace_bytes;
+    long long out_stride, query_stride, prefix_stride, cache_stride, cache_rows;
+    int dtype, n_rows, n_requests, prefix_length, max_length, page_size, table_stride, n_heads, n_kv_heads, head_size;
+    float scale;
+} ml2_prefix_attention_args;
+int ml2_prefix_attention(ml2_ctx* ctx, const ml2_prefix_attention_args* args);
 
 /* ---- host-buffer convenience (the same operators with the copies inside the call) ---------- */
 /* Copies `in`/`inout` (host fp16) to scratch owned by the context, runs ml2_matvec_residual_int4 on

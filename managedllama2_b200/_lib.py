@@ -2,6 +2,7 @@
 import ctypes
 import os
 import re
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libml2b200.so")
@@ -51,13 +52,32 @@ class ConfigStruct(ctypes.Structure):
                 ("seq_len", ctypes.c_int32), ("rope_theta", ctypes.c_float)]
 
 
-class KVStruct(ctypes.Structure):
-    _fields_ = [("key", ctypes.c_void_p), ("value", ctypes.c_void_p), ("row_stride", ctypes.c_longlong), ("rows", ctypes.c_longlong)]
+class Arguments:
+    """The argument struct of a C entry: its members and their kinds (p pointer, l long long / size_t, i int, f float), packed
+    as the C compiler lays them out. Bytes from ``struct`` cost a third of a call with as many ctypes arguments."""
+
+    def __init__(self, *members):
+        self.names, self.kinds = [], ""
+        for kind, names in members:
+            names = names.split()
+            self.names += names
+            self.kinds += kind * len(names)
+        self.pack = struct.Struct("@" + self.kinds.replace("p", "P").replace("l", "q")).pack
+
+    def entry(self, function):
+        function.argtypes = [ctypes.c_void_p, ctypes.c_char_p]
+        function.restype = ctypes.c_int
+        return function
 
 
-def declare(function, arguments):
-    """Sets the argument types of a C entry: p pointer, i int, l long long / size_t, f float (the context's p comes first)."""
-    kinds = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
-    function.argtypes = [kinds[a] for a in arguments.replace(" ", "")]
-    function.restype = ctypes.c_int
-    return function
+BLOCK_TABLES = Arguments(
+    ("p", "lengths new_lengths table free_pages free_count lengths_out free_count_out query_start slots positions refused"),
+    ("i", "n_requests page_size table_stride n_pages max_tokens position_offset"))
+QK_NORM_ROPE = Arguments(
+    ("p", "query_out key_cache value_cache query key value query_weight key_weight positions slots"),
+    ("l", "query_out_stride cache_stride cache_rows query_stride key_stride value_stride"),
+    ("i", "dtype n_tokens n_heads n_kv_heads head_size rotary_size"), ("f", "theta eps"))
+PREFIX_ATTENTION = Arguments(
+    ("p", "out lse query prefix_key prefix_value key_cache value_cache table lengths query_start workspace"),
+    ("l", "workspace_bytes out_stride query_stride prefix_stride cache_stride cache_rows"),
+    ("i", "dtype n_rows n_requests prefix_length max_length page_size table_stride n_heads n_kv_heads head_size"), ("f", "scale"))

@@ -267,13 +267,13 @@ __global__ void __launch_bounds__(256) slot_map_kernel(const TablesParams p)
 
 using namespace ml2;
 
-extern "C" int ml2_block_tables(ml2_ctx* h, const int* lengths, const int* new_lengths, int n_requests, int page_size, int* table,
-                                int table_stride, int* free_pages, const int* free_count, int n_pages, int* lengths_out,
-                                int* free_count_out, int* query_start, int* slots, int* positions, int max_tokens, int* refused,
-                                int position_offset)
+extern "C" int ml2_block_tables(ml2_ctx* h, const ml2_block_tables_args* args)
 {
     Ctx* ctx = reinterpret_cast<Ctx*>(h);
-    if (!ctx || !lengths || !new_lengths || !table || !free_pages || !free_count || !lengths_out || !free_count_out || !query_start || !refused)
+    if (!ctx || !args) return fail(ML2_E_INVALID, "block_tables: null argument");
+    const auto [lengths, new_lengths, table, free_pages, free_count, lengths_out, free_count_out, query_start, slots, positions, refused, n_requests,
+                page_size, table_stride, n_pages, max_tokens, position_offset] = *args;
+    if (!lengths || !new_lengths || !table || !free_pages || !free_count || !lengths_out || !free_count_out || !query_start || !refused)
         return fail(ML2_E_INVALID, "block_tables: null argument");
     if (max_tokens < 0 || (max_tokens > 0 && (!slots || !positions)))
         return fail(ML2_E_INVALID, "block_tables: max_tokens=%d with slots=%p positions=%p", max_tokens, (void*)slots, (void*)positions);

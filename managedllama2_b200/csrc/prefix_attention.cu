@@ -1130,17 +1130,16 @@ int ml2_prefix_attention_workspace(ml2_ctx* h, int n_rows, int n_requests, int p
     return ML2_OK;
 }
 
-int ml2_prefix_attention(ml2_ctx* h, int dtype, void* out, long long out_stride, float* lse, const void* query, long long query_stride,
-                         int n_rows, const ml2_kv* prefix, const ml2_kv* cache, int page_size, const int* table, int table_stride,
-                         const int* lengths, const int* query_start, int n_requests, int max_length, int n_heads, int n_kv_heads,
-                         int head_size, float scale, void* workspace, size_t workspace_bytes)
+int ml2_prefix_attention(ml2_ctx* h, const ml2_prefix_attention_args* args)
 {
     Ctx* ctx = reinterpret_cast<Ctx*>(h);
-    if (!ctx || !prefix || !cache) return fail(ML2_E_INVALID, "prefix_attention: null argument");
+    if (!ctx || !args) return fail(ML2_E_INVALID, "prefix_attention: null argument");
+    const auto [out, lse, query, prefix_key, prefix_value, key_cache, value_cache, table, lengths, query_start, workspace, workspace_bytes, out_stride,
+                query_stride, prefix_stride, cache_stride, cache_rows, dtype, n_rows, n_requests, prefix_length, max_length, page_size, table_stride, n_heads,
+                n_kv_heads, head_size, scale] = *args;
     if (dtype != ML2_F16 && dtype != ML2_BF16) return fail(ML2_E_INVALID, "prefix_attention: dtype=%d is neither ML2_F16 nor ML2_BF16", dtype);
-    if (prefix->rows < 0 || prefix->rows > INT32_MAX || cache->rows < 1 || cache->rows > INT32_MAX)
-        return fail(ML2_E_INVALID, "prefix_attention: the prefix has %lld rows and the cache %lld", prefix->rows, cache->rows);
-    if (int rc = check_sizes("prefix_attention", n_rows, n_requests, (int)prefix->rows, max_length, n_heads, n_kv_heads, head_size)) return rc;
+    if (cache_rows < 1 || cache_rows > INT32_MAX) return fail(ML2_E_INVALID, "prefix_attention: the cache has %lld rows", cache_rows);
+    if (int rc = check_sizes("prefix_attention", n_rows, n_requests, prefix_length, max_length, n_heads, n_kv_heads, head_size)) return rc;
     const int shift = page_shift(page_size);
     if (shift < 0) return fail(ML2_E_INVALID, "prefix_attention: page_size=%d must be a power of two, at most %d", page_size, kMaxPageSize);
     if (table_stride < 1 || (long long)table_stride * page_size > INT32_MAX)
@@ -1149,26 +1148,26 @@ int ml2_prefix_attention(ml2_ctx* h, int dtype, void* out, long long out_stride,
         return fail(ML2_E_INVALID, "prefix_attention: max_length=%d passes the table's %d pages of %d", max_length, table_stride, page_size);
     if (!std::isfinite(scale)) return fail(ML2_E_INVALID, "prefix_attention: scale=%g", (double)scale);
     if (n_rows == 0) return ML2_OK;
-    if (!out || !query || !table || !lengths || !query_start || !cache->key || !cache->value || (prefix->rows && (!prefix->key || !prefix->value)))
+    if (!out || !query || !table || !lengths || !query_start || !key_cache || !value_cache || (prefix_length && (!prefix_key || !prefix_value)))
         return fail(ML2_E_INVALID, "prefix_attention: null argument");
     const long long q_width = (long long)n_heads * head_size, kv_width = (long long)n_kv_heads * head_size;
-    if (out_stride < q_width || query_stride < q_width || cache->row_stride < kv_width || (prefix->rows && prefix->row_stride < kv_width))
+    if (out_stride < q_width || query_stride < q_width || cache_stride < kv_width || (prefix_length && prefix_stride < kv_width))
         return fail(ML2_E_INVALID, "prefix_attention: a row stride is shorter than the row");
-    if ((out_stride | query_stride | cache->row_stride | prefix->row_stride) % 8 || !aligned_to(16, out, query, cache->key, cache->value) ||
-        !aligned_to(16, prefix->key, prefix->value, workspace))
+    if ((out_stride | query_stride | cache_stride | prefix_stride) % 8 || !aligned_to(16, out, query, key_cache, value_cache) ||
+        !aligned_to(16, prefix_key, prefix_value, workspace))
         return fail(ML2_E_INVALID, "prefix_attention: pointers must be 16-byte aligned and row strides multiples of 8 elements");
     if (out == query) return fail(ML2_E_INVALID, "prefix_attention: out must not overlap the queries");
-    const AttnPlan pl = plan_attention(ctx, n_rows, n_requests, (int)prefix->rows, max_length, n_heads, n_kv_heads, head_size);
+    const AttnPlan pl = plan_attention(ctx, n_rows, n_requests, prefix_length, max_length, n_heads, n_kv_heads, head_size);
     if (pl.tiles > INT32_MAX / 2 || (long long)n_rows * (n_heads / n_kv_heads) > INT32_MAX / 2 || (long long)n_rows * n_heads > INT32_MAX)
         return fail(ML2_E_INVALID, "prefix_attention: n_rows=%d with %d heads is too much for one call", n_rows, n_heads);
     if (workspace_bytes < pl.bytes || (pl.bytes && !workspace))
         return fail(ML2_E_INVALID, "prefix_attention: the workspace has %zu bytes, %zu are needed", workspace_bytes, pl.bytes);
     if (int rc = use_device(ctx)) return rc;
     AttnBatch p{};
-    p.out = out; p.lse = lse; p.q = query; p.pk = prefix->key; p.pv = prefix->value; p.k = cache->key; p.v = cache->value;
+    p.out = out; p.lse = lse; p.q = query; p.pk = prefix_key; p.pv = prefix_value; p.k = key_cache; p.v = value_cache;
     p.table = table; p.lengths = lengths; p.query_start = query_start; p.status = input_status(ctx);
-    p.out_stride = out_stride; p.q_stride = query_stride; p.prefix_stride = prefix->row_stride; p.cache_stride = cache->row_stride;
-    p.n_requests = n_requests; p.n_rows = n_rows; p.prefix = (int)prefix->rows; p.max_length = max_length; p.n_pages = (int)(cache->rows >> shift);
+    p.out_stride = out_stride; p.q_stride = query_stride; p.prefix_stride = prefix_stride; p.cache_stride = cache_stride;
+    p.n_requests = n_requests; p.n_rows = n_rows; p.prefix = prefix_length; p.max_length = max_length; p.n_pages = (int)(cache_rows >> shift);
     p.table_stride = table_stride; p.page_shift = shift; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.group = n_heads / n_kv_heads;
     p.scale_log2 = scale * 1.44269504088896340736f;
     char* ws = static_cast<char*>(workspace);
@@ -1178,9 +1177,9 @@ int ml2_prefix_attention(ml2_ctx* h, int dtype, void* out, long long out_stride,
     p.prefix_ctas = pl.prefix_ctas; p.run_ctas = pl.run_ctas;
     p.waits = ctx->status_dev; p.wait_cycles = ctx->wait_cycles;
     PrefixMaps maps{};
-    if (pl.prefix_ctas && (!make_map(&maps.k, dtype, prefix->key, prefix->row_stride, (int)kv_width, p.prefix) ||
-                           !make_map(&maps.v, dtype, prefix->value, prefix->row_stride, (int)kv_width, p.prefix)))
-        return fail(ML2_E_CUDA, "prefix_attention: no tensor map for a prefix of %d rows of %lld, stride %lld", p.prefix, kv_width, prefix->row_stride);
+    if (pl.prefix_ctas && (!make_map(&maps.k, dtype, prefix_key, prefix_stride, (int)kv_width, p.prefix) ||
+                           !make_map(&maps.v, dtype, prefix_value, prefix_stride, (int)kv_width, p.prefix)))
+        return fail(ML2_E_CUDA, "prefix_attention: no tensor map for a prefix of %d rows of %lld, stride %lld", p.prefix, kv_width, prefix_stride);
     cudaError_t e;
     if (head_size == 128) e = dtype == ML2_F16 ? launch_attention<__half, 128>(ctx, p, pl, maps) : launch_attention<__nv_bfloat16, 128>(ctx, p, pl, maps);
     else e = dtype == ML2_F16 ? launch_attention<__half, 64>(ctx, p, pl, maps) : launch_attention<__nv_bfloat16, 64>(ctx, p, pl, maps);

@@ -16,7 +16,7 @@
 
 namespace ml2 {
 
-constexpr int kRopeThreads = 640;  // of a block at most
+constexpr int kRopeThreads = 320;  // of a block at most
 constexpr int kRopeMaxHead = 256;
 
 struct RopeParams {
@@ -28,7 +28,7 @@ struct RopeParams {
     DeviceStatus* status;
     long long q_out_stride, cache_stride, q_stride, k_stride, v_stride, n_slots;
     int n_heads, n_kv, head, rotary, lanes;  // lanes: threads of one head, a power of two
-    float eps;
+    float eps, per_head;                     // per_head: 1 / head
     double turns[kRopeMaxHead / 2];          // theta^(-2 i / rotary) / (2 pi)
 };
 
@@ -37,7 +37,7 @@ struct RopeParams {
 // token, all of it in one pass where the heads fit its threads; the first vectors are asked for before the angles are
 // computed, which hides most of either behind the other.
 template <typename T>
-__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid_constant__ RopeParams p)
+__global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_kernel(const __grid_constant__ RopeParams p)
 {
     __shared__ float2 s_unit[kRopeMaxHead / 2];
     const long long t = blockIdx.x;
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid
     for (int i = threadIdx.x; i < half; i += blockDim.x) {
         const double a = pos * p.turns[i];
         const float r = 2.f * (float)(a - rint(a));
-        s_unit[i] = make_float2(cospif(r), sinpif(r));
+        s_unit[(i & 7) * turned + (i >> 3)] = make_float2(cospif(r), sinpif(r));  // neighbouring lanes read neighbouring entries
     }
     __syncthreads();
 
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid
             for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + b[e] * b[e];
             for (int o = p.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             if (here && w) {
-                const float inv = 1.0f / sqrtf(ss / (float)p.head + p.eps);
+                const float inv = rsqrtf(ss * p.per_head + p.eps);
                 float wa[8], wb[8];
                 unpack8<T>(*reinterpret_cast<const uint4*>(w + at0), wa);
                 unpack8<T>(*reinterpret_cast<const uint4*>(w + at1), wb);
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid
             if (lane < turned) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float2 u = s_unit[8 * lane + e];
+                    const float2 u = s_unit[e * turned + lane];
                     const float r0 = a[e] * u.x - b[e] * u.y, r1 = a[e] * u.y + b[e] * u.x;
                     a[e] = r0;
                     b[e] = r1;
@@ -138,13 +138,12 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid
 
 using namespace ml2;
 
-extern "C" int ml2_qk_norm_rope(ml2_ctx* h, int dtype, void* query_out, long long query_out_stride, const ml2_kv* cache, const void* query,
-                                long long query_stride, const void* key, long long key_stride, const void* value, long long value_stride,
-                                const void* query_weight, const void* key_weight, const int* positions, const int* slots, int n_tokens,
-                                int n_heads, int n_kv_heads, int head_size, int rotary_size, float theta, float eps)
+extern "C" int ml2_qk_norm_rope(ml2_ctx* h, const ml2_qk_norm_rope_args* args)
 {
     Ctx* ctx = reinterpret_cast<Ctx*>(h);
-    if (!ctx || !cache) return fail(ML2_E_INVALID, "qk_norm_rope: null argument");
+    if (!ctx || !args) return fail(ML2_E_INVALID, "qk_norm_rope: null argument");
+    const auto [query_out, key_cache, value_cache, query, key, value, query_weight, key_weight, positions, slots, query_out_stride, cache_stride,
+                cache_rows, query_stride, key_stride, value_stride, dtype, n_tokens, n_heads, n_kv_heads, head_size, rotary_size, theta, eps] = *args;
     if (dtype != ML2_F16 && dtype != ML2_BF16) return fail(ML2_E_INVALID, "qk_norm_rope: dtype=%d is neither ML2_F16 nor ML2_BF16", dtype);
     if (n_tokens < 0) return fail(ML2_E_INVALID, "qk_norm_rope: n_tokens=%d", n_tokens);
     if (n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads || n_heads > 65536)
@@ -155,24 +154,24 @@ extern "C" int ml2_qk_norm_rope(ml2_ctx* h, int dtype, void* query_out, long lon
     if (!(theta > 0.f) || !std::isfinite(theta) || !(eps >= 0.f)) return fail(ML2_E_INVALID, "qk_norm_rope: theta=%g eps=%g", (double)theta, (double)eps);
     if (!query_weight != !key_weight) return fail(ML2_E_INVALID, "qk_norm_rope: query and key weights come together or not at all");
     if (n_tokens == 0) return ML2_OK;
-    if (!query_out || !query || !key || !value || !positions || !slots || !cache->key || !cache->value)
+    if (!query_out || !query || !key || !value || !positions || !slots || !key_cache || !value_cache)
         return fail(ML2_E_INVALID, "qk_norm_rope: null argument");
     const long long q_width = (long long)n_heads * head_size, kv_width = (long long)n_kv_heads * head_size;
-    if (query_out_stride < q_width || query_stride < q_width || key_stride < kv_width || value_stride < kv_width || cache->row_stride < kv_width)
+    if (query_out_stride < q_width || query_stride < q_width || key_stride < kv_width || value_stride < kv_width || cache_stride < kv_width)
         return fail(ML2_E_INVALID, "qk_norm_rope: a row stride is shorter than the row");
-    if (cache->rows < 1 || cache->rows > INT32_MAX) return fail(ML2_E_INVALID, "qk_norm_rope: the cache has %lld rows", cache->rows);
-    if ((query_out_stride | query_stride | key_stride | value_stride | cache->row_stride) % 8 || !aligned_to(16, query_out, query, key, value) ||
-        !aligned_to(16, cache->key, cache->value) || !aligned_to(16, query_weight, key_weight))
+    if (cache_rows < 1 || cache_rows > INT32_MAX) return fail(ML2_E_INVALID, "qk_norm_rope: the cache has %lld rows", cache_rows);
+    if ((query_out_stride | query_stride | key_stride | value_stride | cache_stride) % 8 || !aligned_to(16, query_out, query, key, value) ||
+        !aligned_to(16, key_cache, value_cache) || !aligned_to(16, query_weight, key_weight))
         return fail(ML2_E_INVALID, "qk_norm_rope: pointers must be 16-byte aligned and row strides multiples of 8 elements");
     if (int rc = use_device(ctx)) return rc;
 
     RopeParams p{};
-    p.q_out = query_out; p.k_cache = cache->key; p.v_cache = cache->value;
+    p.q_out = query_out; p.k_cache = key_cache; p.v_cache = value_cache;
     p.q = query; p.k = key; p.v = value; p.qw = query_weight; p.kw = key_weight;
     p.positions = positions; p.slots = slots; p.status = input_status(ctx);
-    p.q_out_stride = query_out_stride; p.cache_stride = cache->row_stride;
-    p.q_stride = query_stride; p.k_stride = key_stride; p.v_stride = value_stride; p.n_slots = cache->rows;
-    p.n_heads = n_heads; p.n_kv = n_kv_heads; p.head = head_size; p.rotary = rotary_size; p.eps = eps;
+    p.q_out_stride = query_out_stride; p.cache_stride = cache_stride;
+    p.q_stride = query_stride; p.k_stride = key_stride; p.v_stride = value_stride; p.n_slots = cache_rows;
+    p.n_heads = n_heads; p.n_kv = n_kv_heads; p.head = head_size; p.rotary = rotary_size; p.eps = eps; p.per_head = 1.0f / (float)head_size;
     p.lanes = 1;
     while (p.lanes * 16 < head_size) p.lanes *= 2;
     if (rotary_size) {

@@ -289,12 +289,15 @@ def _dtype_code(t, what):
 
 
 def _rows(ctx, what, t, width, dtype):
-    """Checks a [rows][width] tensor whose rows may be apart (a slice of columns); returns the row stride in elements."""
+    """Checks a [rows][width] tensor whose rows may be apart (a slice of columns); returns its rows and their stride in elements."""
     if t.dtype is not dtype or t.get_device() != ctx.device:
         raise ValueError("%s: expected %s on cuda:%d, got %s on %s" % (what, dtype, ctx.device, t.dtype, t.device))
-    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and width != 1):
-        raise ValueError("%s: expected [rows][%d] with neighbouring columns, got %s with strides %s" % (what, width, tuple(t.shape), t.stride()))
-    return t.stride(0) if t.shape[0] > 1 else max(width, t.stride(0))
+    if t.dim() == 2:
+        rows, columns = t.shape
+        stride, step = t.stride()
+        if columns == width and (step == 1 or width == 1):
+            return rows, stride if rows > 1 else max(width, stride)
+    raise ValueError("%s: expected [rows][%d] with neighbouring columns, got %s with strides %s" % (what, width, tuple(t.shape), t.stride()))
 
 
 def _ints(ctx, what, t, count):
@@ -315,20 +318,21 @@ class BlockTables(Module):
         super().__init__(cudaContext)
         _use_torch()
         self.pageSize = pageSize
-        self._call = _lib.declare(self.lib.ml2_block_tables, "ppp ii pi ppi ppppp i p i")
+        self._call = _lib.BLOCK_TABLES.entry(self.lib.ml2_block_tables)
 
     def Forward(self, lengths, newLengths, table, freePages, freeCount, lengthsOut, freeCountOut, queryStart, slots, positions, refused,
                 positionOffset=0):
-        c, n = self.ctx, newLengths.numel()
+        c, n, rows = self.ctx, newLengths.numel(), slots.numel()
         if table.dim() != 2 or table.shape[0] != n:
             raise ValueError("table: expected [%d][pages], got %s" % (n, tuple(table.shape)))
-        rows = slots.numel()
-        _lib.check(self._call(c.handle, _ints(c, "lengths", lengths, n), _ints(c, "newLengths", newLengths, n), n, self.pageSize,
-                              _ints(c, "table", table, 1), table.shape[1], _ints(c, "freePages", freePages, 1),
-                              _ints(c, "freeCount", freeCount, 1), freePages.numel(), _ints(c, "lengthsOut", lengthsOut, n),
-                              _ints(c, "freeCountOut", freeCountOut, 1), _ints(c, "queryStart", queryStart, n + 1),
-                              _ints(c, "slots", slots, rows), _ints(c, "positions", positions, rows), rows,
-                              _ints(c, "refused", refused, n), positionOffset))
+        rc = self._call(c.handle, _lib.BLOCK_TABLES.pack(
+            _ints(c, "lengths", lengths, n), _ints(c, "newLengths", newLengths, n), _ints(c, "table", table, 1),
+            _ints(c, "freePages", freePages, 1), _ints(c, "freeCount", freeCount, 1), _ints(c, "lengthsOut", lengthsOut, n),
+            _ints(c, "freeCountOut", freeCountOut, 1), _ints(c, "queryStart", queryStart, n + 1), _ints(c, "slots", slots, rows),
+            _ints(c, "positions", positions, rows), _ints(c, "refused", refused, n), n, self.pageSize, table.shape[1], freePages.numel(), rows,
+            positionOffset))
+        if rc:
+            _lib.check(rc)
 
 
 class QKNormRoPE(Module):
@@ -343,27 +347,34 @@ class QKNormRoPE(Module):
         self.numHeads, self.numKVHeads, self.theta = config.numHeads, config.numKVHeads, config.ropeTheta
         self.headSize = config.dim // config.numHeads
         self.rotarySize = self.headSize if rotarySize is None else rotarySize
-        self._call = _lib.declare(self.lib.ml2_qk_norm_rope, "p i pl p pl pl pl pp pp iiiii ff")
+        self._call = _lib.QK_NORM_ROPE.entry(self.lib.ml2_qk_norm_rope)
+
+    def _weight(self, what, w, dtype):
+        if w is None:
+            return 0
+        if w.dtype is not dtype or w.get_device() != self.ctx.device or not w.is_contiguous() or w.numel() != self.headSize:
+            raise ValueError("%s: expected %d contiguous %s on cuda:%d" % (what, self.headSize, dtype, self.ctx.device))
+        return w.data_ptr()
 
     def Forward(self, queryOutput, keyCache, valueCache, query, key, value, queryWeight, keyWeight, positions, slots, eps=1e-5):
-        c, dtype, n = self.ctx, query.dtype, query.shape[0]
+        c, dtype = self.ctx, query.dtype
         code, width, kvWidth = _dtype_code(query, "query"), self.numHeads * self.headSize, self.numKVHeads * self.headSize
-        qs, ks, vs = _rows(c, "query", query, width, dtype), _rows(c, "key", key, kvWidth, dtype), _rows(c, "value", value, kvWidth, dtype)
-        os, cs = _rows(c, "queryOutput", queryOutput, width, dtype), _rows(c, "keyCache", keyCache, kvWidth, dtype)
-        if _rows(c, "valueCache", valueCache, kvWidth, dtype) != cs or valueCache.shape[0] != keyCache.shape[0]:
+        n, queryStride = _rows(c, "query", query, width, dtype)
+        nk, keyStride = _rows(c, "key", key, kvWidth, dtype)
+        nv, valueStride = _rows(c, "value", value, kvWidth, dtype)
+        no, outStride = _rows(c, "queryOutput", queryOutput, width, dtype)
+        cache = _rows(c, "keyCache", keyCache, kvWidth, dtype)
+        if _rows(c, "valueCache", valueCache, kvWidth, dtype) != cache:
             raise ValueError("keyCache and valueCache must have the same rows and strides")
-        if key.shape[0] != n or value.shape[0] != n or queryOutput.shape[0] < n:
+        if nk != n or nv != n or no < n:
             raise ValueError("query, key, value and queryOutput must have the same rows")
-        weights = [0, 0]
-        for i, (name, w) in enumerate((("queryWeight", queryWeight), ("keyWeight", keyWeight))):
-            if w is not None:
-                if w.dtype is not dtype or w.get_device() != c.device or not w.is_contiguous() or w.numel() != self.headSize:
-                    raise ValueError("%s: expected %d contiguous %s on cuda:%d" % (name, self.headSize, dtype, c.device))
-                weights[i] = w.data_ptr()
-        cache = _lib.KVStruct(keyCache.data_ptr(), valueCache.data_ptr(), cs, keyCache.shape[0])
-        _lib.check(self._call(c.handle, code, queryOutput.data_ptr(), os, ctypes.addressof(cache), query.data_ptr(), qs, key.data_ptr(), ks,
-                              value.data_ptr(), vs, weights[0], weights[1], _ints(c, "positions", positions, n), _ints(c, "slots", slots, n),
-                              n, self.numHeads, self.numKVHeads, self.headSize, self.rotarySize, self.theta, eps))
+        rc = self._call(c.handle, _lib.QK_NORM_ROPE.pack(
+            queryOutput.data_ptr(), keyCache.data_ptr(), valueCache.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(),
+            self._weight("queryWeight", queryWeight, dtype), self._weight("keyWeight", keyWeight, dtype), _ints(c, "positions", positions, n),
+            _ints(c, "slots", slots, n), outStride, cache[1], cache[0], queryStride, keyStride, valueStride, code, n, self.numHeads,
+            self.numKVHeads, self.headSize, self.rotarySize, self.theta, eps))
+        if rc:
+            _lib.check(rc)
 
 
 class PrefixAttention(Module):
@@ -377,31 +388,38 @@ class PrefixAttention(Module):
         _use_torch()
         self.numHeads, self.numKVHeads, self.pageSize = config.numHeads, config.numKVHeads, pageSize
         self.headSize = config.dim // config.numHeads
-        self._size = _lib.declare(self.lib.ml2_prefix_attention_workspace, "p iiiiiii p")
-        self._call = _lib.declare(self.lib.ml2_prefix_attention, "p i pl p pl i pp i pi pp ii iii f pl")
+        self._sizes = {}
+        self._call = _lib.PREFIX_ATTENTION.entry(self.lib.ml2_prefix_attention)
 
     def WorkspaceBytes(self, rows, requests, prefixLength, maxLength):
-        """Size of the workspace for a call of these sizes or smaller ones; calls that may overlap need one each."""
-        n = ctypes.c_size_t()
-        _lib.check(self._size(self.ctx.handle, rows, requests, prefixLength, maxLength, self.numHeads, self.numKVHeads, self.headSize,
-                              ctypes.addressof(n)))
-        return n.value
+        """Size of the workspace for a call of these sizes; calls that may overlap need one each."""
+        sizes = (rows, requests, prefixLength, maxLength)
+        if sizes not in self._sizes:
+            n = ctypes.c_size_t()
+            _lib.check(self.lib.ml2_prefix_attention_workspace(ctypes.c_void_p(getattr(self.ctx.handle, "value", self.ctx.handle)), *sizes,
+                                                               self.numHeads, self.numKVHeads, self.headSize, ctypes.byref(n)))
+            if len(self._sizes) > 1000:
+                self._sizes.clear()
+            self._sizes[sizes] = n.value
+        return self._sizes[sizes]
 
     def Forward(self, output, query, prefixKey, prefixValue, keyCache, valueCache, table, lengths, queryStart, workspace, maxLength,
                 lse=None, scale=None):
         c, dtype, n = self.ctx, query.dtype, lengths.numel()
-        code, width, kvWidth, rows = _dtype_code(query, "query"), self.numHeads * self.headSize, self.numKVHeads * self.headSize, query.shape[0]
-        qs, os, cs = _rows(c, "query", query, width, dtype), _rows(c, "output", output, width, dtype), _rows(c, "keyCache", keyCache, kvWidth, dtype)
-        if _rows(c, "valueCache", valueCache, kvWidth, dtype) != cs or valueCache.shape[0] != keyCache.shape[0]:
+        code, width, kvWidth = _dtype_code(query, "query"), self.numHeads * self.headSize, self.numKVHeads * self.headSize
+        rows, queryStride = _rows(c, "query", query, width, dtype)
+        outRows, outStride = _rows(c, "output", output, width, dtype)
+        cache = _rows(c, "keyCache", keyCache, kvWidth, dtype)
+        if _rows(c, "valueCache", valueCache, kvWidth, dtype) != cache:
             raise ValueError("keyCache and valueCache must have the same rows and strides")
-        if output.shape[0] < rows or table.dim() != 2 or table.shape[0] != n:
-            raise ValueError("output needs %d rows and table %d; got %d and %s" % (rows, n, output.shape[0], tuple(table.shape)))
-        prefix = _lib.KVStruct(0, 0, kvWidth, 0)
+        if outRows < rows or table.dim() != 2 or table.shape[0] != n:
+            raise ValueError("output needs %d rows and table %d; got %d and %s" % (rows, n, outRows, tuple(table.shape)))
+        prefix, prefixKeyPtr, prefixValuePtr = (0, kvWidth), 0, 0
         if prefixKey is not None and prefixKey.shape[0] > 0:
-            ps = _rows(c, "prefixKey", prefixKey, kvWidth, dtype)
-            if _rows(c, "prefixValue", prefixValue, kvWidth, dtype) != ps or prefixValue.shape[0] != prefixKey.shape[0]:
+            prefix = _rows(c, "prefixKey", prefixKey, kvWidth, dtype)
+            if _rows(c, "prefixValue", prefixValue, kvWidth, dtype) != prefix:
                 raise ValueError("prefixKey and prefixValue must have the same rows and strides")
-            prefix = _lib.KVStruct(prefixKey.data_ptr(), prefixValue.data_ptr(), ps, prefixKey.shape[0])
+            prefixKeyPtr, prefixValuePtr = prefixKey.data_ptr(), prefixValue.data_ptr()
         lsePtr = 0
         if lse is not None:
             if lse.dtype is not _torch.float32 or lse.get_device() != c.device or not lse.is_contiguous() or lse.numel() < rows * self.numHeads:
@@ -409,9 +427,11 @@ class PrefixAttention(Module):
             lsePtr = lse.data_ptr()
         if workspace.get_device() != c.device or not workspace.is_contiguous():
             raise ValueError("workspace: expected a contiguous tensor on cuda:%d" % c.device)
-        cache = _lib.KVStruct(keyCache.data_ptr(), valueCache.data_ptr(), cs, keyCache.shape[0])
-        _lib.check(self._call(c.handle, code, output.data_ptr(), os, lsePtr, query.data_ptr(), qs, rows, ctypes.addressof(prefix),
-                              ctypes.addressof(cache), self.pageSize, _ints(c, "table", table, 1), table.shape[1],
-                              _ints(c, "lengths", lengths, n), _ints(c, "queryStart", queryStart, n + 1), n, maxLength, self.numHeads,
-                              self.numKVHeads, self.headSize, self.headSize ** -0.5 if scale is None else scale, workspace.data_ptr(),
-                              workspace.numel() * workspace.element_size()))
+        rc = self._call(c.handle, _lib.PREFIX_ATTENTION.pack(
+            output.data_ptr(), lsePtr, query.data_ptr(), prefixKeyPtr, prefixValuePtr, keyCache.data_ptr(), valueCache.data_ptr(),
+            _ints(c, "table", table, 1), _ints(c, "lengths", lengths, n), _ints(c, "queryStart", queryStart, n + 1), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), outStride, queryStride, prefix[1], cache[1], cache[0], code, rows, n, prefix[0],
+            maxLength, self.pageSize, table.shape[1], self.numHeads, self.numKVHeads, self.headSize,
+            self.headSize ** -0.5 if scale is None else scale))
+        if rc:
+            _lib.check(rc)

@@ -6,7 +6,7 @@ import re
 import pytest
 
 import managedllama2_b200 as ml2
-from managedllama2_b200 import _lib, modules
+from managedllama2_b200 import _lib
 
 E_INVALID = -1
 P = 1 << 20  # stands for a device pointer, 16-byte aligned; never dereferenced
@@ -26,19 +26,26 @@ def calls():
     yield lib, Context.handle, (block, keep)
 
 
+def call(function, arguments, values):
+    return function(values.pop("ctx"), arguments.pack(*(values[name] for name in arguments.names)))
+
+
 def refused(lib, rc, word):
     assert rc == E_INVALID, rc
     assert word in lib.ml2_last_error().decode(), lib.ml2_last_error()
 
 
-def test_declared_arguments_match_the_header():
+@pytest.mark.parametrize("name,arguments", [("ml2_block_tables_args", _lib.BLOCK_TABLES), ("ml2_qk_norm_rope_args", _lib.QK_NORM_ROPE),
+                                            ("ml2_prefix_attention_args", _lib.PREFIX_ATTENTION)])
+def test_argument_structs_match_the_header(name, arguments):
     text = re.sub(r"/\*.*?\*/", "", open(_lib.HEADER_PATH).read(), flags=re.S)
-    found = re.findall(r'declare\(self\.lib\.(ml2_\w+), "([^"]+)"', open(modules.__file__).read())
-    assert len(found) == 4
-    for name, kinds in found:
-        args = re.search(name + r"\s*\(([^;]*)\);", text, re.S).group(1).split(",")
-        want = "".join("p" if "*" in a else "l" if "long long" in a or "size_t" in a else "f" if "float" in a else "i" for a in args)
-        assert kinds.replace(" ", "") == want, name
+    members = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
+    names, kinds = [], ""
+    for line in members.split(";"):
+        for one in filter(None, (x.strip() for x in line.split(","))):
+            names.append(re.search(r"(\w+)$", one).group(1))
+            kinds += "p" if "*" in one else "l" if "long long" in line or "size_t" in line else "f" if "float" in line else "i"
+    assert names == arguments.names and kinds == arguments.kinds
 
 
 TABLES = dict(ctx=None, lengths=P, new_lengths=2 * P, n_requests=4, page_size=16, table=3 * P, table_stride=8, free_pages=4 * P, free_count=5 * P,
@@ -59,20 +66,16 @@ def test_block_tables_refusals(calls, change, word):
     lib, ctx, _ = calls
     a = dict(TABLES, ctx=ctx)
     a.update(change)
-    refused(lib, lib.ml2_block_tables(*a.values()), word)
+    refused(lib, call(lib.ml2_block_tables, _lib.BLOCK_TABLES, a), word)
 
 
-def kv(key=P, value=2 * P, stride=256, rows=64):
-    return _lib.KVStruct(key, value, stride, rows)
-
-
-ROPE = dict(ctx=None, dtype=0, query_out=P, query_out_stride=256, cache=kv(), query=2 * P, query_stride=256, key=3 * P, key_stride=256,
-            value=4 * P, value_stride=256, query_weight=0, key_weight=0, positions=5 * P, slots=6 * P, n_tokens=3, n_heads=2, n_kv_heads=2,
-            head_size=128, rotary_size=128, theta=10000.0, eps=1e-5)
+ROPE = dict(ctx=None, dtype=0, query_out=P, query_out_stride=256, key_cache=P, value_cache=2 * P, cache_stride=256, cache_rows=64, query=2 * P,
+            query_stride=256, key=3 * P, key_stride=256, value=4 * P, value_stride=256, query_weight=0, key_weight=0, positions=5 * P, slots=6 * P,
+            n_tokens=3, n_heads=2, n_kv_heads=2, head_size=128, rotary_size=128, theta=10000.0, eps=1e-5)
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(ctx=0), "null"), (dict(cache=None), "null"), (dict(cache=kv(key=0)), "null"), (dict(cache=kv(value=0)), "null"), (dict(query=0), "null"),
+    (dict(ctx=0), "null"), (dict(key_cache=0), "null"), (dict(value_cache=0), "null"), (dict(query=0), "null"),
     (dict(key=0), "null"), (dict(value=0), "null"), (dict(query_out=0), "null"), (dict(positions=0), "null"), (dict(slots=0), "null"),
     (dict(dtype=2), "dtype"), (dict(dtype=-1), "dtype"), (dict(n_tokens=-1), "n_tokens"), (dict(n_heads=3), "multiple"), (dict(n_kv_heads=0), "multiple"),
     (dict(n_heads=0), "multiple"), (dict(head_size=72), "head_size"), (dict(head_size=272), "head_size"), (dict(head_size=0), "head_size"),
@@ -80,44 +83,38 @@ ROPE = dict(ctx=None, dtype=0, query_out=P, query_out_stride=256, cache=kv(), qu
     (dict(theta=0.0), "theta"), (dict(theta=float("nan")), "theta"), (dict(theta=float("inf")), "theta"), (dict(eps=-1.0), "eps"),
     (dict(eps=float("nan")), "eps"), (dict(query_weight=P), "together"), (dict(key_weight=P), "together"),
     (dict(query_out_stride=248), "shorter"), (dict(query_stride=0), "shorter"), (dict(key_stride=128), "shorter"), (dict(value_stride=255), "shorter"),
-    (dict(cache=kv(stride=128)), "shorter"), (dict(cache=kv(rows=0)), "rows"), (dict(cache=kv(rows=2**31)), "rows"),
-    (dict(query_stride=260), "aligned"), (dict(query=2 * P + 8), "aligned"), (dict(cache=kv(value=P + 2)), "aligned"),
+    (dict(cache_stride=128), "shorter"), (dict(cache_rows=0), "rows"), (dict(cache_rows=2**31), "rows"),
+    (dict(query_stride=260), "aligned"), (dict(query=2 * P + 8), "aligned"), (dict(value_cache=P + 2), "aligned"),
     (dict(query_weight=P + 4, key_weight=P), "aligned"),
 ])
 def test_qk_norm_rope_refusals(calls, change, word):
     lib, ctx, _ = calls
     a = dict(ROPE, ctx=ctx)
     a.update(change)
-    if a["cache"] is not None:
-        a["cache"] = ctypes.addressof(a["cache"])
-    refused(lib, lib.ml2_qk_norm_rope(*a.values()), word)
+    refused(lib, call(lib.ml2_qk_norm_rope, _lib.QK_NORM_ROPE, a), word)
 
 
-ATTN = dict(ctx=None, dtype=0, out=P, out_stride=256, lse=0, query=2 * P, query_stride=256, n_rows=4, prefix=kv(rows=100), cache=kv(rows=160),
-            page_size=16, table=3 * P, table_stride=4, lengths=4 * P, query_start=5 * P, n_requests=4, max_length=64, n_heads=2, n_kv_heads=2,
+ATTN = dict(ctx=None, dtype=0, out=P, out_stride=256, lse=0, query=2 * P, query_stride=256, n_rows=4, prefix_key=P, prefix_value=2 * P,
+            prefix_length=100, prefix_stride=256, key_cache=P, value_cache=2 * P, cache_stride=256, cache_rows=160, page_size=16, table=3 * P, table_stride=4, lengths=4 * P, query_start=5 * P, n_requests=4, max_length=64, n_heads=2, n_kv_heads=2,
             head_size=128, scale=0.1, workspace=6 * P, workspace_bytes=1 << 40)
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(ctx=0), "null"), (dict(prefix=None), "null"), (dict(cache=None), "null"), (dict(out=0), "null"), (dict(query=0), "null"),
-    (dict(table=0), "null"), (dict(lengths=0), "null"), (dict(query_start=0), "null"), (dict(cache=kv(key=0)), "null"),
-    (dict(prefix=kv(value=0)), "null"), (dict(dtype=7), "dtype"), (dict(n_rows=-1), "n_rows"), (dict(n_requests=0), "n_requests"),
+    (dict(ctx=0), "null"), (dict(out=0), "null"), (dict(query=0), "null"),
+    (dict(table=0), "null"), (dict(lengths=0), "null"), (dict(query_start=0), "null"), (dict(key_cache=0), "null"),
+    (dict(prefix_value=0), "null"), (dict(dtype=7), "dtype"), (dict(n_rows=-1), "n_rows"), (dict(n_requests=0), "n_requests"),
     (dict(n_requests=8193), "n_requests"), (dict(n_heads=3), "multiple"), (dict(n_kv_heads=0), "multiple"), (dict(head_size=96), "head_size"),
     (dict(page_size=48), "page_size"), (dict(page_size=0), "page_size"), (dict(table_stride=0), "table_stride"), (dict(max_length=-1), "max_length"),
-    (dict(max_length=65), "max_length"), (dict(cache=kv(rows=0)), "rows"), (dict(cache=kv(rows=2**31)), "rows"), (dict(prefix=kv(rows=-1)), "rows"),
-    (dict(prefix=kv(rows=2**31)), "rows"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(out_stride=128), "shorter"),
-    (dict(query_stride=128), "shorter"), (dict(cache=kv(stride=128)), "shorter"), (dict(prefix=kv(stride=128)), "shorter"),
-    (dict(query=P + 8), "aligned"), (dict(out=P + 2), "aligned"), (dict(out_stride=260), "aligned"), (dict(cache=kv(key=P + 8)), "aligned"),
-    (dict(prefix=kv(stride=258)), "aligned"), (dict(workspace=P + 8), "aligned"), (dict(out=2 * P), "overlap"),
+    (dict(max_length=65), "max_length"), (dict(cache_rows=0), "rows"), (dict(cache_rows=2**31), "rows"), (dict(prefix_length=-1), "rows"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(out_stride=128), "shorter"),
+    (dict(query_stride=128), "shorter"), (dict(cache_stride=128), "shorter"), (dict(prefix_stride=128), "shorter"),
+    (dict(query=P + 8), "aligned"), (dict(out=P + 2), "aligned"), (dict(out_stride=260), "aligned"), (dict(key_cache=P + 8), "aligned"),
+    (dict(prefix_stride=258), "aligned"), (dict(workspace=P + 8), "aligned"), (dict(out=2 * P), "overlap"),
 ])
 def test_prefix_attention_refusals(calls, change, word):
     lib, ctx, _ = calls
     a = dict(ATTN, ctx=ctx)
     a.update(change)
-    for name in ("prefix", "cache"):
-        if a[name] is not None:
-            a[name] = ctypes.addressof(a[name])
-    refused(lib, lib.ml2_prefix_attention(*a.values()), word)
+    refused(lib, call(lib.ml2_prefix_attention, _lib.PREFIX_ATTENTION, a), word)
 
 
 @pytest.mark.parametrize("change,word", [
@@ -129,4 +126,12 @@ def test_prefix_attention_workspace_refusals(calls, change, word):
     n = ctypes.c_size_t()
     a = dict(ctx=ctx, n_rows=4, n_requests=4, prefix=100, max_length=64, n_heads=2, n_kv_heads=2, head_size=128, bytes=ctypes.addressof(n))
     a.update(change)
-    refused(lib, lib.ml2_prefix_attention_workspace(*a.values()), word)
+    kinds = [ctypes.c_void_p] + [ctypes.c_int] * 7 + [ctypes.c_void_p]
+    refused(lib, lib.ml2_prefix_attention_workspace(*(k(v) for k, v in zip(kinds, a.values()))), word)
+
+
+def test_missing_argument_structs_are_refused(calls):
+    lib, ctx, _ = calls
+    for function in (lib.ml2_block_tables, lib.ml2_qk_norm_rope, lib.ml2_prefix_attention):
+        refused(lib, function(ctx, None), "null")
+        refused(lib, function(None, None), "null")
