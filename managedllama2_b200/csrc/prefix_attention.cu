@@ -646,14 +646,17 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
         }
         __syncwarp();
     } else if (warp >= 16) {
-        // ---- the tensor core's queue, one thread for each stream ------------------------------------------------------
-        // (One for both was slower than the products: its own instructions, some 700 cycles for the eight or four products of
-        // a tile, bounded the kernel.)
-        if (lane == 0) {
+        // ---- the tensor core's queue, one warp for each stream ---------------------------------------------------------
+        // (One warp for both was slower than the products.) The whole warp goes through the loops and one lane issues: operands
+        // then lie in uniform registers, 22 cycles a product instead of 47 and more with one lane running all of it.
+        {
+            const bool leader = elect_one();
             constexpr uint32_t kShapeS = tc_shape(128, kKeyTile, kBf16, false), kShapeO = tc_shape(128, kHead, kBf16, true);
             const int s = warp - 16;
-            const uint32_t q_op = tc_operand_low(q_base + s * S::kQBytes, 16), k_op = tc_operand_low(k_ring, 16), v_op = tc_operand_low(v_ring, S::kHalf);
-            const uint32_t t_s = tmem + s * 128, t_o = tmem + 256 + s * 128;
+            auto same = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };  // a value known to be that of the whole warp
+            const uint32_t q_op = same(tc_operand_low(q_base + s * S::kQBytes, 16)), k_op = tc_operand_low(k_ring, 16), v_op = tc_operand_low(v_ring, S::kHalf);
+            const uint32_t t_s = tmem + s * 128, t_o = same(tmem + 256 + s * 128);
+            auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_for(bar, parity, p.wait_cycles, &s_abort)) != 0; };
             unsigned base = 0;                // first tile of the segment
             unsigned asked = 0, added = 0;    // S tiles queued since the start, and P tiles used
             unsigned turn_q = 0;              // Q tiles taken
@@ -665,18 +668,21 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                 auto scores = [&](int j) {
                     for (int t = j * step; t < min(n, (j + 1) * step); ++t) {
                         const unsigned g = base + t, slot = g % kRing;
-                        if (!mbar_wait_for(&b_k[slot], g / kRing & 1, p.wait_cycles, &s_abort)) return false;
+                        if (!wait(&b_k[slot], g / kRing & 1)) return false;
                         if (turns && (t & 1) != s) {
-                            mbar_arrive(&b_s[s][slot]);
+                            if (leader) mbar_arrive(&b_s[s][slot]);
                             continue;
                         }
                         tc_fence_after();
-                        const uint32_t k = k_op + slot * (S::kTileBytes >> 4), to = t_s + (asked++ & 1) * 64;
+                        const uint32_t k = same(k_op + slot * (S::kTileBytes >> 4)), to = same(t_s + (asked++ & 1) * 64);
+                        if (leader) {
 #pragma unroll
-                        for (int i = 0; i < kHead / 16; ++i)
-                            tc_mma_ss(to, tc_operand_at(q_op + (i / 4) * (S::kQHalf >> 4) + (i % 4) * 2),
-                                      tc_operand_at(k + (i / 4) * (S::kHalf >> 4) + (i % 4) * 2), kShapeS, i > 0);
-                        tc_commit(&b_s[s][slot]);
+                            for (int i = 0; i < kHead / 16; ++i)
+                                tc_mma_ss(to, tc_operand_at(q_op + (i / 4) * (S::kQHalf >> 4) + (i % 4) * 2),
+                                          tc_operand_at(k + (i / 4) * (S::kHalf >> 4) + (i % 4) * 2), kShapeS, i > 0);
+                            tc_commit(&b_s[s][slot]);
+                        }
+                        __syncwarp();
                     }
                     return true;
                 };
@@ -684,24 +690,27 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                 auto values = [&](int j) {
                     for (int t = j * step; t < min(n, (j + 1) * step); ++t) {
                         const unsigned g = base + t, slot = g % kRing;
-                        if (!mbar_wait_for(&b_v[slot], g / kRing & 1, p.wait_cycles, &s_abort)) return false;
+                        if (!wait(&b_v[slot], g / kRing & 1)) return false;
                         if (turns && (t & 1) != s) {
-                            mbar_arrive(&b_o[s][slot]);
+                            if (leader) mbar_arrive(&b_o[s][slot]);
                             continue;
                         }
-                        if (!mbar_wait_for(&b_p[s][added & 1], added >> 1 & 1, p.wait_cycles, &s_abort)) return false;
+                        if (!wait(&b_p[s][added & 1], added >> 1 & 1)) return false;
                         tc_fence_after();
-                        const uint32_t v = v_op + slot * (S::kTileBytes >> 4), from = t_s + (added++ & 1) * 64;
-                        tc_mma_ts(t_o, from, tc_operand_at(v), kShapeO, add);
+                        const uint32_t v = same(v_op + slot * (S::kTileBytes >> 4)), from = same(t_s + (added++ & 1) * 64), more = same(add);
+                        if (leader) {
+                            tc_mma_ts(t_o, from, tc_operand_at(v), kShapeO, more);
 #pragma unroll
-                        for (int k = 1; k < kKeyTile / 16; ++k) tc_mma_ts(t_o, from + k * 8, tc_operand_at(v + k * (2048 >> 4)), kShapeO, 1);
-                        tc_commit(&b_o[s][slot]);
+                            for (int k = 1; k < kKeyTile / 16; ++k) tc_mma_ts(t_o, from + k * 8, tc_operand_at(v + k * (2048 >> 4)), kShapeO, 1);
+                            tc_commit(&b_o[s][slot]);
+                        }
+                        __syncwarp();
                         add = 1;
                     }
                     return true;
                 };
                 // a stream without tiles hands over no Q: it could be two phases ahead of this wait otherwise
-                if (share(turns, n, s) && !mbar_wait_for(&b_q[s], turn_q++ & 1, p.wait_cycles, &s_abort)) return false;
+                if (share(turns, n, s) && !wait(&b_q[s], turn_q++ & 1)) return false;
                 if (!scores(0)) return false;
                 // S of the next step goes where P of the one before lay: behind the product that reads it
                 for (int j = 0; j * step < n; ++j)
@@ -710,7 +719,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                 return true;
             });
             if (!done) {  // products that are under way end before the TMEM is given back
-                tc_commit(&b_end[s]);
+                if (leader) tc_commit(&b_end[s]);
                 for (int i = 0; i < 1 << 20 && !mbar_try_wait(&b_end[s], 0); ++i) {}
             }
         }

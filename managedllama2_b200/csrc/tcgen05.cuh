@@ -8,6 +8,14 @@
 
 namespace ml2 {
 
+// true in one lane of a converged warp, always the same one
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 // ---- TMEM: 128 lanes x 512 columns of 32 bits; an address is lane << 16 | column -----------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t* s_addr, uint32_t columns)  // one whole warp
 {
