@@ -187,8 +187,9 @@ int ml2_qk_norm_rope(ml2_ctx* ctx, const ml2_qk_norm_rope_args* args);
  * -inf. Rows from query_start[n_requests] to n_rows stay as they are. Scores, softmax and sums are fp32; the weights are
  * rounded to `dtype` before their product with the values. Prefix rows and cache rows that no query sees are not used,
  * whatever they hold. max_length bounds lengths[]. head_size 64 or 128; strides in elements, multiples of 8; pointers
- * 16-byte aligned. `workspace` (ml2_prefix_attention_workspace bytes for the same sizes, or for larger n_rows, n_requests,
- * prefix and max_length) holds partial results: calls that may run at the same time need one each. */
+ * 16-byte aligned. `workspace` (at least ml2_prefix_attention_workspace bytes for the same sizes) holds partial results: calls that
+ * may run at the same time need one each. n_rows, prefix_length and max_length choose the kernels, the arrays on the device
+ * only the work: a captured call may be replayed with other lengths and query rows within them. */
 int ml2_prefix_attention_workspace(ml2_ctx* ctx, int n_rows, int n_requests, int prefix_length, int max_length, int n_heads,
                                    int n_kv_heads, int head_size, size_t* bytes);
 typedef struct ml2_prefix_attention_args {

@@ -17,7 +17,8 @@
 namespace ml2 {
 
 constexpr int kTablesThreads = 1024;
-constexpr int kTablesFill = 4096;  // up to here one CTA writes the slot map: @@
+// Up to this many rows one CTA writes the slot map. One kernel / two: 4096 rows 5.0 / 7.4 us, 8192 7.4 / 9.2, 32768 18.5 / 10.2.
+constexpr int kTablesFill = 8192;
 
 struct TablesParams {
     const int* lengths;
@@ -300,6 +301,7 @@ extern "C" int ml2_block_tables(ml2_ctx* h, const ml2_block_tables_args* args)
 
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(1);
+    // few requests and rows: the barriers of 8 warps cost less than those of 32 (64 requests 3.6 us instead of 4.1)
     cfg.blockDim = dim3(n_requests <= 256 && p.fill <= 1024 ? 256 : kTablesThreads);
     cfg.dynamicSmemBytes = (4 * (size_t)n_requests + 3) * sizeof(int);
     cfg.stream = ctx->stream;

@@ -49,9 +49,17 @@ __device__ __forceinline__ Span request_span(const AttnBatch& p, int r)
 }
 
 constexpr int kTile = 16;      // keys of a tile: the k of one m16n8k16 product with the values
-constexpr int kStages = 3;     // tiles of a warp's ring
+// tiles of a warp's ring: 24 KB at either head size, so that two blocks of four warps share an SM
+constexpr int stages(int head) { return head == 128 ? 3 : 6; }
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
+// The reference point m of a row moves only when a score exceeds it by more than this many powers of two: weights up to 2^8 fit
+// fp16 with room and sums are fp32, so the sums are rescaled a few times in all instead of at most tiles.
+constexpr float kSlack = 8.f;
+// Places of a run at least, where the longest sequence has n: a lone warp needs 0.7 us a place and the join 0.1 us a result, so
+// that n places are best left to 2 sqrt(n) runs. One place a run where there are more warps than places: 19.8 us instead of 13.3
+// for 8 heads of 8 and 1024 keys, 13.5 instead of 12.2 for 5 heads and 512; ten places: 17.1 and 15.9.
+__device__ __forceinline__ int shortest_run(int n) { return max(1, (int)(0.5f * sqrtf((float)n) + 0.5f)); }
 constexpr int kOpen = 1;       // what it costs to begin a sequence (its queries, its result), in key tiles: 2300 cycles against 2200
 
 template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -99,7 +107,26 @@ __device__ __forceinline__ int tiles_seen(const AttnBatch& p, int count, int len
     const int last = (row0 + rows - 1) / p.group, seen = min(length, length - count + last + 1);
     return seen > 0 ? (seen + kTile - 1) / kTile : 0;
 }
-__device__ __forceinline__ int places(int length) { return length ? kOpen + (length + kTile - 1) / kTile : 0; }
+// A request's share of the runs: `seqs` row tiles for each key head, the first of which sees `low` key tiles and the last `high`.
+// Places before row tile rt, for one key head: kOpen and the key tiles of each row tile, the latter taken to grow evenly from low
+// to high and, where they grow, two more, which covers every row tile (checked for heads of a group from 1 to 32; 7 % more
+// places than are needed, where `high` for all would be 70 % more).
+struct Share {
+    int seqs, low, high;
+};
+__device__ __forceinline__ Share request_share(const AttnBatch& p, int count, int length)
+{
+    const int n = row_tiles(p, count);
+    if (!n) return {0, 0, 0};
+    return {n, tiles_seen(p, count, length, 0, min(16, count * p.group)), tiles_seen(p, count, length, 16 * (n - 1), count * p.group - 16 * (n - 1))};
+}
+__device__ __forceinline__ int places_before(const Share& s, int rt)
+{
+    if (!s.high) return 0;
+    long long n = (long long)rt * (kOpen + s.low);
+    if (s.high > s.low) n += 2 * rt + (long long)(s.high - s.low) * rt * (rt - 1) / (2 * (s.seqs - 1));
+    return (int)n;
+}
 // Where the result of run `run` for the 16 rows from row0 on of a key head begins: runs and rows are numbered through, so that
 // no two results meet and all need no more than one entry per row and head, and 16 per run.
 __device__ __forceinline__ long long result_row(const AttnBatch& p, bool prefix, int first, int row0, int rows, int kvh, int run)
@@ -114,6 +141,7 @@ struct Walk {
     int request;               // n_requests: the prefix
     int rt, kvh, k;            // row tile, key head, place in the sequence
     int first, count, length;  // query rows and keys of the request
+    Share share;
     int places, need, rows;    // places of a sequence, those up to the last key tile that its rows see, its rows
 };
 __device__ __forceinline__ void open_request(const AttnBatch& p, Walk& w, int total_rows)
@@ -128,11 +156,13 @@ __device__ __forceinline__ void open_request(const AttnBatch& p, Walk& w, int to
         w.count = s.count;
         w.length = s.length;
     }
-    w.places = places(w.length);
+    const int all = (w.length + kTile - 1) / kTile;
+    w.share = w.request == p.n_requests ? Share{row_tiles(p, w.count), all, all} : request_share(p, w.count, w.length);
 }
 __device__ __forceinline__ void open_rows(const AttnBatch& p, Walk& w)
 {
     w.rows = min(16, w.count * p.group - w.rt * 16);
+    w.places = places_before(w.share, w.rt + 1) - places_before(w.share, w.rt);
     w.need = w.request == p.n_requests ? w.places : kOpen + tiles_seen(p, w.count, w.length, w.rt * 16, w.rows);
 }
 __device__ __forceinline__ void open_walk(const AttnBatch& p, const int* s_base, int total_rows, Walk& w)
@@ -146,12 +176,19 @@ __device__ __forceinline__ void open_walk(const AttnBatch& p, const int* s_base,
     }
     w.request = lo;
     open_request(p, w, total_rows);
-    const int local = w.pos - s_base[lo], seq = local / w.places;
-    w.k = local - seq * w.places;
-    // key heads, next to one another in the cache, go to neighbouring runs
-    w.rt = seq / p.n_kv;
-    w.kvh = seq - w.rt * p.n_kv;
+    const int local = w.pos - s_base[lo];
+    int rt = 0;
+    for (int n = w.share.seqs; n > 1;) {
+        const int half = n >> 1;
+        if (places_before(w.share, rt + half) * p.n_kv <= local) rt += half;
+        n -= half;
+    }
+    w.rt = rt;
     open_rows(p, w);
+    // key heads, next to one another in the cache, go to neighbouring runs
+    const int rest = local - places_before(w.share, rt) * p.n_kv;
+    w.kvh = rest / w.places;
+    w.k = rest - w.kvh * w.places;
 }
 // Moves to the next key tile that somebody sees; false at the end of the run.
 __device__ __forceinline__ bool settle(const AttnBatch& p, const int* s_base, int total_rows, Walk& w)
@@ -169,7 +206,7 @@ __device__ __forceinline__ bool settle(const AttnBatch& p, const int* s_base, in
         if (w.pos >= w.end) return false;
         if (++w.kvh < p.n_kv) continue;
         w.kvh = 0;
-        if (++w.rt == row_tiles(p, w.count)) {
+        if (++w.rt == w.share.seqs) {
             w.rt = 0;
             do ++w.request;
             while (s_base[w.request + 1] == s_base[w.request]);
@@ -187,16 +224,17 @@ __device__ __forceinline__ bool settle(const AttnBatch& p, const int* s_base, in
 template <typename T, int kHead>
 __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const __grid_constant__ AttnBatch p)
 {
-    constexpr int kRowBytes = kHead * 2, kChunks = kHead / 8, kTileBytes = kTile * kRowBytes, kSteps = kHead / 16;
+    constexpr int kRowBytes = kHead * 2, kChunks = kHead / 8, kTileBytes = kTile * kRowBytes, kSteps = kHead / 16, kStages = stages(kHead);
     extern __shared__ __align__(128) unsigned char s_mem[];
     __shared__ unsigned s_valid[kAttnWarps][kStages];
-    __shared__ int s_sum[kAttnWarps];
+    __shared__ int s_sum[kAttnWarps], s_long[kAttnWarps];
     int* s_base = reinterpret_cast<int*>(s_mem + kAttnWarps * kStages * 2 * kTileBytes);  // places before request r; the prefix last
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // after the prefix kernel, which has waited for what comes before both, this one starts beside it
     if (!p.prefix_ctas) pdl_wait();
     const int total_rows = min(max(p.query_start[p.n_requests], 0), p.n_rows);
+    int longest = kOpen + (p.prefix_ctas ? 0 : (p.prefix + kTile - 1) / kTile);
     // ---- how many places every request has -----------------------------------------------------------------------------
     {
         const int per = ceil_div(p.n_requests, kAttnThreads), r0 = min((int)threadIdx.x * per, p.n_requests), r1 = min(r0 + per, p.n_requests);
@@ -205,7 +243,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
             const Span s = request_span(p, r);
             if (!s.good && blockIdx.x == 0) report_input_error(p.status, kInputLength, r);
             s_base[r] = mine;
-            mine += row_tiles(p, s.count) * p.n_kv * places(s.length);
+            const Share share = request_share(p, s.count, s.length);
+            mine += places_before(share, share.seqs) * p.n_kv;
+            longest = max(longest, kOpen + share.high);
         }
         int incl = mine;
 #pragma unroll
@@ -213,22 +253,27 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += v;
         }
-        if (lane == 31) s_sum[warp] = incl;
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        if (lane == 31) {
+            s_sum[warp] = incl;
+            s_long[warp] = longest;
+        }
         __syncthreads();
         int base = incl - mine, all = 0;
 #pragma unroll
         for (int w = 0; w < kAttnWarps; ++w) {
             if (w < warp) base += s_sum[w];
             all += s_sum[w];
+            longest = max(longest, s_long[w]);
         }
         for (int r = r0; r < r1; ++r) s_base[r] += base;
         if (threadIdx.x == 0) {
             s_base[p.n_requests] = all;
-            s_base[p.n_requests + 1] = all + (p.prefix_ctas ? 0 : row_tiles(p, total_rows) * p.n_kv * places(p.prefix));
+            s_base[p.n_requests + 1] = all + (p.prefix_ctas || !p.prefix ? 0 : row_tiles(p, total_rows) * p.n_kv * (kOpen + (p.prefix + kTile - 1) / kTile));
         }
         __syncthreads();
     }
-    const int all = s_base[p.n_requests + 1], per = (all + gridDim.x * kAttnWarps - 1) / (gridDim.x * kAttnWarps), run = blockIdx.x * kAttnWarps + warp;
+    const int all = s_base[p.n_requests + 1], per = max(shortest_run(longest), (all + (int)gridDim.x * kAttnWarps - 1) / ((int)gridDim.x * kAttnWarps)), run = blockIdx.x * kAttnWarps + warp;
     if (blockIdx.x == 0) {  // the join finds the results by these
         for (int r = threadIdx.x; r <= p.n_requests; r += kAttnThreads) p.run_base[r] = s_base[r];
         if (threadIdx.x == 0) p.run_base[p.n_requests + 1] = per;
@@ -245,7 +290,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
     open_walk(p, s_base, total_rows, ld);
     Walk w = ld;
     bool more = settle(p, s_base, total_rows, ld);
-    long long row = -1;  // lanes 0..15: cache row of the tile's key `lane`, -1 for none
+    int row = -1;  // lanes 0..15: cache row of the tile's key `lane`, -1 for none
     auto find_rows = [&]() {
         const int key = (ld.k - kOpen) * kTile + (lane & 15);
         row = -1;
@@ -253,7 +298,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
             if (ld.request == p.n_requests) row = key;
             else {
                 const int page = p.table[(long long)ld.request * p.table_stride + (key >> p.page_shift)];
-                if (page >= 0 && page < p.n_pages) row = ((long long)page << p.page_shift) + (key & page_mask);
+                if (page >= 0 && page < p.n_pages) row = (page << p.page_shift) + (key & page_mask);
                 else report_input_error(p.status, kInputPage, ld.request);
             }
         }
@@ -261,20 +306,19 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
     auto load_tile = [&](int stage) {
         if (more) {
             const bool prefix = ld.request == p.n_requests;
-            const T* kb = static_cast<const T*>(prefix ? p.pk : p.k) + (long long)ld.kvh * kHead;
-            const T* vb = static_cast<const T*>(prefix ? p.pv : p.v) + (long long)ld.kvh * kHead;
-            const long long step = prefix ? p.prefix_stride : p.cache_stride;
+            const char* kb = static_cast<const char*>(prefix ? p.pk : p.k) + (ld.kvh * kHead + lane % kChunks * 8) * 2;
+            const char* vb = static_cast<const char*>(prefix ? p.pv : p.v) + (ld.kvh * kHead + lane % kChunks * 8) * 2;
+            const unsigned step = (unsigned)(prefix ? p.prefix_stride : p.cache_stride) * 2u;  // bytes, below 2^32
             const unsigned valid = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
             if (lane == 0) s_valid[warp][stage] = valid;
-            const uint32_t dst = ring_u32 + stage * 2 * kTileBytes;
+            const uint32_t dst = ring_u32 + stage * 2 * kTileBytes + lane / kChunks * kRowBytes;
 #pragma unroll
             for (int i = 0; i < kChunks / 2; ++i) {
-                const int at = i * 32 + lane, key = at / kChunks, c = at % kChunks;
-                const long long r = __shfl_sync(0xffffffffu, row, key);
-                const long long off = r < 0 ? 0 : r * step + c * 8;
-                const uint32_t to = dst + key * kRowBytes + ((c ^ (key & 7)) << 4);
-                cp_async16(to, kb + off, r < 0 ? 0 : 16);
-                cp_async16(to + kTileBytes, vb + off, r < 0 ? 0 : 16);
+                const int key = i * (32 / kChunks) + lane / kChunks, r = __shfl_sync(0xffffffffu, row, key), bytes = r < 0 ? 0 : 16;
+                const unsigned long long off = (unsigned long long)(unsigned)max(r, 0) * step;
+                const uint32_t to = dst + i * (32 / kChunks) * kRowBytes + (((lane % kChunks) ^ (key & 7)) << 4);
+                cp_async16(to, kb + off, bytes);
+                cp_async16(to + kTileBytes, vb + off, bytes);
             }
             ++ld.k;
             ++ld.pos;
@@ -329,14 +373,19 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
 
             float s[2][4] = {};
             {
+                float odd[2][4] = {};  // the steps alternate between two sums: half as long a chain of products
                 const int kr = (lane & 7) + ((lane >> 4) & 1) * 8, kc = (lane >> 3) & 1;
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
                     uint32_t b[4];
                     ldsm4(b, kt + kr * kRowBytes + (((2 * k + kc) ^ (kr & 7)) << 4));
-                    mma16816<T>(s[0], qf[k], b[0], b[1]);
-                    mma16816<T>(s[1], qf[k], b[2], b[3]);
+                    mma16816<T>(k & 1 ? odd[0] : s[0], qf[k], b[0], b[1]);
+                    mma16816<T>(k & 1 ? odd[1] : s[1], qf[k], b[2], b[3]);
                 }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][e] += odd[n][e];
             }
             const bool causal = key + kTile > seen_by_all && seen_by_all < w.length, masked = valid != 0xffffu || causal;
 #pragma unroll
@@ -355,10 +404,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
             t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
             t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
             t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
-            const float n0 = fmaxf(mx0, t0), n1 = fmaxf(mx1, t1);
-            const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-            if (__any_sync(0xffffffffu, n0 > mx0 || n1 > mx1)) {  // a larger score: what was summed shrinks
-                const float c0 = exp2_fast(mx0 - b0), c1 = exp2_fast(mx1 - b1);
+            if (__any_sync(0xffffffffu, t0 > mx0 + kSlack || t1 > mx1 + kSlack)) {  // a much larger score: what was summed shrinks
+                const float n0 = t0 > mx0 + kSlack ? t0 : mx0, n1 = t1 > mx1 + kSlack ? t1 : mx1;
+                const float c0 = n0 == mx0 ? 1.f : exp2_fast(mx0 - n0), c1 = n1 == mx1 ? 1.f : exp2_fast(mx1 - n1);
                 l0 *= c0;
                 l1 *= c1;
 #pragma unroll
@@ -371,6 +419,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
                 mx0 = n0;
                 mx1 = n1;
             }
+            const float b0 = mx0 == -INFINITY ? 0.f : mx0, b1 = mx1 == -INFINITY ? 0.f : mx1;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 s[n][0] = exp2_fast(s[n][0] - b0);
@@ -420,7 +469,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
                     __syncwarp();
                 }
             }
-            // weights of at most 1, rounded to 16 bits for the product: the same half step the output's own rounding costs
+            // weights of at most 2^kSlack, rounded to 16 bits for the product: the same half step the output's own rounding costs
             const uint32_t pf[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]), pack2<T>(s[1][2], s[1][3])};
             {
                 const int vr = (lane & 7) + ((lane >> 3) & 1) * 8, vc = lane >> 4;
@@ -462,19 +511,18 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
 // cut into one contiguous run per CTA, so all CTAs do the same work within one tile and a block's runs ("segments") are
 // joined afterwards. Two streams of a CTA alternate on the tensor core:
 //   S = Q K^T (operands in shared memory, S in TMEM, two of them a stream: one is filled while the other is used),
-//   P = exp2(S - m), rounded to 16 bits, over S in TMEM   (256 threads, half a row each; with 128 the exponentials' latency
-//                                                          was open: 70 us instead of @@ for 1024 rows and 16384 keys of 8 heads)
+//   P = exp2(S - m), rounded to 16 bits, over S in TMEM   (256 threads, half a row each)
 //   O += P V (P from TMEM, V as it lies: MN-major)
 // With more than 128 rows both streams use each key tile, the first with rows 0..127, the second with 128..255. With fewer,
 // both have the same rows and take the key tiles in turn: then HBM bounds the kernel and eight tiles of 16 KB are under way.
-// The reference point m of a row moves only when a score exceeds it by more than 8 (weights up to 2^8 fit fp16 with room, and
-// sums are fp32): O is rescaled in TMEM a few times in all instead of at every tile.
 constexpr int kBlockRows = 256;
 constexpr int kKeyTile = 64;
 constexpr int kRing = 4;                 // key tiles in shared memory, and value tiles
 constexpr int kBlockThreads = 608;       // per stream 8 softmax warps and one that feeds the tensor core; load warp
-constexpr float kSlack = 8.f;
-constexpr int kBlockPrefix = 512;        // from this length on the prefix is done by blocks
+// From which length on the prefix is done by blocks, not by runs, with up to 16 rows of a key head and with more. Measured (us by
+// blocks / by runs): 1 row of 40 heads, 1024 keys 17.8 / 14.9, 4096 27.0 / 27.9, 8192 38.9 / 41.6; 64 rows of 40 heads, 512 keys
+// 26.2 / 21.7, 1024 28.6 / 28.1, 2048 33.0 / 37.3; 512 rows of 8 heads, 512 keys 23.6 / 22.0, 1024 24.3 / 30.5, 4096 32.2 / 84.4.
+constexpr int kBlockPrefixFewRows = 4096, kBlockPrefix = 1024;
 
 struct PrefixMaps {
     CUtensorMap k, v;
@@ -742,7 +790,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
         };
         unsigned base = 0;  // first tile of the segment
         // The stream's product with the values of tile g is done. Not asked for before the one of tile g - 4 is seen to be done, and
-        // the slot is not used again before this: a block has at least eight tiles (kBlockPrefix), so that a stream has no tile only
+        // the slot is not used again before this: a block has more than eight tiles (kBlockPrefix), so that a stream has no tile only
         // in a run's first or last segment.
         auto o_done = [&](unsigned g) { wait(&b_o[s][g % kRing], g / kRing & 1); };
         for_segments([&](int kvh, int block, int tile, int n) {
@@ -904,7 +952,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
 
 // Joins the partial results of one row and head: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. A block takes one row and
 // some of its heads: the row's request is looked up once, the warps then go from head to head. (One warp for each row and head,
-// all of them looking up: 50 us instead of @@ for 1229 rows of 32 heads.)
+// all of them looking up: 50 us instead of 36 for 1229 rows of 32 heads, cold.)
 constexpr int kJoinWarps = 8;
 template <typename T, int kHead>
 __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const __grid_constant__ AttnBatch p)
@@ -953,7 +1001,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
             pre_at = id;
             pre_step = (long long)total_rows * p.n_heads;
         } else if (p.prefix) {
-            const int m = t * p.group + g, row0 = m & ~15, rows = min(16, total_rows * p.group - row0), n = places(p.prefix);
+            const int m = t * p.group + g, row0 = m & ~15, rows = min(16, total_rows * p.group - row0), n = kOpen + (p.prefix + kTile - 1) / kTile;
             const int a = s_row[4] + ((row0 >> 4) * p.n_kv + kvh) * n, first = (a + kOpen) / per;
             pre = (a + n - 1) / per - first + 1;
             pre_at = result_row(p, true, 0, row0, rows, kvh, first) + (m & 15);
@@ -963,7 +1011,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
         }
         if (length > 0) {
             const int m = (t - first_row) * p.group + g, row0 = m & ~15, rows = min(16, count * p.group - row0);
-            const int a = s_row[3] + ((row0 >> 4) * p.n_kv + kvh) * places(length) + kOpen, first = a / per, need = tiles_seen(p, count, length, row0, rows);
+            const Share share = request_share(p, count, length);
+            const int before = places_before(share, row0 >> 4), here = places_before(share, (row0 >> 4) + 1) - before;
+            const int a = s_row[3] + before * p.n_kv + kvh * here + kOpen, first = a / per, need = tiles_seen(p, count, length, row0, rows);
             own = need ? (a + need - 1) / per - first + 1 : 0;
             own_at = result_row(p, false, first_row, row0, rows, kvh, first) + (m & 15);
         }
@@ -1030,8 +1080,8 @@ static AttnPlan plan_attention(const Ctx* ctx, int n_rows, int n_requests, int p
     if (!n_rows) return pl;
     const int sms = std::max(1, ctx->sm_count);
     const long long rows = (long long)n_rows * (n_heads / n_kv);  // of a key head
-    long long pre_rows = 0, run_rows = 0, run_tiles = (n_requests + rows / 16) * n_kv * (max_length ? kOpen + ceil_div(max_length, kTile) : 0);
-    if (prefix >= kBlockPrefix) {
+    long long pre_rows = 0, run_rows = 0, run_tiles = (n_requests + rows / 16) * n_kv * (max_length ? kOpen + ceil_div(max_length, kTile) + 3 : 0);
+    if (prefix >= (rows <= 16 ? kBlockPrefixFewRows : kBlockPrefix)) {
         const long long blocks = (rows + kBlockRows - 1) / kBlockRows, key_tiles = ceil_div(prefix, kKeyTile);
         pl.tiles = blocks * n_kv * key_tiles;
         pl.prefix_ctas = (int)std::min<long long>(sms, pl.tiles);
@@ -1101,7 +1151,7 @@ static cudaError_t launch_attention(Ctx* ctx, const AttnBatch& p, const AttnPlan
     if (pl.run_ctas) {
         cfg.gridDim = dim3(pl.run_ctas);
         cfg.blockDim = dim3(kAttnThreads);
-        cfg.dynamicSmemBytes = kAttnWarps * kStages * 2 * kTile * kHead * 2 + (p.n_requests + 2) * sizeof(int);
+        cfg.dynamicSmemBytes = kAttnWarps * stages(kHead) * 2 * kTile * kHead * 2 + (p.n_requests + 2) * sizeof(int);
         if ((e = cudaLaunchKernelEx(&cfg, attention_runs_kernel<T, kHead>, p)) != cudaSuccess) return e;
         ++ctx->launches;
         cfg.numAttrs = 1;
@@ -1165,6 +1215,8 @@ int ml2_prefix_attention(ml2_ctx* h, const ml2_prefix_attention_args* args)
     if ((out_stride | query_stride | cache_stride | prefix_stride) % 8 || !aligned_to(16, out, query, key_cache, value_cache) ||
         !aligned_to(16, prefix_key, prefix_value, workspace))
         return fail(ML2_E_INVALID, "prefix_attention: pointers must be 16-byte aligned and row strides multiples of 8 elements");
+    if (cache_stride > INT32_MAX / 2 || prefix_stride > INT32_MAX / 2)
+        return fail(ML2_E_INVALID, "prefix_attention: cache rows are further apart than 2^30 elements");
     if (out == query) return fail(ML2_E_INVALID, "prefix_attention: out must not overlap the queries");
     const AttnPlan pl = plan_attention(ctx, n_rows, n_requests, prefix_length, max_length, n_heads, n_kv_heads, head_size);
     if (pl.tiles > INT32_MAX / 2 || (long long)n_rows * (n_heads / n_kv_heads) > INT32_MAX / 2 || (long long)n_rows * n_heads > INT32_MAX)

@@ -180,9 +180,10 @@ extern "C" int ml2_qk_norm_rope(ml2_ctx* h, const ml2_qk_norm_rope_args* args)
         double f = 0.15915494309189533577;  // 1 / (2 pi)
         for (int i = 0; i < rotary_size / 2; ++i, f *= ratio) p.turns[i] = f;
     }
-    // one pass with up to kRopeThreads threads; a few tokens with many heads are cut over several blocks of 256
+    // Up to kRopeThreads threads a token; while the tokens do not fill the SMs, their heads are cut over blocks of 256 threads (40
+    // heads of 128: 1 token 2.8 us instead of 4.1, 128 tokens 4.1 instead of 4.6, 256 tokens 5.7 against 5.4).
     const int lanes = (n_heads + 2 * n_kv_heads) * p.lanes;
-    const bool few = n_tokens * 2 < ctx->sm_count;
+    const bool few = n_tokens <= ctx->sm_count;
     const int threads = std::min(few ? 256 : kRopeThreads, ceil_div(lanes, 32) * 32);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)n_tokens, few ? (unsigned)std::min(ceil_div(lanes, threads), std::max(1, 2 * ctx->sm_count / n_tokens)) : 1u);

@@ -108,7 +108,7 @@ ATTN = dict(ctx=None, dtype=0, out=P, out_stride=256, lse=0, query=2 * P, query_
     (dict(max_length=65), "max_length"), (dict(cache_rows=0), "rows"), (dict(cache_rows=2**31), "rows"), (dict(prefix_length=-1), "rows"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(out_stride=128), "shorter"),
     (dict(query_stride=128), "shorter"), (dict(cache_stride=128), "shorter"), (dict(prefix_stride=128), "shorter"),
     (dict(query=P + 8), "aligned"), (dict(out=P + 2), "aligned"), (dict(out_stride=260), "aligned"), (dict(key_cache=P + 8), "aligned"),
-    (dict(prefix_stride=258), "aligned"), (dict(workspace=P + 8), "aligned"), (dict(out=2 * P), "overlap"),
+    (dict(prefix_stride=258), "aligned"), (dict(cache_stride=2**30), "further apart"), (dict(prefix_stride=2**31), "further apart"), (dict(workspace=P + 8), "aligned"), (dict(out=2 * P), "overlap"),
 ])
 def test_prefix_attention_refusals(calls, change, word):
     lib, ctx, _ = calls
