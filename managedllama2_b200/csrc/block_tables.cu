@@ -276,7 +276,9 @@ extern "C" int ml2_block_tables(ml2_ctx* h, const ml2_block_tables_args* args)
                 page_size, table_stride, n_pages, max_tokens, position_offset] = *args;
     if (!lengths || !new_lengths || !table || !free_pages || !free_count || !lengths_out || !free_count_out || !query_start || !refused)
         return fail(ML2_E_INVALID, "block_tables: null argument");
-    if (max_tokens < 0 || (max_tokens > 0 && (!slots || !positions)))
+    if (!aligned_to(4, lengths, new_lengths, table, free_pages, free_count) || !aligned_to(4, lengths_out, free_count_out, query_start, slots, positions, refused))
+        return fail(ML2_E_INVALID, "block_tables: arrays must be 4-byte aligned");
+    if (max_tokens < 0 || max_tokens > INT32_MAX / 2 || (max_tokens > 0 && (!slots || !positions)))
         return fail(ML2_E_INVALID, "block_tables: max_tokens=%d with slots=%p positions=%p", max_tokens, (void*)slots, (void*)positions);
     if (n_requests < 1 || n_requests > kMaxRequests)
         return fail(ML2_E_INVALID, "block_tables: n_requests=%d must be 1..%d", n_requests, kMaxRequests);

@@ -1213,11 +1213,10 @@ int ml2_prefix_attention(ml2_ctx* h, const ml2_prefix_attention_args* args)
     if (out_stride < q_width || query_stride < q_width || cache_stride < kv_width || (prefix_length && prefix_stride < kv_width))
         return fail(ML2_E_INVALID, "prefix_attention: a row stride is shorter than the row");
     if ((out_stride | query_stride | cache_stride | prefix_stride) % 8 || !aligned_to(16, out, query, key_cache, value_cache) ||
-        !aligned_to(16, prefix_key, prefix_value, workspace))
-        return fail(ML2_E_INVALID, "prefix_attention: pointers must be 16-byte aligned and row strides multiples of 8 elements");
+        !aligned_to(16, prefix_key, prefix_value, workspace) || !aligned_to(4, lse, table, lengths, query_start))
+        return fail(ML2_E_INVALID, "prefix_attention: pointers must be 16-byte aligned (lse and int arrays 4) and row strides multiples of 8 elements");
     if (cache_stride > INT32_MAX / 2 || prefix_stride > INT32_MAX / 2)
         return fail(ML2_E_INVALID, "prefix_attention: cache rows are further apart than 2^30 elements");
-    if (out == query) return fail(ML2_E_INVALID, "prefix_attention: out must not overlap the queries");
     const AttnPlan pl = plan_attention(ctx, n_rows, n_requests, prefix_length, max_length, n_heads, n_kv_heads, head_size);
     if (pl.tiles > INT32_MAX / 2 || (long long)n_rows * (n_heads / n_kv_heads) > INT32_MAX / 2 || (long long)n_rows * n_heads > INT32_MAX)
         return fail(ML2_E_INVALID, "prefix_attention: n_rows=%d with %d heads is too much for one call", n_rows, n_heads);

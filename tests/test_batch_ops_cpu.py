@@ -56,7 +56,7 @@ TABLES = dict(ctx=None, lengths=P, new_lengths=2 * P, n_requests=4, page_size=16
 @pytest.mark.parametrize("change,word", [
     (dict(ctx=0), "null"), (dict(lengths=0), "null"), (dict(new_lengths=0), "null"), (dict(table=0), "null"), (dict(free_pages=0), "null"),
     (dict(free_count=0), "null"), (dict(lengths_out=0), "null"), (dict(free_count_out=0), "null"), (dict(query_start=0), "null"),
-    (dict(refused=0), "null"), (dict(slots=0), "slots"), (dict(positions=0), "positions"), (dict(max_tokens=-1), "max_tokens"),
+    (dict(refused=0), "null"), (dict(slots=0), "slots"), (dict(positions=0), "positions"), (dict(max_tokens=-1), "max_tokens"), (dict(max_tokens=2**31 - 1), "max_tokens"), (dict(slots=P + 2), "aligned"), (dict(table=P + 1), "aligned"),
     (dict(n_requests=0), "n_requests"), (dict(n_requests=8193), "n_requests"), (dict(page_size=0), "page_size"), (dict(page_size=24), "page_size"),
     (dict(page_size=2048), "page_size"), (dict(table_stride=0), "table_stride"), (dict(n_pages=0), "n_pages"),
     (dict(position_offset=-1), "32 bits"), (dict(position_offset=2**31 - 100), "32 bits"), (dict(n_pages=2**27), "32 bits"),
@@ -85,7 +85,7 @@ ROPE = dict(ctx=None, dtype=0, query_out=P, query_out_stride=256, key_cache=P, v
     (dict(query_out_stride=248), "shorter"), (dict(query_stride=0), "shorter"), (dict(key_stride=128), "shorter"), (dict(value_stride=255), "shorter"),
     (dict(cache_stride=128), "shorter"), (dict(cache_rows=0), "rows"), (dict(cache_rows=2**31), "rows"),
     (dict(query_stride=260), "aligned"), (dict(query=2 * P + 8), "aligned"), (dict(value_cache=P + 2), "aligned"),
-    (dict(query_weight=P + 4, key_weight=P), "aligned"),
+    (dict(query_weight=P + 4, key_weight=P), "aligned"), (dict(slots=P + 2), "aligned"),
 ])
 def test_qk_norm_rope_refusals(calls, change, word):
     lib, ctx, _ = calls
@@ -108,7 +108,7 @@ ATTN = dict(ctx=None, dtype=0, out=P, out_stride=256, lse=0, query=2 * P, query_
     (dict(max_length=65), "max_length"), (dict(cache_rows=0), "rows"), (dict(cache_rows=2**31), "rows"), (dict(prefix_length=-1), "rows"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(out_stride=128), "shorter"),
     (dict(query_stride=128), "shorter"), (dict(cache_stride=128), "shorter"), (dict(prefix_stride=128), "shorter"),
     (dict(query=P + 8), "aligned"), (dict(out=P + 2), "aligned"), (dict(out_stride=260), "aligned"), (dict(key_cache=P + 8), "aligned"),
-    (dict(prefix_stride=258), "aligned"), (dict(cache_stride=2**30), "further apart"), (dict(prefix_stride=2**31), "further apart"), (dict(workspace=P + 8), "aligned"), (dict(out=2 * P), "overlap"),
+    (dict(prefix_stride=258), "aligned"), (dict(cache_stride=2**30), "further apart"), (dict(prefix_stride=2**31), "further apart"), (dict(workspace=P + 8), "aligned"), (dict(table=P + 2), "aligned"), (dict(lse=P + 1), "aligned"),
 ])
 def test_prefix_attention_refusals(calls, change, word):
     lib, ctx, _ = calls

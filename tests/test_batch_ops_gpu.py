@@ -420,7 +420,9 @@ def test_attention_prefix_lengths(ctx, prefix):
 
 @pytest.mark.parametrize("heads,kv,head,prefix,requests", [
     (40, 40, 128, 4032, 1), (40, 40, 128, 4032, 64), (5, 5, 128, 513, 3), (37, 37, 64, 640, 2), (16, 2, 128, 2048, 16), (16, 2, 128, 2049, 17),
-    (24, 3, 64, 1111, 33), (8, 1, 64, 9000, 65), (64, 64, 64, 600, 130), (3, 1, 128, 700, 300), (12, 12, 128, 1500, 257)])
+    (24, 3, 64, 1111, 33), (8, 1, 64, 9000, 65), (64, 64, 64, 600, 130), (3, 1, 128, 700, 300), (12, 12, 128, 1500, 257),
+    (5, 5, 128, 1025, 33), (37, 37, 64, 1100, 20), (64, 64, 64, 1088, 130), (3, 1, 128, 1300, 300), (40, 40, 128, 4096, 1), (8, 8, 64, 4200, 2),
+    (1, 1, 128, 20000, 1), (2, 2, 64, 1024, 513)])
 def test_attention_prefix_in_blocks(ctx, heads, kv, head, prefix, requests):
     """Runs of key tiles that begin and end anywhere in a head, blocks of up to 128, 129..256 and more rows; called twenty
     times over without waiting."""
@@ -428,8 +430,8 @@ def test_attention_prefix_in_blocks(ctx, heads, kv, head, prefix, requests):
     b = Batch(prefix + heads, "fp16" if heads % 2 else "bf16", heads, kv, head, 16, prefix, lengths, [1] * requests, extra_rows=2)
     first, z = b.check(ctx)
     op = ml2.PrefixAttention(ctx, b.cfg, 16)
-    ws = torch.full((op.WorkspaceBytes(b.q.shape[0], requests, prefix, 30),), 0xFF, dtype=torch.uint8, device="cuda")
-    results = [b.call(ctx, workspace=ws, max_length=30) for _ in range(20)]
+    ws = torch.full((op.WorkspaceBytes(b.q.shape[0], requests, prefix, max(lengths)),), 0xFF, dtype=torch.uint8, device="cuda")
+    results = [b.call(ctx, workspace=ws) for _ in range(20)]
     for out, lse in results:
         assert torch.equal(out, first) and torch.equal(lse, z)
 
@@ -614,10 +616,10 @@ def test_modules_refuse_wrong_tensors(ctx):
 
 
 # ---- together ----------------------------------------------------------------------------------------------------------
-def decode_steps(ctx, graph):
+def decode_steps(ctx, graph, prefix):
     """Four samples behind one prompt, five steps: prompts of different length first, then one token each, one request that
     ends and one that begins; returns what the last step gave and the plain form of it."""
-    heads, kv, head, page, width, prefix = 6, 2, 64, 16, 8, 77
+    heads, kv, head, page, width = 6, 2, 64, 16, 8
     cfg = ml2.Config(heads * head, 0, 1, heads, kv, 0, 0)
     g = torch.Generator(device="cuda").manual_seed(11)
     pk, pv = (torch.randn(prefix, kv * head, generator=g, device="cuda").half() for _ in range(2))
@@ -693,6 +695,67 @@ def decode_steps(ctx, graph):
     return out[:row].clone()
 
 
-def test_decode_steps_together_and_in_a_graph(ctx):
-    eager = decode_steps(ctx, graph=False)
-    assert torch.equal(eager, decode_steps(ctx, graph=True))
+@pytest.mark.parametrize("prefix", [0, 77, 1500])  # none, by runs, by blocks
+def test_decode_steps_together_and_in_a_graph(ctx, prefix):
+    eager = decode_steps(ctx, False, prefix)
+    assert torch.equal(eager, decode_steps(ctx, True, prefix))
+
+
+def test_samples_behind_a_prompt_in_a_transformers_own_cache(ctx):
+    """The prompt goes through ``Transformer.Forward`` token by token; layer 0's rows of its key and value caches are then
+    the shared prefix, in place."""
+    cfg = ml2.Config(256, 768, 2, 2, 2, 512, 64)
+    tr = ml2.Transformer(cfg, ml2.synthetic_weights(ctx, cfg, seed=3, sigma=1.0), ctx)
+    prompt = [7, 99, 300, 5, 41, 17, 250, 8, 130]
+    tr.set_tokens(prompt)
+    for pos in range(len(prompt)):
+        tr.Forward(pos, pos + 1, False)
+    tr.synchronize()
+    rs = tr.runstate_ptrs()
+
+    class Rows:  # the library's own buffer as a tensor
+        def __init__(self, ptr):
+            self.__cuda_array_interface__ = {"shape": (cfg.seqLength, cfg.dim), "typestr": "<f2", "data": (ptr, False), "version": 2}
+    k, v = (torch.as_tensor(Rows(p), device="cuda")[:len(prompt)] for p in (rs.key_cache, rs.value_cache))
+    assert bool((k != 0).any()) and bool((v != 0).any())
+    b = Batch(12, "fp16", 2, 2, 128, 16, len(prompt), [4, 30, 1], [1, 1, 1])
+    b.pk, b.pv = k, v
+    b.check(ctx)
+    tr.close()
+
+
+@pytest.mark.parametrize("prefix", [300, 2000])
+def test_attention_over_its_own_queries(ctx, prefix):
+    b = Batch(prefix, "bf16", 8, 2, 128, 16, prefix, [70, 3, 40], [1, 2, 9], extra_rows=1)
+    want, z = b.call(ctx)
+    q = b.q.clone()
+    op = ml2.PrefixAttention(ctx, b.cfg, 16)
+    ws = torch.empty(op.WorkspaceBytes(13, 3, prefix, 70), dtype=torch.uint8, device="cuda")
+    op.Forward(q, q, b.pk, b.pv, b.k, b.v, b.table, b.lengths, b.start, ws, 70)
+    assert torch.equal(q[:12], want[:12]) and torch.equal(q[12:], b.q[12:])
+
+
+@pytest.mark.parametrize("head", [64, 128])
+def test_calls_of_two_contexts_at_the_same_time(head):
+    """Two contexts, each with its stream and workspace, the same kernels from both in flight together."""
+    cases = []
+    for i in range(2):
+        c, s = ml2.CudaContext(0), torch.cuda.Stream()
+        b = Batch(20 + i, "fp16", 8, 2, head, 16, 2000 + 100 * i, *ragged(i, 40, 120, 1))
+        want, z = b.check(c)
+        op = ml2.PrefixAttention(c, b.cfg, 16)
+        ws = torch.empty(op.WorkspaceBytes(40, 40, b.prefix, 120), dtype=torch.uint8, device="cuda")
+        outs = [(torch.zeros(40, 8 * head, dtype=b.t, device="cuda"), torch.zeros(40, 8, device="cuda")) for _ in range(10)]
+        torch.cuda.synchronize()
+        c.set_stream(s.cuda_stream)
+        cases.append((c, s, b, op, ws, outs, want, z))
+    for k in range(10):
+        for c, s, b, op, ws, outs, want, z in cases:
+            op.Forward(outs[k][0], b.q, b.pk, b.pv, b.k, b.v, b.table, b.lengths, b.start, ws, 120, outs[k][1])
+    for c, s, b, op, ws, outs, want, z in cases:
+        s.synchronize()
+        for out, lse in outs:
+            assert torch.equal(out, want) and torch.equal(lse, z)
+        assert c.status() == (0, 0)
+        c.close()
+
