@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // after the prefix kernel, which has waited for what comes before both, this one starts beside it
     if (!p.prefix_ctas) pdl_wait();
+    pdl_launch_dependents();  // every block is resident by the time the join's come, which look up their rows meanwhile
     const int total_rows = min(max(p.query_start[p.n_requests], 0), p.n_rows);
     int longest = kOpen + (p.prefix_ctas ? 0 : (p.prefix + kTile - 1) / kTile);
     // ---- how many places every request has -----------------------------------------------------------------------------
@@ -959,10 +960,14 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
 {
     constexpr int kPer = kHead / 32;
     __shared__ int s_row[6];  // first query row, queries, length, places before the request, before the prefix, of a run
-    pdl_wait();
+    // what stood in these arrays before the call's first kernel is there already: that kernel has waited for it
     const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (!p.run_ctas && !p.prefix_ctas) pdl_wait();
     const int total_rows = min(p.query_start[p.n_requests], p.n_rows);
-    if (t >= total_rows) return;
+    if (t >= total_rows) {
+        pdl_wait();  // all the same: what follows in the stream follows this kernel
+        return;
+    }
     if (warp == 0) {
         // the request of this row: the lanes look at 32 places at a time
         int lo = 0;
@@ -975,6 +980,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
         }
         const Span s = request_span(p, lo);
         const bool own = p.run_ctas && s.good && t >= s.first && t < s.first + s.count;
+        pdl_wait();
         if (lane == 0) {
             s_row[0] = s.first;
             s_row[1] = s.count;
@@ -984,6 +990,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
             s_row[5] = p.run_ctas ? max(p.run_base[p.n_requests + 1], 1) : 1;
         }
     }
+    pdl_wait();  // the results, from here on
     __syncthreads();
     const int first_row = s_row[0], count = s_row[1], length = s_row[2], per = s_row[5];
     for (int h = blockIdx.y * kJoinWarps + warp; h < p.n_heads; h += gridDim.y * kJoinWarps) {
