@@ -993,9 +993,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
     pdl_wait();  // the results, from here on
     __syncthreads();
     const int first_row = s_row[0], count = s_row[1], length = s_row[2], per = s_row[5];
+    // what the heads have in common (integer divisions are most of this kernel's instructions)
+    const PrefixRuns runs = p.prefix_ctas ? prefix_runs(total_rows, p.group, p.n_kv, p.prefix, p.prefix_ctas) : PrefixRuns{};
+    const Share share = length > 0 ? request_share(p, count, length) : Share{0, 0, 0};
+    int row_tile = -1, before = 0, here_places = 0, need = 0, rows16 = 0;  // of the row tile last seen
     for (int h = blockIdx.y * kJoinWarps + warp; h < p.n_heads; h += gridDim.y * kJoinWarps) {
         const long long id = (long long)t * p.n_heads + h;
-        const int g = h % p.group, kvh = h / p.group;
+        const int kvh = h / p.group, g = h - kvh * p.group;
         // results: of the prefix (by blocks: `step` apart; by runs), then of the own tokens
         long long pre_at = 0, pre_step = 0, own_at = 0;
         int pre = 0, own = 0;
@@ -1003,7 +1007,6 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
         const float2 *pre_ml = p.pre_ml, *own_ml = p.run_ml;
         if (p.prefix_ctas) {
             int first;
-            const PrefixRuns runs = prefix_runs(total_rows, p.group, p.n_kv, p.prefix, p.prefix_ctas);
             block_segments(runs, kvh, (t * p.group + g) / kBlockRows, &first, &pre);
             pre_at = id;
             pre_step = (long long)total_rows * p.n_heads;
@@ -1017,12 +1020,17 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
             pre_ml = p.run_ml;
         }
         if (length > 0) {
-            const int m = (t - first_row) * p.group + g, row0 = m & ~15, rows = min(16, count * p.group - row0);
-            const Share share = request_share(p, count, length);
-            const int before = places_before(share, row0 >> 4), here = places_before(share, (row0 >> 4) + 1) - before;
-            const int a = s_row[3] + before * p.n_kv + kvh * here + kOpen, first = a / per, need = tiles_seen(p, count, length, row0, rows);
+            const int m = (t - first_row) * p.group + g, row0 = m & ~15;
+            if (row0 >> 4 != row_tile) {
+                row_tile = row0 >> 4;
+                rows16 = min(16, count * p.group - row0);
+                before = places_before(share, row_tile);
+                here_places = places_before(share, row_tile + 1) - before;
+                need = tiles_seen(p, count, length, row0, rows16);
+            }
+            const int a = s_row[3] + before * p.n_kv + kvh * here_places + kOpen, first = a / per;
             own = need ? (a + need - 1) / per - first + 1 : 0;
-            own_at = result_row(p, false, first_row, row0, rows, kvh, first) + (m & 15);
+            own_at = result_row(p, false, first_row, row0, rows16, kvh, first) + (m & 15);
         }
         const int splits = pre + own;
 

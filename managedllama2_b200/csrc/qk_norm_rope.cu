@@ -27,7 +27,7 @@ struct RopeParams {
     const int *positions, *slots;
     DeviceStatus* status;
     long long q_out_stride, cache_stride, q_stride, k_stride, v_stride, n_slots;
-    int n_heads, n_kv, head, rotary, lanes;  // lanes: threads of one head, a power of two
+    int n_heads, n_kv, head, rotary, lanes, lanes_log2;  // lanes: threads of one head, a power of two
     float eps, per_head;                     // per_head: 1 / head
     double turns[kRopeMaxHead / 2];          // theta^(-2 i / rotary) / (2 pi)
 };
@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_kernel(const __g
 {
     __shared__ float2 s_unit[kRopeMaxHead / 2];
     const long long t = blockIdx.x;
-    const int lane = threadIdx.x % p.lanes, per_block = blockDim.x / p.lanes, units = p.head >> 4, turned = p.rotary >> 4, half = p.rotary >> 1;
+    const int lane = threadIdx.x & (p.lanes - 1), per_block = blockDim.x >> p.lanes_log2, units = p.head >> 4, turned = p.rotary >> 4, half = p.rotary >> 1;
     const int at0 = lane < turned ? 8 * lane : 16 * lane, at1 = lane < turned ? 8 * lane + half : 16 * lane + 8;
     const int heads = p.n_heads + 2 * p.n_kv;
     auto source = [&](int h) {
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_kernel(const __g
         return static_cast<const T*>(p.v) + t * p.v_stride + (long long)(h - p.n_kv) * p.head;
     };
     pdl_wait();
-    int h = blockIdx.y * per_block + threadIdx.x / p.lanes;
+    int h = blockIdx.y * per_block + (threadIdx.x >> p.lanes_log2);
     uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
     if (lane < units && h < heads) {
         const T* in = source(h);
@@ -91,9 +91,13 @@ __global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_kernel(const __g
         unpack8<T>(x0, a);
         unpack8<T>(x1, b);
         if (p.qw) {
-            float ss = 0.f;
+            float ss = 0.f, st = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + b[e] * b[e];
+            for (int e = 0; e < 8; ++e) {
+                ss = fmaf(a[e], a[e], ss);
+                st = fmaf(b[e], b[e], st);
+            }
+            ss += st;
             for (int o = p.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             if (here && w) {
                 const float inv = rsqrtf(ss * p.per_head + p.eps);
@@ -173,7 +177,10 @@ extern "C" int ml2_qk_norm_rope(ml2_ctx* h, const ml2_qk_norm_rope_args* args)
     p.q_stride = query_stride; p.k_stride = key_stride; p.v_stride = value_stride; p.n_slots = cache_rows;
     p.n_heads = n_heads; p.n_kv = n_kv_heads; p.head = head_size; p.rotary = rotary_size; p.eps = eps; p.per_head = 1.0f / (float)head_size;
     p.lanes = 1;
-    while (p.lanes * 16 < head_size) p.lanes *= 2;
+    while (p.lanes * 16 < head_size) {
+        p.lanes *= 2;
+        ++p.lanes_log2;
+    }
     if (rotary_size) {
         // one pow, then products: i of them leave a relative error of i 2^-53, far below what the angle needs
         const double ratio = std::pow((double)theta, -2.0 / rotary_size);
