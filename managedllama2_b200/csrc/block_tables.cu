@@ -8,7 +8,8 @@
 // One CTA does the sums in shared memory, then the lists, cut evenly over its threads, each element finding its request by
 // bisection of the sums. What bounds it is latency: loads of the lengths, the scan's barriers, dependent loads and the store.
 // Where the tokens are many (a step that brings prompts), a second kernel of many CTAs writes the slot map from the finished
-// table: 196000 tokens of 512 requests took the one CTA 150 us.
+// table: 186000 tokens of 512 requests take 14.7 us, 13 of them the first kernel's; one CTA alone took 150. 64 requests that grow
+// by one token take 3.6 us.
 #include "../../include/ml2b200.h"
 
 #include "batch_common.cuh"

@@ -218,9 +218,12 @@ __device__ __forceinline__ bool settle(const AttnBatch& p, const int* s_base, in
 }
 
 // Every warp works for itself: the key tiles of all requests, one after the other, and one place more for every sequence, are
-// cut into runs of the same length, one a warp (without that place runs through short requests took 1.5 times as long). It streams its tiles through a ring of its own (cp.async; the next two are under way while one is used, across the
-// borders of sequences) and leaves a result for every sequence that it has a part of. 16 rows are all the tensor core's m16
-// has, so a tile of 16 keys (8 KB at head 128) costs 32 products however few rows are real; at one row HBM still bounds it.
+// cut into runs of the same length, one a warp (without that place runs through short requests took 1.5 times as long). It
+// streams its tiles through a ring of its own (cp.async; the next ones are under way while one is used, across the borders of
+// sequences) and leaves a result for every sequence that it has a part of. 16 rows are all the tensor core's m16 has, so a tile of
+// 16 keys (8 KB at head 128) costs 32 products however few rows are real: with one row a request HBM bounds it (64 requests of 135
+// tokens, 40 heads of 128: 173 MB in 36 us, 4.8 TB/s), with many the instructions and their latency (1229 queries of 8 requests,
+// 32 heads: 53000 tiles in 67 us, the keys read again for every 16 queries).
 template <typename T, int kHead>
 __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const __grid_constant__ AttnBatch p)
 {
@@ -515,7 +518,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
 //   P = exp2(S - m), rounded to 16 bits, over S in TMEM   (256 threads, half a row each)
 //   O += P V (P from TMEM, V as it lies: MN-major)
 // With more than 128 rows both streams use each key tile, the first with rows 0..127, the second with 128..255. With fewer,
-// both have the same rows and take the key tiles in turn: then HBM bounds the kernel and eight tiles of 16 KB are under way.
+// both have the same rows and take the key tiles in turn: then HBM bounds the kernel and eight tiles of 16 KB are under way
+// (64 rows of 40 heads, 4032 keys: 83 MB in 22 us, start included). With many rows the products themselves (N = 64 reads its
+// operands from shared memory at 47 cycles a product instead of 32) and the instructions of the warps that queue them bound it:
+// 1024 rows of 8 heads, 16384 keys: 69 GFLOP in 78 us, the tensor pipe 55 % active. Without the softmax it takes 12 us less,
+// without seven of eight products 31 us less. S tiles of 128 keys, one a stream, took 100 us.
 constexpr int kBlockRows = 256;
 constexpr int kKeyTile = 64;
 constexpr int kRing = 4;                 // key tiles in shared memory, and value tiles
