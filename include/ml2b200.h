@@ -180,7 +180,7 @@ typedef struct ml2_qk_norm_rope_args {
     float theta, eps;
 } ml2_qk_norm_rope_args;
 int ml2_qk_norm_rope(ml2_ctx* ctx, const ml2_qk_norm_rope_args* args);
-/* Attention of a batch that shares a prefix. Query rows query_start[r] .. query_start[r + 1] - 1 belong to request r, whose
+/* Attention of a batch that shares a prefix. Query rows query_start[r] .. query_start[r + 1] - 1 belong to request r (query_start[0] is 0), whose
  * lengths[r] own tokens (the new ones included) lie in the pages table[r]; row i of `queries` sees all prefix_length rows of
  * the prefix and own tokens 0 .. lengths[r] - queries + i. out[row][head] = softmax(scale q.k) v (out may be query); lse (may be null, fp32
  * [n_rows][n_heads]) = log sum exp(scale q.k). A row that sees nothing, or whose scores are all -inf, gives zeros and

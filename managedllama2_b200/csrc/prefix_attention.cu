@@ -44,7 +44,7 @@ struct Span {
 __device__ __forceinline__ Span request_span(const AttnBatch& p, int r)
 {
     const int a = p.query_start[r], b = p.query_start[r + 1], length = p.lengths[r];
-    const bool good = a >= 0 && b >= a && b <= p.n_rows && length >= 0 && length <= p.max_length;
+    const bool good = a >= 0 && (r > 0 || a == 0) && b >= a && b <= p.n_rows && length >= 0 && length <= p.max_length;
     return good ? Span{a, b - a, length, true} : Span{0, 0, 0, false};
 }
 

@@ -479,6 +479,38 @@ def test_attention_peaked_and_flat_scores(ctx, sigma, scale):
     Batch(5, "fp16", 4, 2, 64, 16, 333, [70, 1, 20], [1, 1, 9], sigma=sigma).check(ctx, scale=scale)
 
 
+@pytest.mark.parametrize("sigma,scale", [(30.0, None), (0.0, None), (2.0, 0.0), (2.0, -0.3), (200.0, 1.0)])
+@pytest.mark.parametrize("requests", [17, 150])
+def test_attention_peaked_and_flat_scores_in_blocks(ctx, sigma, scale, requests):
+    """The reference point moves with a score that is much larger: first tiles of small scores, then larger and larger ones."""
+    b = Batch(7, "fp16", 4, 2, 128, 16, 1500, [20] * requests, [1] * requests, sigma=sigma)
+    b.check(ctx, scale=scale)
+    b.pk *= (torch.arange(1500, device="cuda") / 300)[:, None].half()
+    b.check(ctx, scale=scale)
+
+
+@pytest.mark.parametrize("requests", [17, 150])
+def test_attention_infinite_scores_in_blocks(ctx, requests):
+    b = Batch(2, "bf16", 2, 2, 64, 16, 1100, [20] * requests, [1] * requests)
+    b.q[:, 0], b.q[:, 64] = 1.0, 1.0
+    clean, _ = b.call(ctx)
+    b.pk[3, 0] = float("-inf")  # one key of head 0 has no weight
+    out, z = b.call(ctx)
+    want, lse, tol, tol_lse = b.want()
+    assert bool(((out.double() - want).abs() <= torch.nan_to_num(tol, posinf=1.0)).all()) and bool(z.isfinite().all())
+    assert torch.equal(out[:, 64:], clean[:, 64:])
+    b.pk[:, 0] = float("-inf")  # none of the prefix has: the own tokens alone
+    out, z = b.call(ctx)
+    own = Batch(2, "bf16", 2, 2, 64, 16, 1100, [20] * requests, [1] * requests)
+    own.q[:, 0], own.q[:, 64] = 1.0, 1.0
+    own.pk, own.pv, own.prefix = own.pk[:0], own.pv[:0], 0
+    want, lse, tol, tol_lse = own.want()
+    assert bool(((out.double() - want).abs() <= tol)[:, :64].all()) and bool(((z.double() - lse).abs() <= tol_lse)[:, 0].all())
+    b.pk[5, 64] = float("inf")  # and NaN for every row of head 1
+    out, z = b.call(ctx)
+    assert bool(out[:, 64:].isnan().all()) and bool(out[:, :64].isfinite().all())
+
+
 def test_attention_without_log_sums_equals_with(ctx):
     b = Batch(9, "fp16", 4, 4, 128, 16, 500, [70, 3], [1, 2])
     assert torch.equal(b.call(ctx, lse=False)[0], b.call(ctx)[0])
@@ -547,7 +579,7 @@ def test_attention_bad_tables_are_left_out_and_reported(ctx):
         ctx.status()
 
 
-@pytest.mark.parametrize("start", [[0, 3, 1, 2], [5, 6, 7, 8], [0, 1, 2, 2**31 - 1], [-5, 0, 1, 2], [0, -1, -2, -3]])
+@pytest.mark.parametrize("start", [[0, 3, 1, 2], [1, 1, 2, 3], [5, 6, 7, 8], [0, 1, 2, 2**31 - 1], [-5, 0, 1, 2], [0, -1, -2, -3]])
 def test_attention_query_rows_out_of_order_stay_in_bounds(ctx, start):
     b = Batch(4, "fp16", 2, 2, 64, 16, 30, [40, 40, 3], [1, 1, 1])
     b.start = ints(start)
@@ -699,6 +731,12 @@ def decode_steps(ctx, graph, prefix):
 def test_decode_steps_together_and_in_a_graph(ctx, prefix):
     eager = decode_steps(ctx, False, prefix)
     assert torch.equal(eager, decode_steps(ctx, True, prefix))
+    ctx.set_pdl(True)  # programmatic launch edges between the calls too
+    try:
+        assert torch.equal(eager, decode_steps(ctx, False, prefix))
+        assert torch.equal(eager, decode_steps(ctx, True, prefix))
+    finally:
+        ctx.set_pdl(False)
 
 
 def test_samples_behind_a_prompt_in_a_transformers_own_cache(ctx):
