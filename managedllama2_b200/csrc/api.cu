@@ -278,8 +278,9 @@ int ml2_ctx_status(ml2_ctx* h, unsigned* error, unsigned* detail)
     DeviceStatus both[2] = {};
     cudaError_t e = cudaMemcpyAsync(both, c->status_dev, sizeof(both), cudaMemcpyDeviceToHost, c->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
-    const DeviceStatus& st = both[0].error ? both[0] : both[1];
-    if (e == cudaSuccess && st.error) e = cudaMemsetAsync(c->status_dev, 0, sizeof(both), c->stream);
+    const int which = both[0].error ? 0 : 1;  // the other word, if it is set too, is reported by the next call
+    const DeviceStatus& st = both[which];
+    if (e == cudaSuccess && st.error) e = cudaMemsetAsync(c->status_dev + which, 0, sizeof(st), c->stream);
     if (e != cudaSuccess) return fail(ML2_E_CUDA, "status: %s", cudaGetErrorString(e));
     if (error) *error = st.error;
     if (detail) *detail = st.detail;

@@ -986,6 +986,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
             n = min(step, n - k * step);
         }
         const Span s = request_span(p, lo);
+        if (!s.good && lane == 0) report_input_error(p.status, kInputLength, lo);
         const bool own = p.run_ctas && s.good && t >= s.first && t < s.first + s.count;
         pdl_wait();
         if (lane == 0) {

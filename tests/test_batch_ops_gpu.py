@@ -588,6 +588,18 @@ def test_attention_query_rows_out_of_order_stay_in_bounds(ctx, start):
         ctx.status()
 
 
+@pytest.mark.parametrize("prefix", [30, 1200])
+def test_attention_lengths_above_a_bound_of_zero_are_reported(ctx, prefix):
+    """A call for no own tokens at all: a request that has some gets the prefix alone, and is reported."""
+    b = Batch(4, "fp16", 34, 2, 64, 16, prefix, [0, 0, 0], [1, 1, 1])
+    want, z = b.check(ctx)
+    b.lengths = ints([0, 7, 0])
+    out, z2 = b.call(ctx, max_length=0)
+    with pytest.raises(ml2.Ml2Error, match="length or the query rows of request 1"):
+        ctx.status()
+    assert torch.equal(out, want) and torch.equal(z, z2)
+
+
 def test_attention_same_result_twice_and_on_another_stream(ctx):
     b = Batch(6, "bf16", 8, 2, 128, 16, 1000, *ragged(6, 20, 100, 1))
     first, z = b.check(ctx)
