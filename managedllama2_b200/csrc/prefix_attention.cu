@@ -23,7 +23,7 @@ struct AttnBatch {
     DeviceStatus* status;
     DeviceStatus* waits;
     // Partial results, for a row and head the sum o = sum of exp2(score - m) v over some of the keys [head], and (m, l): a
-    // reference near the largest score (in powers of two) and l = sum of exp2(score - m). One without keys has m = -inf, l = 0
+    // reference up to 2^15 below the largest score (in powers of two) and l = sum of exp2(score - m). One without keys has m = -inf, l = 0
     // and an o that is not read. pre: of the prefix by blocks, [segments][rows that are there][n_heads]; run: of the warps' runs.
     float *pre_o, *run_o;
     float2 *pre_ml, *run_ml;
@@ -53,9 +53,12 @@ constexpr int kTile = 16;      // keys of a tile: the k of one m16n8k16 product 
 constexpr int stages(int head) { return head == 128 ? 3 : 6; }
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-// The reference point m of a row moves only when a score exceeds it by more than this many powers of two: weights up to 2^8 fit
-// fp16 with room and sums are fp32, so the sums are rescaled a few times in all instead of at most tiles.
-constexpr float kSlack = 8.f;
+// The reference point m of a row is set kLower powers of two below a score and moves only when one exceeds it by more than
+// kSlack: weights of at most 2^15 fit fp16 and sums are fp32, so the sums are rescaled a few times in all instead of at most
+// tiles. Set as low as that, it leaves fp16 (whose smallest number is 2^-24) the weights down to 2^-32 of the largest: 65536
+// keys of 2^-25.06 each beside one of 1 had no part in the output at all with m at the score itself. (The difference t - m is
+// exact where it matters; t > m + kSlack could let 2^16 pass, which is infinite in fp16, where scores of 2^24 are 2 apart.)
+constexpr float kSlack = 15.f, kLower = 7.f;
 // Places of a run at least, where the longest sequence has n: a lone warp needs 0.7 us a place and the join 0.1 us a result, so
 // that n places are best left to 2 sqrt(n) runs. One place a run where there are more warps than places: 19.8 us instead of 13.3
 // for 8 heads of 8 and 1024 keys, 13.5 instead of 12.2 for 5 heads and 512; ten places: 17.1 and 15.9.
@@ -408,8 +411,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
             t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
             t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
             t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
-            if (__any_sync(0xffffffffu, t0 > mx0 + kSlack || t1 > mx1 + kSlack)) {  // a much larger score: what was summed shrinks
-                const float n0 = t0 > mx0 + kSlack ? t0 : mx0, n1 = t1 > mx1 + kSlack ? t1 : mx1;
+            if (__any_sync(0xffffffffu, t0 - mx0 > kSlack || t1 - mx1 > kSlack)) {  // a much larger score: what was summed shrinks
+                const float n0 = t0 - mx0 > kSlack ? t0 - kLower : mx0, n1 = t1 - mx1 > kSlack ? t1 - kLower : mx1;
                 const float c0 = n0 == mx0 ? 1.f : exp2_fast(mx0 - n0), c1 = n1 == mx1 ? 1.f : exp2_fast(mx1 - n1);
                 l0 *= c0;
                 l1 *= c1;
@@ -858,12 +861,12 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                     float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                     t = t == -INFINITY ? t : t * scale;
                     // both halves have their S in registers after this barrier, so P may go over it
-                    if (pair_any(pair, t > m + kSlack || m == -INFINITY)) {
+                    if (pair_any(pair, t - m > kSlack || m == -INFINITY)) {
                         s_top[s][half][row] = t;
                         named_bar_sync(pair, 64);
                         t = fmaxf(t, s_top[s][half ^ 1][row]);
-                        const bool move = t > m + kSlack || m == -INFINITY;
-                        const float to = move ? t : m, ref = to == -INFINITY ? 0.f : to, c = move ? exp2_fast(m - ref) : 1.f;
+                        const bool move = t - m > kSlack || m == -INFINITY;
+                        const float to = move ? t - kLower : m, ref = to == -INFINITY ? 0.f : to, c = move ? exp2_fast(m - ref) : 1.f;
                         m = to;
                         const uint64_t c2 = two(c, c);
                         sum[0] = fma2(sum[0], c2, 0);

@@ -1,0 +1,83 @@
+"""Edges of the batched-decoding operators: what a call may hold beyond the ordinary (long flat tails under a peak, scales of
+zero, broken tables, request counts around a limit of the launch) and memory that a call must leave alone."""
+import math
+import os
+import random
+import subprocess
+import sys
+
+import pytest
+import torch
+
+import managedllama2_b200 as ml2
+import test_batch_ops_gpu as base
+from test_batch_ops_gpu import Batch, ints
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = ml2.CudaContext(0)
+    c.set_wait_limit(2 * 10**9)
+    yield c
+    c.close()
+
+
+@pytest.fixture(autouse=True)
+def clean(ctx):
+    yield
+    assert ctx.status() == (0, 0)
+
+
+# ---- many small weights under one large one --------------------------------------------------------------------------------
+# One key scores 0 powers of two and has values of 0, all others score -25.0625 and have values of 1: next to a weight of 1
+# theirs are less than half of fp16's smallest number, but together they are the output, keys * 2^-25.0625 and a little less.
+# A reference point at least 2^7 below the largest score leaves them a rounding of at most 2^-32 each. The rest is relative to
+# the output: half a step of its own, 2^-11; 32-bit sums of keys / 8 weights (2^-24 each) and of keys / 16 products (2^-23).
+FLAT, PEAK_ROOM = -25.0625, 7
+
+
+def flat_tail(rows, columns):
+    k, v = torch.zeros(rows, columns, device="cuda", dtype=torch.float16), torch.ones(rows, columns, device="cuda", dtype=torch.float16)
+    k[1:, ::64] = FLAT
+    v[0] = 0
+    return k, v
+
+
+def check_flat_tail(out, lse, keys):
+    tail = (keys - 1) * 2.0 ** FLAT
+    want = tail / (1 + tail)
+    bound = keys * 2.0 ** (-25 - PEAK_ROOM) + want * (2.0 ** -11 + keys / 8 * 2.0 ** -24 + keys / 16 * 2.0 ** -23) + 2.0 ** -25
+    worst = (out.double() - want).abs().max().item()
+    assert worst <= bound, "off by %.3g, %.3g allowed" % (worst, bound)
+    assert (lse.double() - math.log1p(tail)).abs().max().item() <= keys / 8 * 2.0 ** -24 + 2.0 ** -20
+
+
+@pytest.mark.parametrize("rows", [1, 130])
+def test_attention_long_flat_tail_in_blocks(ctx, rows):
+    """As many key heads as SMs: one block walks through most of a head's keys."""
+    heads, keys = 148, 65536
+    pk, pv = flat_tail(keys, heads * 64)
+    q = torch.zeros(rows, heads * 64, device="cuda", dtype=torch.float16)
+    q[:, ::64] = 1
+    own = torch.zeros(16, heads * 64, device="cuda", dtype=torch.float16)
+    op = ml2.PrefixAttention(ctx, ml2.Config(heads * 64, 0, 1, heads, heads, 0, 0), 16)
+    ws = torch.empty(op.WorkspaceBytes(rows, 1, keys, 0), dtype=torch.uint8, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros(rows, heads, device="cuda")
+    op.Forward(out, q, pk, pv, own, own, ints([[0]]), ints([0]), ints([0, rows]), ws, 0, lse, math.log(2.0))
+    check_flat_tail(out, lse, keys)
+
+
+def test_attention_long_flat_tail_in_own_pages(ctx):
+    """As many requests and key heads as warps, all over the same pages: one warp walks through most of a request's keys."""
+    heads, requests, keys, page = 4, 296, 65536, 64
+    k, v = flat_tail(keys, heads * 64)
+    q = torch.zeros(requests, heads * 64, device="cuda", dtype=torch.float16)
+    q[:, ::64] = 1
+    table = torch.arange(keys // page, device="cuda", dtype=torch.int32).repeat(requests, 1)
+    op = ml2.PrefixAttention(ctx, ml2.Config(heads * 64, 0, 1, heads, heads, 0, 0), page)
+    ws = torch.empty(op.WorkspaceBytes(requests, requests, 0, keys), dtype=torch.uint8, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros(requests, heads, device="cuda")
+    op.Forward(out, q, None, None, k, v, table, ints([keys] * requests), ints(list(range(requests + 1))), ws, keys, lse, math.log(2.0))
+    check_flat_tail(out, lse, keys)
