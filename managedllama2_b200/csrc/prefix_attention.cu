@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
         // its sign goes into Q, so that the largest S is the largest score; never 0, so that -inf stays -inf
         const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);
         const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
-        const uint64_t scale2 = two(scale, scale);
+        const uint64_t scale2 = two(scale, scale), lower2 = two(kLower, kLower);
         unsigned used = 0;  // S tiles of this stream since the start
         bool dead = false;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -836,6 +836,8 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
             }
 
             const bool busy = quarter * 32 < rows;  // warps without rows only keep step
+            // Largest S so far but for kSlack - kLower, before the scale. S - m comes first: score * scale less a rounded m would be off
+            // by half a step of m, which is no weight at all or an infinite one where scores are huge.
             float m = -INFINITY;
             uint64_t sum[2] = {0, 0};
             for (int j = 0; j < ns; ++j, ++used) {
@@ -859,15 +861,14 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
 #pragma unroll
                         for (int i = 0; i < 4; ++i) top[i] = fmaxf(fmaxf(top[i], __uint_as_float(x[e + 2 * i])), __uint_as_float(x[e + 2 * i + 1]));
                     float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                    t = t == -INFINITY ? t : t * scale;
                     // both halves have their S in registers after this barrier, so P may go over it
-                    if (pair_any(pair, t - m > kSlack || m == -INFINITY)) {
+                    if (pair_any(pair, (t - m) * scale > kSlack - kLower)) {
                         s_top[s][half][row] = t;
                         named_bar_sync(pair, 64);
                         t = fmaxf(t, s_top[s][half ^ 1][row]);
-                        const bool move = t - m > kSlack || m == -INFINITY;
-                        const float to = move ? t - kLower : m, ref = to == -INFINITY ? 0.f : to, c = move ? exp2_fast(m - ref) : 1.f;
-                        m = to;
+                        const bool move = (t - m) * scale > kSlack - kLower;
+                        const float c = move ? exp2_fast((m - t) * scale) : 1.f;
+                        m = move ? t : m;
                         const uint64_t c2 = two(c, c);
                         sum[0] = fma2(sum[0], c2, 0);
                         sum[1] = fma2(sum[1], c2, 0);
@@ -891,7 +892,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                     uint32_t w[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float2 y = apart(fma2((uint64_t)x[2 * e + 1] << 32 | x[2 * e], scale2, ref2));
+                        const float2 y = apart(fma2(add2((uint64_t)x[2 * e + 1] << 32 | x[2 * e], ref2), scale2, lower2));
                         const float a = exp2_fast(y.x), b = exp2_fast(y.y);
                         sum[e & 1] = add2(sum[e & 1], two(a, b));
                         w[e] = pack2<T>(a, b);
@@ -918,7 +919,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                 const float2 l2 = apart(add2(sum[0], sum[1]));
                 if (half) s_top[s][1][row] = l2.x + l2.y;
                 named_bar_sync(pair, 64);
-                if (!half && row < rows && !dead) p.pre_ml[results_at + at_row] = make_float2(m, l2.x + l2.y + s_top[s][1][row]);
+                if (!half && row < rows && !dead) p.pre_ml[results_at + at_row] = make_float2(m * scale - kLower, l2.x + l2.y + s_top[s][1][row]);
                 named_bar_sync(pair, 64);
                 if (ns) {
                     // through this warp's own 16 rows of the Q tile (others may have the next segment's rows in theirs), 16 dims

@@ -81,3 +81,24 @@ def test_attention_long_flat_tail_in_own_pages(ctx):
     out, lse = torch.zeros_like(q), torch.zeros(requests, heads, device="cuda")
     op.Forward(out, q, None, None, k, v, table, ints([keys] * requests), ints(list(range(requests + 1))), ws, keys, lse, math.log(2.0))
     check_flat_tail(out, lse, keys)
+
+
+# ---- scores so large that neighbouring 32-bit numbers are far apart ------------------------------------------------------------
+@pytest.mark.parametrize("prefix", [300, 1500])
+@pytest.mark.parametrize("rows", [1, 3, 70, 200])
+@pytest.mark.parametrize("dtype,size,scale", [("fp16", 60000.0, 1.0), ("fp16", 60000.0, None), ("fp16", 60000.0, -1.0), ("bf16", 1e18, 1.0), ("bf16", 1e18, -0.37),
+                                              ("fp16", 2000.0, 1.0), ("fp16", 300.0, 0.7)])
+def test_attention_huge_scores_give_the_key_that_has_the_largest(ctx, dtype, size, scale, rows, prefix):
+    """The largest score is twice the next: its key has weight 1 and the others none, whichever tile they lie in."""
+    b = Batch(29, dtype, 4, 2, 64, 16, prefix, [20] * rows, [1] * rows)
+    b.q[:] = size
+    sign = -1.0 if scale is not None and scale < 0 else 1.0
+    b.pk[:] = (torch.rand(prefix, 1, device="cuda") * 0.45 * size * sign).to(b.t)
+    b.pk[prefix // 2] = size * sign
+    b.k[torch.cat(b.rows)] = sign * size / 2
+    out, z = b.call(ctx, scale=scale)
+    want = b.pv[prefix // 2].reshape(2, 1, 64).expand(2, 2, 64).reshape(1, -1)
+    assert torch.equal(out, want.expand_as(out))
+    # 64 products, then the scale: half a step each, and a step at the reference point
+    score = 64 * float(torch.tensor(size, dtype=b.t)) ** 2 * (64 ** -0.5 if scale is None else abs(scale))
+    assert ((z.double() - score).abs().max() <= 80 * 2.0 ** -24 * score).item()
