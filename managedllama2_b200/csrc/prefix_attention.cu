@@ -102,6 +102,14 @@ __device__ __forceinline__ float exp2_fast(float x)
     return y;
 }
 
+// 0x8000 for either of two 16-bit values that is infinite or NaN: an exponent of ones carries over
+template <typename T> __device__ __forceinline__ uint32_t not_finite(uint32_t w)
+{
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    return ((w & (kHalf ? 0x7c007c00u : 0x7f807f80u)) + (kHalf ? 0x04000400u : 0x00800080u)) & 0x80008000u;
+}
+template <typename T> __device__ __forceinline__ uint32_t times_zero(uint32_t w) { return (not_finite<T>(w) >> 15) * 0x7fffu; }  // 0 or NaN
+
 // Rows of a request that has `count` queries (or of the prefix, which all see), counted 16 at a time.
 __device__ __forceinline__ int row_tiles(const AttnBatch& p, int count) { return (count * p.group + 15) >> 4; }
 // Key tiles that the 16 rows from row0 on look at: as many as the last of them sees.
@@ -439,7 +447,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
             if (causal) {
                 // Weight 0 times a value that is not finite would be NaN in the rows that do not see its key. Such keys are
                 // taken out of the product and added to the rows that see them one by one.
-                constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u, kOne = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
                 unsigned odd = 0;
                 for (int i = 0; i < kChunks / 2; ++i) {
                     const int at = i * 32 + lane;  // 16 bytes of key at / kChunks
@@ -447,7 +454,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
                     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(vt + at * 16) : "memory");
                     bool bad = false;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) bad |= (((v[e] & kExp) + kOne) & 0x80008000u) != 0;  // an exponent of ones carries over
+                    for (int e = 0; e < 4; ++e) bad |= not_finite<T>(v[e]) != 0;
                     if (bad) odd |= 1u << (at / kChunks);
                 }
                 odd = __reduce_or_sync(0xffffffffu, odd);
@@ -790,8 +797,8 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
         const int s = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane, pair = 1 + s * 4 + quarter;
         const uint32_t lanes = (uint32_t)quarter << 21, t_o = tmem + 256 + s * 128 + half * (kHead / 2) + lanes;
         const uint32_t q_tile = q_base + s * S::kQBytes;
-        // its sign goes into Q, so that the largest S is the largest score; never 0, so that -inf stays -inf
-        const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);
+        // its sign goes into Q, so that the largest S is the largest score; so does a scale of 0 (masked keys have -inf to keep)
+        const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
         const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
         const uint64_t scale2 = two(scale, scale), lower2 = two(kLower, kLower);
         unsigned used = 0;  // S tiles of this stream since the start
@@ -821,6 +828,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                     const long long at = __shfl_sync(0xffffffffu, q_at, r);
                     v[i] = make_uint4(0, 0, 0, 0);
                     if (quarter * 32 + r < rows) v[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + at + c * 8);
+                    if (p.scale_log2 == 0.f) v[i] = make_uint4(times_zero<T>(v[i].x), times_zero<T>(v[i].y), times_zero<T>(v[i].z), times_zero<T>(v[i].w));
                 }
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {

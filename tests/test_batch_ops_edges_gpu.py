@@ -102,3 +102,28 @@ def test_attention_huge_scores_give_the_key_that_has_the_largest(ctx, dtype, siz
     # 64 products, then the scale: half a step each, and a step at the reference point
     score = 64 * float(torch.tensor(size, dtype=b.t)) ** 2 * (64 ** -0.5 if scale is None else abs(scale))
     assert ((z.double() - score).abs().max() <= 80 * 2.0 ** -24 * score).item()
+
+
+# ---- scales next to zero -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("prefix", [300, 1500])  # by runs, by blocks
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-39, -1e-39])
+def test_attention_scale_of_zero_and_below_the_normal_numbers(ctx, prefix, scale):
+    """Products of size 10^37: a scale of zero makes every weight the same, one of 10^-39 nearly so."""
+    b = Batch(13, "bf16", 2, 1, 64, 16, prefix, [20] * 70, [1] * 70, sigma=1.0)
+    b.q[:] = (torch.sign(b.q) * 1e18).to(b.t)
+    b.pk[:] = (torch.sign(b.pk) * 5e17).to(b.t)
+    b.k[torch.cat(b.rows)] = (torch.sign(b.k[torch.cat(b.rows)]) * 5e17).to(b.t)
+    b.check(ctx, scale=scale)
+
+
+@pytest.mark.parametrize("prefix", [300, 1500])
+def test_attention_scale_of_zero_times_infinity_is_nan(ctx, prefix):
+    b = Batch(13, "bf16", 2, 2, 64, 16, prefix, [20] * 70, [1] * 70)
+    b.q[:, 0] = 1.0
+    b.pk[3, 0] = float("-inf")
+    b.q[5, 70], b.q[6, 127] = float("inf"), float("nan")
+    out, z = b.call(ctx, scale=0.0)
+    assert bool(out[:, :64].isnan().all()) and bool(z[:, 0].isnan().all())
+    fine = torch.ones(70, dtype=torch.bool, device="cuda")
+    fine[5:7] = False
+    assert bool(out[fine, 64:].isfinite().all()) and bool(out[5:7].isnan().all()) and bool(z[5:7].isnan().all())
