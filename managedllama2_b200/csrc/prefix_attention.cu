@@ -1240,7 +1240,8 @@ int ml2_prefix_attention(ml2_ctx* h, const ml2_prefix_attention_args* args)
         return fail(ML2_E_INVALID, "prefix_attention: table_stride=%d with page_size=%d", table_stride, page_size);
     if (max_length > table_stride * page_size)
         return fail(ML2_E_INVALID, "prefix_attention: max_length=%d passes the table's %d pages of %d", max_length, table_stride, page_size);
-    if (!std::isfinite(scale)) return fail(ML2_E_INVALID, "prefix_attention: scale=%g", (double)scale);
+    constexpr float kLog2e = 1.44269504088896340736f;
+    if (!std::isfinite(scale * kLog2e)) return fail(ML2_E_INVALID, "prefix_attention: scale=%g", (double)scale);
     if (n_rows == 0) return ML2_OK;
     if (!out || !query || !table || !lengths || !query_start || !key_cache || !value_cache || (prefix_length && (!prefix_key || !prefix_value)))
         return fail(ML2_E_INVALID, "prefix_attention: null argument");
@@ -1264,7 +1265,7 @@ int ml2_prefix_attention(ml2_ctx* h, const ml2_prefix_attention_args* args)
     p.out_stride = out_stride; p.q_stride = query_stride; p.prefix_stride = prefix_stride; p.cache_stride = cache_stride;
     p.n_requests = n_requests; p.n_rows = n_rows; p.prefix = prefix_length; p.max_length = max_length; p.n_pages = (int)(cache_rows >> shift);
     p.table_stride = table_stride; p.page_shift = shift; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.group = n_heads / n_kv_heads;
-    p.scale_log2 = scale * 1.44269504088896340736f;
+    p.scale_log2 = scale * kLog2e;
     char* ws = static_cast<char*>(workspace);
     p.pre_o = reinterpret_cast<float*>(ws); p.run_o = reinterpret_cast<float*>(ws + pl.run_o);
     p.pre_ml = reinterpret_cast<float2*>(ws + pl.pre_ml); p.run_ml = reinterpret_cast<float2*>(ws + pl.run_ml);
