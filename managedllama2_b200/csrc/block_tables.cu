@@ -6,7 +6,8 @@
 //   pops    every request that grows takes pages(new) - pages(old) pages off the top,
 //   tokens  token old[r] + j of a growing request gets row start[r] + j of the slot map.
 // One CTA does the sums in shared memory, then the lists, cut evenly over its threads, each element finding its request by
-// bisection of the sums. What bounds it is latency: loads of the lengths, the scan's barriers, dependent loads and the store.
+// bisection of the sums. A page number that is none of the cache's is reported where it is met; it stays off the free stack,
+// and the table that would have it gets -1. What bounds it is latency: loads of the lengths, the scan's barriers, dependent loads and the store.
 // Where the tokens are many (a step that brings prompts), a second kernel of many CTAs writes the slot map from the finished
 // table: 186000 tokens of 512 requests take 14.7 us, 13 of them the first kernel's; one CTA alone took 150. 64 requests that grow
 // by one token take 3.6 us.
@@ -127,12 +128,7 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Tabl
         if (threadIdx.x == 0) report_input_error(p.status, kInputFreeCount, count);
         count = min(max(count, 0), p.n_pages);
     }
-    if (total.back > p.n_pages - count && threadIdx.x == 0) report_input_error(p.status, kInputFreeOverflow, total.back);
-    const int have = min(count + min(total.back, p.n_pages - count), p.n_pages);
-    const bool all_fit = total.tokens <= p.max_tokens && total.need <= have;
-
-    // Exclusive sums of what is served. The usual case takes them from the scan above; when something does not fit, the
-    // two cuts (tokens first, then pages among the rest) each move the sums behind them, so they are scanned again.
+    const int threads = (int)blockDim.x, me = (int)threadIdx.x, room = p.n_pages - count;
     {
         int push = before.back;
         for (int r = r0; r < r1; ++r) {
@@ -141,6 +137,43 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Tabl
             push += change(r).back;
         }
     }
+    if (total.back) {
+        __syncthreads();
+        bool broken = false;
+        for (unsigned x = me; x < (unsigned)total.back; x += threads) {
+            const int r = bisect(s_push, p.n, x), id = p.table[(size_t)r * p.width + pages(p.new_lengths[r]) + (x - s_push[r])];
+            if (id < 0 || id >= p.n_pages) {
+                report_input_error(p.status, kInputPage, r);
+                broken = true;
+            } else if ((int)x < room) {
+                p.free_pages[count + x] = id;
+            }
+        }
+        // pages that are none stay off the stack: the others move together, each thread those of its requests
+        if (__syncthreads_or(broken)) {
+            auto given = [&](auto&& f) {
+                for (int r = r0; r < r1; ++r)
+                    for (int left = change(r).back, i = pages(p.new_lengths[r]); left > 0; --left, ++i) {
+                        const int id = p.table[(size_t)r * p.width + i];
+                        if (id >= 0 && id < p.n_pages) f(id);
+                    }
+            };
+            Sums part{0, 0, 0}, sound;
+            given([&](int) { ++part.back; });
+            int at = block_scan(part, s_scan, &sound).back;
+            given([&](int id) {
+                if (at < room) p.free_pages[count + at] = id;
+                ++at;
+            });
+            total.back = sound.back;
+        }
+    }
+    if (total.back > room && threadIdx.x == 0) report_input_error(p.status, kInputFreeOverflow, total.back);
+    const int have = count + min(total.back, room);
+    const bool all_fit = total.tokens <= p.max_tokens && total.need <= have;
+
+    // Exclusive sums of what is served. The usual case takes them from the scan above; when something does not fit, the
+    // two cuts (tokens first, then pages among the rest) each move the sums behind them, so they are scanned again.
     if (all_fit) {
         for (int r = r0; r < r1; ++r) {
             const Sums v = change(r);
@@ -195,22 +228,20 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(const Tabl
     if (threadIdx.x == 0) {
         s_start[p.n] = (int)total.tokens;
         s_pop[p.n] = total.need;
-        s_push[p.n] = have - count;
-    }
-    __syncthreads();
-
-    const int threads = (int)blockDim.x, me = (int)threadIdx.x;
-    const int n_push = have - count, n_pop = total.need, n_tokens = (int)total.tokens;
-    for (int x = me; x < n_push; x += threads) {
-        const int r = bisect(s_push, p.n, x);
-        p.free_pages[count + x] = p.table[(size_t)r * p.width + pages(p.new_lengths[r]) + (x - s_push[r])];
     }
     // Pages given back are taken again below, and the lengths may be written over the ones read above: everybody is done
     // reading and pushing first.
     __syncthreads();
-    for (int x = me; x < n_pop; x += threads) {
+
+    const int n_pop = total.need, n_tokens = (int)total.tokens;
+    for (unsigned x = me; x < (unsigned)n_pop; x += threads) {
         const int r = bisect(s_pop, p.n, x);
-        p.table[(size_t)r * p.width + pages(s_old[r]) + (x - s_pop[r])] = p.free_pages[have - 1 - x];
+        int id = p.free_pages[have - 1 - x];
+        if (id < 0 || id >= p.n_pages) {
+            report_input_error(p.status, kInputPage, r);
+            id = -1;
+        }
+        p.table[(size_t)r * p.width + pages(s_old[r]) + (x - s_pop[r])] = id;
     }
     for (int t = me; t < p.fill; t += threads) {
         int slot = -1, position = 0;

@@ -127,3 +127,64 @@ def test_attention_scale_of_zero_times_infinity_is_nan(ctx, prefix):
     fine = torch.ones(70, dtype=torch.bool, device="cuda")
     fine[5:7] = False
     assert bool(out[fine, 64:].isfinite().all()) and bool(out[5:7].isnan().all()) and bool(z[5:7].isnan().all())
+
+
+# ---- block tables: pages that are none -----------------------------------------------------------------------------------------
+def step_with(ctx, table, free, old, new, page=4, rows=16):
+    op, n = ml2.BlockTables(ctx, page), len(old)
+    got = dict(table=ints(table), free=ints(free), count=ints([sum(x != -9 for x in free)]), lengths=ints(old), start=ints([0] * (n + 1)),
+               slots=ints([7] * rows), positions=ints([7] * rows), refused=ints([7] * n))
+    op.Forward(got["lengths"], ints(new), got["table"], got["free"], got["count"], got["lengths"], got["count"], got["start"], got["slots"],
+               got["positions"], got["refused"])
+    return {k: v.tolist() for k, v in got.items()}
+
+
+@pytest.mark.parametrize("bad", [-1, 8, 2**31 - 1, -2**31])
+def test_block_tables_pages_given_back_that_are_none_stay_off_the_stack(ctx, bad):
+    """Request 1 gives back three pages, the middle one of which is none; request 0 takes what is free, in order."""
+    got = step_with(ctx, [[0, -1, -1], [1, bad, 2], [3, 4, -1]], [5] + [-9] * 7, [4, 12, 8], [12, 0, 4])
+    with pytest.raises(ml2.Ml2Error, match="page of request 1"):
+        ctx.status()
+    # pushed on 5: 1 and 2 of request 1, 4 of request 2; taken: 4, then 2
+    assert got["free"][:4] == [5, 1, 2, 4] and got["count"] == [2]
+    assert got["table"][0] == [0, 4, 2] and got["lengths"] == [12, 0, 4] and got["refused"] == [0, 0, 0]
+    assert got["slots"][:8] == [16, 17, 18, 19, 8, 9, 10, 11] and got["slots"][8:] == [-1] * 8
+
+
+def test_block_tables_pages_that_are_none_do_not_count_as_free(ctx):
+    """Two of three pages given back are none: the one that is left serves request 0 alone."""
+    got = step_with(ctx, [[0, -1], [1, -1], [-1, 9]], [-9] * 8, [4, 4, 8], [5, 5, 0])
+    with pytest.raises(ml2.Ml2Error, match="page of request 2"):
+        ctx.status()
+    assert got["refused"] == [2, 2, 0] and got["count"] == [0] and got["slots"] == [-1] * 16 and got["lengths"] == [4, 4, 0]
+    got = step_with(ctx, [[0, -1], [1, -1], [-1, 6]], [-9] * 8, [4, 4, 8], [5, 5, 0])
+    with pytest.raises(ml2.Ml2Error, match="page of request 2"):
+        ctx.status()
+    assert got["refused"] == [0, 2, 0] and got["count"] == [0] and got["slots"][:2] == [24, -1] and got["table"][0] == [0, 6]
+
+
+def test_block_tables_pages_taken_that_are_none_are_entered_as_none(ctx):
+    got = step_with(ctx, [[0, -1], [1, -1]], [2, 8] + [-9] * 6, [4, 4], [6, 5])
+    with pytest.raises(ml2.Ml2Error, match="page of request 0"):
+        ctx.status()
+    assert got["table"] == [[0, -1], [1, 2]] and got["slots"][:3] == [-1, -1, 8] and got["count"] == [0]
+
+
+@pytest.mark.parametrize("n", [1, 40, 1500])
+def test_block_tables_many_broken_pages(ctx, n):
+    """Every other page of requests that end is none; the rest lies on the stack in order of request and page."""
+    rng = random.Random(n)
+    width, page = 5, 4
+    ids = list(range(n * width))
+    rng.shuffle(ids)
+    table = [[ids.pop() if (r + i) % 2 else -1 - i for i in range(width)] for r in range(n)]
+    old, new = [width * page] * n, [rng.randint(0, width * page) for _ in range(n)]
+    free = [-9] * (n * width)
+    got = step_with(ctx, table, free, old, new, page)
+    want = [table[r][i] for r in range(n) for i in range(-(-new[r] // page), width) if (r + i) % 2]
+    broken = any((r + i) % 2 == 0 for r in range(n) for i in range(-(-new[r] // page), width))
+    assert broken == (n > 1 or new[0] <= 16)
+    if broken:
+        with pytest.raises(ml2.Ml2Error, match="page of request"):
+            ctx.status()
+    assert got["free"][:len(want)] == want and got["count"] == [len(want)] and got["lengths"] == new
