@@ -345,7 +345,8 @@ extern "C" int ml2_block_tables(ml2_ctx* h, const ml2_block_tables_args* args)
     cfg.attrs = attr;
     cfg.numAttrs = ctx->pdl ? 1 : 0;
     cudaError_t e = cudaSuccess;
-    if (cfg.dynamicSmemBytes > 48 * 1024)
+    // 48 KB of a block without this, the kernel's static shared memory among them
+    if (cfg.dynamicSmemBytes + sizeof(Sums) * 33 > 48 * 1024)
         e = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((4 * kMaxRequests + 3) * sizeof(int)));
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, block_tables_kernel, p);
     if (e == cudaSuccess) {

@@ -188,3 +188,25 @@ def test_block_tables_many_broken_pages(ctx, n):
         with pytest.raises(ml2.Ml2Error, match="page of request"):
             ctx.status()
     assert got["free"][:len(want)] == want and got["count"] == [len(want)] and got["lengths"] == new
+
+
+# ---- block tables: request counts around the launch's limit of shared memory ---------------------------------------------------
+def tables_of_many_requests():
+    c = ml2.CudaContext(0)
+    for n in (3030, 3038, 3039, 3055, 3071, 3100):
+        plain, dev = base.tables_setup(random.Random(n), n, 16, 2, 2 * n + 5)
+        new = [min(x + 1, 32) for x in plain.old]
+        base.tables_step(c, plain, dev, new, n, 0)
+    assert c.status() == (0, 0)
+    c.close()
+
+
+def test_block_tables_around_the_default_shared_memory_of_a_launch():
+    """In a process of its own: a larger call made before would have raised the limit."""
+    code = "import sys; sys.path[:0] = %r; import test_batch_ops_edges_gpu as t; t.tables_of_many_requests()" % ([os.path.dirname(__file__), base_root()],)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def base_root():
+    return os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
