@@ -62,7 +62,8 @@ class Arguments:
             names = names.split()
             self.names += names
             self.kinds += kind * len(names)
-        self.pack = struct.Struct("@" + self.kinds.replace("p", "P").replace("l", "q")).pack
+        # 0P: the end is padded to a pointer's alignment, as the struct's is
+        self.pack = struct.Struct("@" + self.kinds.replace("p", "P").replace("l", "q") + "0P").pack
 
     def entry(self, function):
         function.argtypes = [ctypes.c_void_p, ctypes.c_char_p]

@@ -1,4 +1,6 @@
 """Edges of the batched-decoding operators' arguments, without a GPU."""
+import ctypes
+
 import pytest
 
 from managedllama2_b200 import _lib
@@ -9,3 +11,16 @@ from test_batch_ops_cpu import ATTN, call, calls, refused  # noqa: F401  (calls 
 def test_prefix_attention_refuses_a_scale_that_overflows_in_powers_of_two(calls, scale):  # noqa: F811
     lib, ctx, _ = calls
     refused(lib, call(lib.ml2_prefix_attention, _lib.PREFIX_ATTENTION, dict(ATTN, ctx=ctx, scale=scale)), "scale")
+
+
+@pytest.mark.parametrize("name,arguments", [("ml2_block_tables_args", _lib.BLOCK_TABLES), ("ml2_qk_norm_rope_args", _lib.QK_NORM_ROPE),
+                                            ("ml2_prefix_attention_args", _lib.PREFIX_ATTENTION)])
+def test_packed_arguments_are_as_long_as_the_struct(name, arguments):
+    """The library copies the whole struct, the bytes behind its last member among them."""
+    kinds = {"p": ctypes.c_void_p, "l": ctypes.c_longlong, "i": ctypes.c_int, "f": ctypes.c_float}
+    layout = type(name, (ctypes.Structure,), {"_fields_": [(n, kinds[k]) for n, k in zip(arguments.names, arguments.kinds)]})
+    values = range(1, len(arguments.names) + 1)
+    packed = arguments.pack(*values)
+    assert len(packed) == ctypes.sizeof(layout)
+    got = layout.from_buffer_copy(packed)
+    assert [getattr(got, n) for n in arguments.names] == list(values)
