@@ -27,7 +27,9 @@ struct AttnBatch {
     // and an o that is not read. pre: of the prefix by blocks, [segments][rows that are there][n_heads]; run: of the warps' runs.
     float *pre_o, *run_o;
     float2 *pre_ml, *run_ml;
-    int* run_base;      // [n_requests + 1]: places before request r, of all requests; then the places of a run
+    int* run_base;      // [n_requests + 1]: places before request r, of all requests; then the places of a run, negative where
+                        // the requests have more than own_places
+    int own_places;     // of all requests at most, whose query rows do not overlap
     long long wait_cycles;
     long long out_stride, q_stride, prefix_stride, cache_stride;
     int n_requests, n_rows, prefix, max_length, n_pages, table_stride, page_shift, n_heads, n_kv, group;
@@ -120,7 +122,7 @@ __device__ __forceinline__ int tiles_seen(const AttnBatch& p, int count, int len
 }
 // A request's share of the runs: `seqs` row tiles for each key head, the first of which sees `low` key tiles and the last `high`.
 // Places before row tile rt, for one key head: kOpen and the key tiles of each row tile, the latter taken to grow evenly from low
-// to high and, where they grow, two more, which covers every row tile (checked for heads of a group from 1 to 32; 7 % more
+// to high and, where they grow, two more, which covers every row tile (checked for groups of up to 65536 heads; 7 % more
 // places than are needed, where `high` for all would be 70 % more).
 struct Share {
     int seqs, low, high;
@@ -144,6 +146,9 @@ __device__ __forceinline__ long long result_row(const AttnBatch& p, bool prefix,
 {
     return (prefix ? (long long)p.n_rows * p.n_heads : 0) + ((long long)first * p.group + row0) * p.n_kv + kvh * rows + 16ll * run;
 }
+
+// a + b of numbers that are not negative, 2^31 - 1 at most
+__device__ __forceinline__ int add_up_to(int a, int b) { return (int)min((unsigned)a + (unsigned)b, 0x7fffffffu); }
 
 // A walk over one run: 16 rows of one key head and request (a sequence), kOpen places for its beginning and one for each of its
 // key tiles, then the next sequence.
@@ -249,6 +254,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
     if (!p.prefix_ctas) pdl_wait();
     pdl_launch_dependents();  // every block is resident by the time the join's come, which look up their rows meanwhile
     const int total_rows = min(max(p.query_start[p.n_requests], 0), p.n_rows);
+    bool too_many;
     int longest = kOpen + (p.prefix_ctas ? 0 : (p.prefix + kTile - 1) / kTile);
     // ---- how many places every request has -----------------------------------------------------------------------------
     {
@@ -259,29 +265,35 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
             if (!s.good && blockIdx.x == 0) report_input_error(p.status, kInputLength, r);
             s_base[r] = mine;
             const Share share = request_share(p, s.count, s.length);
-            mine += places_before(share, share.seqs) * p.n_kv;
+            mine = add_up_to(mine, places_before(share, share.seqs) * p.n_kv);
             longest = max(longest, kOpen + share.high);
         }
+        // Rows that several requests lay claim to (query rows out of order, reported above) count for each of them: their sum may pass
+        // what the host saw fits, and 32 bits. Nobody has own tokens then.
         int incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
+            if (lane >= o) incl = add_up_to(incl, v);
         }
+        int before = __shfl_up_sync(0xffffffffu, incl, 1);
+        if (lane == 0) before = 0;
         longest = __reduce_max_sync(0xffffffffu, longest);
         if (lane == 31) {
             s_sum[warp] = incl;
             s_long[warp] = longest;
         }
         __syncthreads();
-        int base = incl - mine, all = 0;
+        int base = before, all = 0;
 #pragma unroll
         for (int w = 0; w < kAttnWarps; ++w) {
-            if (w < warp) base += s_sum[w];
-            all += s_sum[w];
+            if (w < warp) base = add_up_to(base, s_sum[w]);
+            all = add_up_to(all, s_sum[w]);
             longest = max(longest, s_long[w]);
         }
-        for (int r = r0; r < r1; ++r) s_base[r] += base;
+        too_many = all > p.own_places;
+        if (too_many) all = 0;
+        for (int r = r0; r < r1; ++r) s_base[r] = too_many ? 0 : s_base[r] + base;
         if (threadIdx.x == 0) {
             s_base[p.n_requests] = all;
             s_base[p.n_requests + 1] = all + (p.prefix_ctas || !p.prefix ? 0 : row_tiles(p, total_rows) * p.n_kv * (kOpen + (p.prefix + kTile - 1) / kTile));
@@ -291,7 +303,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
     const int all = s_base[p.n_requests + 1], per = max(shortest_run(longest), (all + (int)gridDim.x * kAttnWarps - 1) / ((int)gridDim.x * kAttnWarps)), run = blockIdx.x * kAttnWarps + warp;
     if (blockIdx.x == 0) {  // the join finds the results by these
         for (int r = threadIdx.x; r <= p.n_requests; r += kAttnThreads) p.run_base[r] = s_base[r];
-        if (threadIdx.x == 0) p.run_base[p.n_requests + 1] = per;
+        if (threadIdx.x == 0) p.run_base[p.n_requests + 1] = too_many ? -per : per;
     }
 
     unsigned char* ring = s_mem + warp * kStages * 2 * kTileBytes;
@@ -999,15 +1011,17 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
         }
         const Span s = request_span(p, lo);
         if (!s.good && lane == 0) report_input_error(p.status, kInputLength, lo);
-        const bool own = p.run_ctas && s.good && t >= s.first && t < s.first + s.count;
+        bool own = p.run_ctas && s.good && t >= s.first && t < s.first + s.count;
         pdl_wait();
         if (lane == 0) {
+            const int per = p.run_ctas ? p.run_base[p.n_requests + 1] : 1;
+            own = own && per > 0;
             s_row[0] = s.first;
             s_row[1] = s.count;
             s_row[2] = own ? s.length : 0;
             s_row[3] = own ? p.run_base[lo] : 0;
             s_row[4] = p.run_ctas ? p.run_base[p.n_requests] : 0;
-            s_row[5] = p.run_ctas ? max(p.run_base[p.n_requests + 1], 1) : 1;
+            s_row[5] = max(abs(per), 1);
         }
     }
     pdl_wait();  // the results, from here on
@@ -1107,6 +1121,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
 struct AttnPlan {
     int prefix_ctas, run_ctas;
     long long tiles;   // key tiles of either kernel, at most
+    long long own_places;  // of the runs, without the prefix, at most
     size_t run_o, pre_ml, run_ml, run_base, bytes;  // offsets into the workspace (pre_o comes first), and its size
 };
 static AttnPlan plan_attention(const Ctx* ctx, int n_rows, int n_requests, int prefix, int max_length, int n_heads, int n_kv, int head)
@@ -1116,6 +1131,7 @@ static AttnPlan plan_attention(const Ctx* ctx, int n_rows, int n_requests, int p
     const int sms = std::max(1, ctx->sm_count);
     const long long rows = (long long)n_rows * (n_heads / n_kv);  // of a key head
     long long pre_rows = 0, run_rows = 0, run_tiles = (n_requests + rows / 16) * n_kv * (max_length ? kOpen + ceil_div(max_length, kTile) + 3 : 0);
+    pl.own_places = run_tiles;
     if (prefix >= (rows <= 16 ? kBlockPrefixFewRows : kBlockPrefix)) {
         const long long blocks = (rows + kBlockRows - 1) / kBlockRows, key_tiles = ceil_div(prefix, kKeyTile);
         pl.tiles = blocks * n_kv * key_tiles;
@@ -1270,7 +1286,7 @@ int ml2_prefix_attention(ml2_ctx* h, const ml2_prefix_attention_args* args)
     p.pre_o = reinterpret_cast<float*>(ws); p.run_o = reinterpret_cast<float*>(ws + pl.run_o);
     p.pre_ml = reinterpret_cast<float2*>(ws + pl.pre_ml); p.run_ml = reinterpret_cast<float2*>(ws + pl.run_ml);
     p.run_base = reinterpret_cast<int*>(ws + pl.run_base);
-    p.prefix_ctas = pl.prefix_ctas; p.run_ctas = pl.run_ctas;
+    p.prefix_ctas = pl.prefix_ctas; p.run_ctas = pl.run_ctas; p.own_places = (int)pl.own_places;
     p.waits = ctx->status_dev; p.wait_cycles = ctx->wait_cycles;
     PrefixMaps maps{};
     if (pl.prefix_ctas && (!make_map(&maps.k, dtype, prefix_key, prefix_stride, (int)kv_width, p.prefix) ||

@@ -210,3 +210,95 @@ def test_block_tables_around_the_default_shared_memory_of_a_launch():
 
 def base_root():
     return os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+# ---- memory that a call leaves alone -------------------------------------------------------------------------------------------
+def guarded(shape, fill, dtype, before=64, behind=4096):
+    """A tensor in the middle of a buffer that holds `fill` everywhere, and a check of what lies around it."""
+    n = math.prod(shape)
+    buffer = torch.full((before + n + behind,), fill, dtype=dtype, device="cuda")
+
+    def untouched():
+        return bool((buffer[:before] == fill).all()) and bool((buffer[before + n:] == fill).all())
+    return buffer[before:before + n].view(shape), untouched
+
+
+def guarded_call(ctx, b, scale=None, max_length=None):
+    """A call whose workspace ends where it has to; nothing behind or before any output changes."""
+    op = ml2.PrefixAttention(ctx, b.cfg, b.page)
+    rows, most, width = b.q.shape[0], max(b.own) if max_length is None else max_length, b.heads * b.head
+    need = op.WorkspaceBytes(rows, len(b.own), b.prefix, most)
+    ws, ws_fine = guarded((need,), 0xA5, torch.uint8, behind=1 << 20)
+    wide, out_fine = guarded((rows, width + 16), 7.0, b.t)
+    z, z_fine = guarded((rows, b.heads), 7.0, torch.float32)
+    op.Forward(wide[:, :width], b.q, b.pk, b.pv, b.k, b.v, b.table, b.lengths, b.start, ws, most, z, scale)
+    assert ws_fine(), "written outside the workspace"
+    assert out_fine() and bool((wide[:, width:] == 7.0).all()), "written outside the output"
+    assert z_fine(), "written outside the log sums"
+    return wide[:, :width], z
+
+
+@pytest.mark.parametrize("heads,kv,head,prefix,requests,length,queries", [
+    (1, 1, 64, 0, 1, 1, 1), (1, 1, 128, 5000, 1, 30, 1), (40, 40, 128, 4096, 1, 64, 1), (40, 40, 64, 1024, 17, 30, 1), (3, 1, 64, 1025, 129, 7, 1),
+    (64, 1, 128, 1100, 3, 40, 2), (71, 1, 64, 1500, 5, 90, 20), (71, 1, 64, 300, 5, 90, 20), (200, 2, 64, 100, 2, 40, 9), (5, 5, 128, 0, 300, 20, 3),
+    (8, 8, 64, 2000, 4, 700, 300), (8, 2, 128, 1600, 33, 60, 30), (148, 148, 64, 1024, 1, 1, 1), (1, 1, 64, 40000, 130, 3, 1), (12, 3, 64, 1, 1000, 4, 4)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_attention_writes_nothing_around_its_outputs_and_workspace(ctx, heads, kv, head, prefix, requests, length, queries, dtype):
+    b = Batch(prefix + heads, dtype, heads, kv, head, 16, prefix, *base.ragged(heads + requests, requests, length, queries), extra_rows=3)
+    out, z = guarded_call(ctx, b)
+    want, lse, tol, tol_lse = b.want()
+    total = sum(b.count)
+    assert bool(((out[:total].double() - want).abs() <= tol).all()) and bool(((z[:total].double() - lse).abs() <= tol_lse).all())
+    assert bool((out[total:] == 7.0).all()) and bool((z[total:] == 7.0).all())
+    # fewer query rows than the call has room for, as a replayed graph may meet them
+    for k in (0, requests // 2):
+        b.start[k + 1:] = b.start[k].item()
+        out, z = guarded_call(ctx, b)
+        rows = int(b.start[k])
+        assert bool(((out[:rows].double() - want[:rows]).abs() <= tol[:rows]).all()) and bool((out[rows:] == 7.0).all()) and bool((z[rows:] == 7.0).all())
+
+
+@pytest.mark.parametrize("prefix", [0, 30, 1200])
+@pytest.mark.parametrize("start", [[0, 3, 1, 2], [1, 1, 2, 3], [5, 6, 7, 8], [0, 1, 2, 2**31 - 1], [-5, 0, 1, 2], [0, -1, -2, -3], [0, 3, 0, 3],
+                                   [0, 2, 2, -2**31]])
+def test_attention_query_rows_out_of_order_write_nothing_around(ctx, start, prefix):
+    b = Batch(4, "fp16", 4, 2, 64, 16, prefix, [40, 40, 3], [1, 1, 1])
+    b.start = ints(start)
+    guarded_call(ctx, b)
+    with pytest.raises(ml2.Ml2Error, match="length or the query rows of request"):
+        ctx.status()
+
+
+def test_attention_rows_claimed_by_many_requests_have_the_prefix_alone(ctx):
+    """Every other request claims all 2048 rows, with 2^22 own tokens each: 2^32 tiles in all, where a call that is in order has
+    2^27 at most. Nobody has own tokens then, and the call is reported."""
+    requests, rows, page, prefix = 128, 2048, 1024, 30
+    b = Batch(5, "fp16", 2, 2, 64, page, prefix, [1] * requests, [rows // requests] * requests)
+    alone = Batch(5, "fp16", 2, 2, 64, page, prefix, [0] * requests, [rows // requests] * requests)
+    alone.q, alone.pk, alone.pv = b.q, b.pk, b.pv
+    want, lse, tol, tol_lse = alone.want()
+    b.table = torch.zeros(requests, 4096, dtype=torch.int32, device="cuda")
+    b.lengths = ints([4096 * page] * requests)
+    b.start = ints([0, rows] * (requests // 2) + [rows])
+    out, z = guarded_call(ctx, b, max_length=4096 * page)
+    with pytest.raises(ml2.Ml2Error, match="length or the query rows of request"):
+        ctx.status()
+    assert bool(((out.double() - want).abs() <= tol).all()) and bool(((z.double() - lse).abs() <= tol_lse).all())
+
+
+def test_tables_write_nothing_around_their_arrays(ctx):
+    rng = random.Random(3)
+    for n, page, width, rows in ((1, 16, 3, 1), (7, 4, 5, 60), (300, 16, 4, 1500), (1100, 8, 6, 9000), (40, 2, 700, 20000)):
+        plain, dev = base.tables_setup(rng, n, page, width, n * width + 3)
+        new = [rng.randint(0, width * page) for _ in range(n)]
+        arrays = {k: guarded(v.shape, 77, torch.int32) for k, v in dev.items()}
+        for k, v in dev.items():
+            arrays[k][0].copy_(v)
+        for k, m in (("start", n + 1), ("slots", rows), ("positions", rows), ("refused", n)):
+            arrays[k] = guarded((m,), 77, torch.int32)
+        a = {k: v[0] for k, v in arrays.items()}
+        ml2.BlockTables(ctx, page).Forward(a["lengths"], ints(new), a["table"], a["free"], a["count"], a["lengths"], a["count"], a["start"],
+                                           a["slots"], a["positions"], a["refused"], 5)
+        refused, start, slots, positions = plain.step(new, width, rows, 5)
+        assert a["refused"].tolist() == refused and a["start"].tolist() == start and a["slots"].tolist() == slots and a["positions"].tolist() == positions
+        assert all(v[1]() for v in arrays.values()), [k for k, v in arrays.items() if not v[1]()]
