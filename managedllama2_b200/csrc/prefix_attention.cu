@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                 ++(key ? keys : vals);
                 return true;
             };
-            const bool done = for_segments([&](int kvh, int block, int tile, int n) {
+            for_segments([&](int kvh, int block, int tile, int n) {
                 const int step = runs.rows - block * kBlockRows <= kBlockRows / 2 ? 2 : 1;
                 auto loads = [&](bool key, int j) {
                     for (int t = j * step; t < min(n, (j + 1) * step); ++t)
@@ -713,14 +713,14 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                 base += n;
                 return true;
             });
-            if (!done) {  // copies that are under way land before this CTA leaves
-                auto land = [&](uint64_t* full, unsigned n) {
-                    for (unsigned g = n > kRing ? n - kRing : 0; g < n; ++g)
-                        for (int i = 0; i < 1 << 20 && !mbar_try_wait(&full[g % kRing], g / kRing & 1); ++i) {}
-                };
-                land(b_k, keys);
-                land(b_v, vals);
-            }
+            // Copies that are under way land before this CTA leaves: not only where this thread has given up, for those who would
+            // wait for the last ones may have.
+            auto land = [&](uint64_t* full, unsigned n) {
+                for (unsigned g = n > kRing ? n - kRing : 0; g < n; ++g)
+                    for (int i = 0; i < 1 << 20 && !mbar_try_wait(&full[g % kRing], g / kRing & 1); ++i) {}
+            };
+            land(b_k, keys);
+            land(b_v, vals);
         }
         __syncwarp();
     } else if (warp >= 16) {
@@ -738,7 +738,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
             unsigned base = 0;                // first tile of the segment
             unsigned asked = 0, added = 0;    // S tiles queued since the start, and P tiles used
             unsigned turn_q = 0;              // Q tiles taken
-            const bool done = for_segments([&](int, int block, int, int n) {
+            for_segments([&](int, int block, int, int n) {
                 const bool turns = runs.rows - block * kBlockRows <= kBlockRows / 2;
                 const int step = turns ? 2 : 1;
                 // Step j's key or value tiles. Each stream looks at every tile, and lets go at once of one that is the other's: who
@@ -796,10 +796,9 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                 base += n;
                 return true;
             });
-            if (!done) {  // products that are under way end before the TMEM is given back
-                if (leader) tc_commit(&b_end[s]);
-                for (int i = 0; i < 1 << 20 && !mbar_try_wait(&b_end[s], 0); ++i) {}
-            }
+            // products that are under way end before the TMEM is given back, whoever has given up
+            if (leader) tc_commit(&b_end[s]);
+            for (int i = 0; i < 1 << 20 && !mbar_try_wait(&b_end[s], 0); ++i) {}
         }
         __syncwarp();
     } else {
