@@ -33,6 +33,25 @@ int use_device(const Ctx* ctx)
     return ML2_OK;
 }
 
+int use_callers_stream(Ctx* ctx)
+{
+    if (int rc = use_device(ctx)) return rc;
+    if (ctx->stream == ctx->caller_stream) return ML2_OK;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(ctx->caller_stream, &capture);
+    if (e == cudaSuccess && capture == cudaStreamCaptureStatusNone) {  // a capture cannot wait for what lies outside it
+        cudaEvent_t queued;
+        if ((e = cudaEventCreateWithFlags(&queued, cudaEventDisableTiming)) == cudaSuccess) {
+            e = cudaEventRecord(queued, ctx->stream);
+            if (e == cudaSuccess) e = cudaStreamWaitEvent(ctx->caller_stream, queued, 0);
+            cudaEventDestroy(queued);
+        }
+    }
+    if (e != cudaSuccess) return fail(ML2_E_CUDA, "caller's stream: %s", cudaGetErrorString(e));
+    ctx->stream = ctx->caller_stream;
+    return ML2_OK;
+}
+
 // ---- launch planning for the streaming mat-vec ---------------------------------------------------
 // Picks rows-per-warp (RW), chunks per stage (MW), ring depth and CTAs per SM so that (a) every bulk
 // copy is 16-byte aligned, (b) a kernel stays within ~half an SM (shared memory, threads, registers)
@@ -246,7 +265,8 @@ int ml2_ctx_destroy(ml2_ctx* h)
 int ml2_ctx_set_stream(ml2_ctx* h, void* s)
 {
     if (!h) return fail(ML2_E_INVALID, "null context");
-    reinterpret_cast<Ctx*>(h)->stream = static_cast<cudaStream_t>(s);
+    Ctx* c = reinterpret_cast<Ctx*>(h);
+    c->stream = c->caller_stream = static_cast<cudaStream_t>(s);
     return ML2_OK;
 }
 int ml2_ctx_set_pdl(ml2_ctx* h, int on)
@@ -265,8 +285,10 @@ int ml2_ctx_set_wait_limit(ml2_ctx* h, long long sm_cycles)
 int ml2_ctx_synchronize(ml2_ctx* h)
 {
     if (!h) return fail(ML2_E_INVALID, "null context");
-    if (int rc = use_device(reinterpret_cast<Ctx*>(h))) return rc;
-    const cudaError_t e = cudaStreamSynchronize(reinterpret_cast<Ctx*>(h)->stream);
+    Ctx* c = reinterpret_cast<Ctx*>(h);
+    if (int rc = use_device(c)) return rc;
+    cudaError_t e = cudaStreamSynchronize(c->stream);
+    if (e == cudaSuccess && c->stream != c->caller_stream) e = cudaStreamSynchronize(c->caller_stream);
     if (e != cudaSuccess) return fail(ML2_E_CUDA, "synchronize: %s", cudaGetErrorString(e));
     return ML2_OK;
 }
@@ -276,7 +298,8 @@ int ml2_ctx_status(ml2_ctx* h, unsigned* error, unsigned* detail)
     if (!c) return fail(ML2_E_INVALID, "null context");
     if (int rc = use_device(c)) return rc;
     DeviceStatus both[2] = {};
-    cudaError_t e = cudaMemcpyAsync(both, c->status_dev, sizeof(both), cudaMemcpyDeviceToHost, c->stream);
+    cudaError_t e = c->stream != c->caller_stream ? cudaStreamSynchronize(c->caller_stream) : cudaSuccess;
+    if (e == cudaSuccess) e = cudaMemcpyAsync(both, c->status_dev, sizeof(both), cudaMemcpyDeviceToHost, c->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
     const int which = both[0].error ? 0 : 1;  // the other word, if it is set too, is reported by the next call
     const DeviceStatus& st = both[which];

@@ -324,7 +324,7 @@ extern "C" int ml2_block_tables(ml2_ctx* h, const ml2_block_tables_args* args)
                     n_requests, table_stride, page_size, n_pages, position_offset);
     if (new_lengths == lengths_out || new_lengths == lengths)
         return fail(ML2_E_INVALID, "block_tables: new_lengths must be an array of its own");
-    if (int rc = use_device(ctx)) return rc;
+    if (int rc = use_callers_stream(ctx)) return rc;
 
     TablesParams p{};
     p.lengths = lengths; p.new_lengths = new_lengths; p.table = table; p.free_pages = free_pages; p.free_count = free_count;

@@ -13,7 +13,8 @@ namespace ml2 {
 struct Ctx {
     int device = 0;
     int sm_count = 0;
-    cudaStream_t stream = nullptr;
+    cudaStream_t stream = nullptr;         // of the next launch: the caller's, or a model's own once that has run
+    cudaStream_t caller_stream = nullptr;  // what ml2_ctx_set_stream was given last
     bool pdl = false;
     DeviceStatus* status_dev = nullptr;   // [0] waits that ran out, [1] invalid indices met by an operator
     void* scratch = nullptr;          // host-buffer entry points stage their vectors here
@@ -38,6 +39,9 @@ int fail(int code, const char* fmt, ...);
 // Makes the context's device current for the calling thread (every entry point does this first: a thread may hold
 // several contexts, or may have switched device in between).
 int use_device(const Ctx* ctx);
+// The same, and the context's launches go to the caller's stream again, behind what a model of the context has queued on its own:
+// a caller's tensors are ordered by the caller's stream.
+int use_callers_stream(Ctx* ctx);
 int plan_matvec(const Ctx* ctx, Fmt fmt, Epi epi, int rows, int cols, int nmat, MatVecPlan* pl);
 int launch_matvec(Ctx* ctx, Fmt fmt, Epi epi, Pro pro, const MatVecPlan& pl, MatVecParams prm, bool pdl);
 

@@ -985,7 +985,8 @@ int ml2_model_destroy(ml2_model* h)
     if (m->mega_op_tiles) cudaFree(m->mega_op_tiles);
     if (m->mega_done) cudaFree(m->mega_done);
     for (void* p : m->owned) cudaFree(p);
-    if (m->ctx->stream == m->stream) m->ctx->stream = nullptr;
+    if (m->ctx->caller_stream == m->stream) m->ctx->caller_stream = nullptr;
+    if (m->ctx->stream == m->stream) m->ctx->stream = m->ctx->caller_stream;
     if (m->stream) cudaStreamDestroy(m->stream);
     delete m;
     return ML2_OK;

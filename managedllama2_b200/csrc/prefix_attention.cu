@@ -1273,7 +1273,7 @@ int ml2_prefix_attention(ml2_ctx* h, const ml2_prefix_attention_args* args)
         return fail(ML2_E_INVALID, "prefix_attention: n_rows=%d with %d heads is too much for one call", n_rows, n_heads);
     if (workspace_bytes < pl.bytes || (pl.bytes && !workspace))
         return fail(ML2_E_INVALID, "prefix_attention: the workspace has %zu bytes, %zu are needed", workspace_bytes, pl.bytes);
-    if (int rc = use_device(ctx)) return rc;
+    if (int rc = use_callers_stream(ctx)) return rc;
     AttnBatch p{};
     p.out = out; p.lse = lse; p.q = query; p.pk = prefix_key; p.pv = prefix_value; p.k = key_cache; p.v = value_cache;
     p.table = table; p.lengths = lengths; p.query_start = query_start; p.status = input_status(ctx);

@@ -168,7 +168,7 @@ extern "C" int ml2_qk_norm_rope(ml2_ctx* h, const ml2_qk_norm_rope_args* args)
     if ((query_out_stride | query_stride | key_stride | value_stride | cache_stride) % 8 || !aligned_to(16, query_out, query, key, value) ||
         !aligned_to(16, key_cache, value_cache) || !aligned_to(16, query_weight, key_weight) || !aligned_to(4, positions, slots))
         return fail(ML2_E_INVALID, "qk_norm_rope: pointers must be 16-byte aligned (int arrays 4) and row strides multiples of 8 elements");
-    if (int rc = use_device(ctx)) return rc;
+    if (int rc = use_callers_stream(ctx)) return rc;
 
     RopeParams p{};
     p.q_out = query_out; p.k_cache = key_cache; p.v_cache = value_cache;

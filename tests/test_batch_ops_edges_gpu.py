@@ -1,5 +1,6 @@
 """Edges of the batched-decoding operators: what a call may hold beyond the ordinary (long flat tails under a peak, scales of
 zero, broken tables, request counts around a limit of the launch) and memory that a call must leave alone."""
+import ctypes
 import math
 import os
 import random
@@ -302,3 +303,126 @@ def test_tables_write_nothing_around_their_arrays(ctx):
         refused, start, slots, positions = plain.step(new, width, rows, 5)
         assert a["refused"].tolist() == refused and a["start"].tolist() == start and a["slots"].tolist() == slots and a["positions"].tolist() == positions
         assert all(v[1]() for v in arrays.values()), [k for k, v in arrays.items() if not v[1]()]
+
+
+# ---- a model on the same context -----------------------------------------------------------------------------------------------
+def small_model(c):
+    cfg = ml2.Config(256, 768, 2, 2, 2, 512, 64)
+    tr = ml2.Transformer(cfg, ml2.synthetic_weights(c, cfg, seed=3, sigma=1.0), c)
+    tr.set_tokens([7, 99, 300, 41])
+    return tr
+
+
+def busy(stream):
+    """About 20 ms of nothing on a stream."""
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(40_000_000)
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_operators_run_on_the_callers_stream_after_a_model_has_run(own_stream):
+    """Their inputs come late, on the caller's stream: a launch on the stream of the model, which is idle, would miss them."""
+    c = ml2.CudaContext(0)
+    tr = small_model(c)
+    stream = torch.cuda.Stream() if own_stream else torch.cuda.current_stream()
+    if own_stream:
+        c.set_stream(stream.cuda_stream)
+    b = Batch(6, "fp16", 4, 2, 128, 16, 300, [20] * 5, [1] * 5)
+    n, head = 5, 128
+    kc, vc = torch.zeros(16, 2 * head, device="cuda").half(), torch.zeros(16, 2 * head, device="cuda").half()
+    tables, norm, attend = ml2.BlockTables(c, 16), ml2.QKNormRoPE(c, b.cfg), ml2.PrefixAttention(c, b.cfg, 16)
+    ws = torch.empty(attend.WorkspaceBytes(n, n, 300, 20), dtype=torch.uint8, device="cuda")
+    late = dict(q=b.q.clone(), new=ints([3] * n), positions=ints(list(range(n))), slots=ints([9, 3, 5, 0, 1]))
+    now = {k: torch.zeros_like(v) for k, v in late.items()}
+    out, z, turned = torch.zeros(n, 4 * head, device="cuda").half(), torch.zeros(n, 4, device="cuda"), torch.zeros(n, 4 * head, device="cuda").half()
+    t = dict(lengths=ints([0] * n), table=ints([[-1]] * n), free=ints(list(range(n))), count=ints([n]), start=ints([0] * (n + 1)),
+             slots=ints([7] * 15), positions=ints([7] * 15), refused=ints([7] * n))
+
+    def calls():
+        tables.Forward(t["lengths"], now["new"], t["table"], t["free"], t["count"], t["lengths"], t["count"], t["start"], t["slots"], t["positions"],
+                       t["refused"])
+        norm.Forward(turned, kc, vc, now["q"], b.pk[:n], b.pv[:n], None, None, now["positions"], now["slots"])
+        attend.Forward(out, now["q"], b.pk, b.pv, b.k, b.v, b.table, b.lengths, b.start, ws, 20, z)
+    torch.cuda.synchronize()
+    for first in ("tables", "norm", "attend"):  # each of them the first call after the model
+        for v in now.values():
+            v.zero_()
+        t["lengths"].zero_()
+        t["count"].fill_(n)
+        torch.cuda.synchronize()
+        tr.Forward(0, 1, False)
+        tr.synchronize()
+        busy(stream)
+        with torch.cuda.stream(stream):
+            for k, v in late.items():
+                now[k].copy_(v)
+            if first == "norm":
+                norm.Forward(turned, kc, vc, now["q"], b.pk[:n], b.pv[:n], None, None, now["positions"], now["slots"])
+            elif first == "attend":
+                attend.Forward(out, now["q"], b.pk, b.pv, b.k, b.v, b.table, b.lengths, b.start, ws, 20, z)
+            calls()
+            got = out.clone(), z.clone(), kc.clone(), t["slots"].clone()
+        stream.synchronize()
+        want, lse, tol, tol_lse = b.want()
+        assert bool(((got[0].double() - want).abs() <= tol).all()) and bool(((got[1].double() - lse).abs() <= tol_lse).all()), first
+        assert bool((got[2][[9, 3, 5, 0, 1]] != 0).any(1).all()) and bool((got[2][[2, 4, 6, 7, 8]] == 0).all()), first
+        assert got[3].tolist() == [16 * (n - 1 - r) + i for r in range(n) for i in range(3)], first
+    assert c.status() == (0, 0)
+    tr.close()
+    c.close()
+
+
+def test_operators_follow_what_a_model_has_queued():
+    """The prompt is still under way when its rows are asked for as the prefix."""
+    c = ml2.CudaContext(0)
+    tr = small_model(c)
+    ptr = ctypes.c_void_p()
+    ml2._lib.check(tr.lib.ml2_model_stream(tr.handle, ctypes.byref(ptr)))
+    rs = tr.runstate_ptrs()
+
+    class Rows:
+        def __init__(self, at):
+            self.__cuda_array_interface__ = {"shape": (64, 256), "typestr": "<f2", "data": (at, False), "version": 2}
+    b = Batch(12, "fp16", 2, 2, 128, 16, 4, [4, 30, 1], [1, 1, 1])
+    b.pk, b.pv = (torch.as_tensor(Rows(p), device="cuda")[:4] for p in (rs.key_cache, rs.value_cache))
+    b.pk.zero_()
+    b.pv.zero_()
+    b.call(c)
+    torch.cuda.synchronize()
+    busy(torch.cuda.ExternalStream(ptr.value))
+    for pos in range(4):
+        tr.Forward(pos, pos + 1, False)
+    out, z = b.call(c)
+    got, lse = out.clone(), z.clone()
+    torch.cuda.synchronize()
+    assert bool((b.pk != 0).any(1).all())
+    want, want_lse, tol, tol_lse = b.want()
+    assert bool(((got.double() - want).abs() <= tol).all()) and bool(((lse.double() - want_lse).abs() <= tol_lse).all())
+    assert c.status() == (0, 0)
+    tr.close()
+    c.close()
+
+
+def test_a_captured_call_after_a_model_has_run_lands_on_the_callers_stream():
+    c = ml2.CudaContext(0)
+    tr = small_model(c)
+    b = Batch(6, "fp16", 4, 2, 128, 16, 1300, [20] * 5, [1] * 5)
+    want, lse = b.call(c)
+    op = ml2.PrefixAttention(c, b.cfg, 16)
+    ws = torch.empty(op.WorkspaceBytes(5, 5, 1300, 20), dtype=torch.uint8, device="cuda")
+    out, z = torch.zeros(5, 512, device="cuda").half(), torch.zeros(5, 4, device="cuda")
+    s = torch.cuda.Stream()
+    c.set_stream(s.cuda_stream)
+    tr.Forward(0, 1, False)
+    tr.synchronize()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        op.Forward(out, b.q, b.pk, b.pv, b.k, b.v, b.table, b.lengths, b.start, ws, 20, z)
+    assert bool((out == 0).all())
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(z, lse) and c.status() == (0, 0)
+    del g
+    tr.close()
+    c.close()
