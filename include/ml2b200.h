@@ -78,11 +78,14 @@ int ml2_ctx_set_pdl(ml2_ctx* ctx, int enabled);
 int ml2_ctx_synchronize(ml2_ctx* ctx);
 /* Budget of every device-side wait (mbarrier phases, operator counters, peer counters), in SM clock
  * cycles; default 2e10 (about ten seconds). A wait that runs out writes the error word and the kernel
- * runs to its end; the next synchronising call returns ML2_E_DEVICE. No counterpart in the reference
- * (its kernels never wait on one another). */
+ * runs to its end; the next synchronising call of the model (ml2_model_*) returns ML2_E_DEVICE. After
+ * ml2_prefix_attention it is ml2_ctx_status alone that does, and the call's output is undefined; a model
+ * of the same context is not affected. No counterpart in the reference (its kernels never wait on one
+ * another). */
 int ml2_ctx_set_wait_limit(ml2_ctx* ctx, long long sm_cycles);
 /* Reads and clears the device error words: a kernel's bounded wait expired, or (codes from 0x101 on) one of the
- * batched-decoding operators left out an element because its index in a device table was out of range. */
+ * batched-decoding operators left out an element because its index in a device table was out of range, or
+ * (0x106) gave up waiting itself. */
 int ml2_ctx_status(ml2_ctx* ctx, unsigned* error, unsigned* detail);
 /* Number of kernels this library has launched through `ctx` so far. */
 long long ml2_ctx_launch_count(ml2_ctx* ctx);

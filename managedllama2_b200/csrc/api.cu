@@ -315,6 +315,7 @@ int ml2_ctx_status(ml2_ctx* h, unsigned* error, unsigned* detail)
     case kInputPage: return fail(ML2_E_DEVICE, "a page of request %u lies outside the cache", st.detail);
     case kInputSlot: return fail(ML2_E_DEVICE, "the slot of token %u lies outside the cache", st.detail);
     case kInputLength: return fail(ML2_E_DEVICE, "the length or the query rows of request %u are out of range", st.detail);
+    case kAttentionGaveUp: return fail(ML2_E_DEVICE, "prefix_attention: a wait of block %u ran out, the output is undefined", st.detail);
     default: return fail(ML2_E_DEVICE, "input error %u (%u)", st.error, st.detail);
     }
 }

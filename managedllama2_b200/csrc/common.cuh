@@ -17,9 +17,7 @@ struct DeviceStatus {
     unsigned int detail;
 };
 
-constexpr unsigned int kAttentionGaveUp = 0x50;  // a wait inside the prefix kernel ran out (first status word)
-
-// What an operator that reads indices from device tables found wrong in them (second status word of the context). The
+// What a batched-decoding operator found wrong in device tables (second status word of the context). The
 // first finding is kept; the element is left out (its row, token or page counts as absent) and the kernel goes on.
 enum InputError : unsigned int {
     kInputFreeCount = 0x101,     // count of the free pages outside 0..n_pages; detail = the count
@@ -27,6 +25,7 @@ enum InputError : unsigned int {
     kInputPage = 0x103,          // page number outside the cache; detail = request
     kInputSlot = 0x104,          // slot outside the cache; detail = token
     kInputLength = 0x105,        // length above max_length or negative, or query rows out of order; detail = request
+    kAttentionGaveUp = 0x106,    // no fault of the input: a wait inside the prefix kernel ran out; detail = CTA
 };
 
 __host__ __device__ constexpr int ceil_div(int a, int b) { return (a + b - 1) / b; }

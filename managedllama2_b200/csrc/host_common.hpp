@@ -16,7 +16,7 @@ struct Ctx {
     cudaStream_t stream = nullptr;         // of the next launch: the caller's, or a model's own once that has run
     cudaStream_t caller_stream = nullptr;  // what ml2_ctx_set_stream was given last
     bool pdl = false;
-    DeviceStatus* status_dev = nullptr;   // [0] waits that ran out, [1] invalid indices met by an operator
+    DeviceStatus* status_dev = nullptr;   // [0] waits of a model that ran out, [1] what a batched-decoding operator met
     void* scratch = nullptr;          // host-buffer entry points stage their vectors here
     size_t scratch_bytes = 0;
     long long launches = 0;
@@ -45,7 +45,8 @@ int use_callers_stream(Ctx* ctx);
 int plan_matvec(const Ctx* ctx, Fmt fmt, Epi epi, int rows, int cols, int nmat, MatVecPlan* pl);
 int launch_matvec(Ctx* ctx, Fmt fmt, Epi epi, Pro pro, const MatVecPlan& pl, MatVecParams prm, bool pdl);
 
-// What an operator finds wrong in device tables goes here: apart from the waits' word, which stops the persistent kernel.
+// What an operator finds wrong in device tables, or its own waits that ran out, go here: apart from the word of a model's waits,
+// which stops the persistent kernel.
 inline DeviceStatus* input_status(const Ctx* ctx) { return ctx->status_dev + 1; }
 
 constexpr int kMaxPageSize = 1024;

@@ -21,7 +21,6 @@ struct AttnBatch {
     const void *q, *pk, *pv, *k, *v;
     const int *table, *lengths, *query_start;
     DeviceStatus* status;
-    DeviceStatus* waits;
     // Partial results, for a row and head the sum o = sum of exp2(score - m) v over some of the keys [head], and (m, l): a
     // reference up to 2^15 below the largest score (in powers of two) and l = sum of exp2(score - m). One without keys has m = -inf, l = 0
     // and an o that is not read. pre: of the prefix by blocks, [segments][rows that are there][n_heads]; run: of the warps' runs.
@@ -976,7 +975,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
         });
     }
     __syncthreads();
-    if (threadIdx.x == 0 && s_abort) atomicCAS(&p.waits->error, 0u, kAttentionGaveUp);
+    if (threadIdx.x == 0 && s_abort) report_input_error(p.status, kAttentionGaveUp, blockIdx.x);
     tc_fence_after();
     if (warp == 16) tmem_free(tmem, 512);
 }
@@ -1286,7 +1285,7 @@ int ml2_prefix_attention(ml2_ctx* h, const ml2_prefix_attention_args* args)
     p.pre_ml = reinterpret_cast<float2*>(ws + pl.pre_ml); p.run_ml = reinterpret_cast<float2*>(ws + pl.run_ml);
     p.run_base = reinterpret_cast<int*>(ws + pl.run_base);
     p.prefix_ctas = pl.prefix_ctas; p.run_ctas = pl.run_ctas; p.own_places = (int)pl.own_places;
-    p.waits = ctx->status_dev; p.wait_cycles = ctx->wait_cycles;
+    p.wait_cycles = ctx->wait_cycles;
     PrefixMaps maps{};
     if (pl.prefix_ctas && (!make_map(&maps.k, dtype, prefix_key, prefix_stride, (int)kv_width, p.prefix) ||
                            !make_map(&maps.v, dtype, prefix_value, prefix_stride, (int)kv_width, p.prefix)))

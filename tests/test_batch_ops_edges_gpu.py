@@ -426,3 +426,36 @@ def test_a_captured_call_after_a_model_has_run_lands_on_the_callers_stream():
     del g
     tr.close()
     c.close()
+
+
+# ---- waits that run out ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads,kv,head,prefix,requests", [(64, 8, 128, 16384, 128), (40, 40, 128, 4096, 64), (8, 8, 64, 20000, 1), (37, 37, 64, 1100, 150)])
+def test_attention_that_gives_up_waiting_is_reported_and_leaves_a_model_alone(heads, kv, head, prefix, requests):
+    """With a limit of 1000 cycles waits for keys that come from memory run out (of a small prefix that is in the cache none
+    need to). The call comes to its end, is reported by ``status``, writes nothing outside its outputs, and neither a model
+    of the same context nor the next call suffers. One that is not reported is right."""
+    c = ml2.CudaContext(0)
+    tr = small_model(c)
+    b = Batch(3, "fp16", heads, kv, head, 16, prefix, [20] * requests, [1] * requests)
+    want, lse = b.call(c)
+    reports = 0
+    for _ in range(3):
+        c.set_wait_limit(1000)
+        out, z = guarded_call(c, b)
+        c.synchronize()
+        c.set_wait_limit(2 * 10**9)
+        tr.Forward(0, 1, False)
+        tr.synchronize()
+        try:
+            c.status()
+        except ml2.Ml2Error as e:
+            reports += 1
+            assert "prefix_attention: a wait of block" in str(e)
+        else:
+            assert torch.equal(out, want) and torch.equal(z, lse)
+        assert c.status() == (0, 0)
+        out, z = b.call(c)
+        assert torch.equal(out, want) and torch.equal(z, lse)
+    assert reports or requests < 128 or prefix < 16384  # 220 tiles a block: it waits for every ring slot
+    tr.close()
+    c.close()
