@@ -1287,8 +1287,12 @@ int ml2_prefix_attention(ml2_ctx* h, const ml2_prefix_attention_args* args)
     p.prefix_ctas = pl.prefix_ctas; p.run_ctas = pl.run_ctas; p.own_places = (int)pl.own_places;
     p.wait_cycles = ctx->wait_cycles;
     PrefixMaps maps{};
-    if (pl.prefix_ctas && (!make_map(&maps.k, dtype, prefix_key, prefix_stride, (int)kv_width, p.prefix) ||
-                           !make_map(&maps.v, dtype, prefix_value, prefix_stride, (int)kv_width, p.prefix)))
+    auto make_maps = [&] {
+        return make_map(&maps.k, dtype, prefix_key, prefix_stride, (int)kv_width, p.prefix) &&
+               make_map(&maps.v, dtype, prefix_value, prefix_stride, (int)kv_width, p.prefix);
+    };
+    // The driver makes no map in a thread that has not used the device yet (the runtime's own calls bind it as they need it).
+    if (pl.prefix_ctas && !make_maps() && (cudaSetDevice(ctx->device) != cudaSuccess || !make_maps()))
         return fail(ML2_E_CUDA, "prefix_attention: no tensor map for a prefix of %d rows of %lld, stride %lld", p.prefix, kv_width, prefix_stride);
     cudaError_t e;
     if (head_size == 128) e = dtype == ML2_F16 ? launch_attention<__half, 128>(ctx, p, pl, maps) : launch_attention<__nv_bfloat16, 128>(ctx, p, pl, maps);

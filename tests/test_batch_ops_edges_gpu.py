@@ -6,6 +6,7 @@ import os
 import random
 import subprocess
 import sys
+import threading
 
 import pytest
 import torch
@@ -204,13 +205,15 @@ def tables_of_many_requests():
 
 def test_block_tables_around_the_default_shared_memory_of_a_launch():
     """In a process of its own: a larger call made before would have raised the limit."""
-    code = "import sys; sys.path[:0] = %r; import test_batch_ops_edges_gpu as t; t.tables_of_many_requests()" % ([os.path.dirname(__file__), base_root()],)
+    run_alone("tables_of_many_requests")
+
+
+def run_alone(name):
+    """A function of this file in a process of its own."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = "import sys; sys.path[:0] = %r; import test_batch_ops_edges_gpu as t; t.%s()" % ([here, os.path.dirname(here)], name)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
-
-
-def base_root():
-    return os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 # ---- memory that a call leaves alone -------------------------------------------------------------------------------------------
@@ -459,3 +462,41 @@ def test_attention_that_gives_up_waiting_is_reported_and_leaves_a_model_alone(he
     assert reports or requests < 128 or prefix < 16384  # 220 tiles a block: it waits for every ring slot
     tr.close()
     c.close()
+
+
+# ---- calls from several threads --------------------------------------------------------------------------------------------------
+def first_calls_from_threads():
+    cases = []
+    for i in range(4):
+        c, s = ml2.CudaContext(0), torch.cuda.Stream()
+        b = Batch(40 + i, ("fp16", "bf16")[i & 1], 4, 2, (64, 128)[i >> 1], 16, 1100 + i, *base.ragged(i, 20, 60, 2))
+        op = ml2.PrefixAttention(c, b.cfg, 16)
+        ws = torch.empty(op.WorkspaceBytes(b.q.shape[0], 20, b.prefix, 60), dtype=torch.uint8, device="cuda")
+        out = torch.zeros(b.q.shape[0], 4 * b.head, dtype=b.t, device="cuda")
+        c.set_stream(s.cuda_stream)
+        cases.append((c, s, b, op, ws, out))
+    torch.cuda.synchronize()
+    errors = []
+
+    def calls(c, s, b, op, ws, out):
+        try:
+            for _ in range(50):
+                op.Forward(out, b.q, b.pk, b.pv, b.k, b.v, b.table, b.lengths, b.start, ws, 60)
+            c.synchronize()
+            assert c.status() == (0, 0)
+        except BaseException as e:
+            errors.append(e)
+    threads = [threading.Thread(target=calls, args=case) for case in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for c, s, b, op, ws, out in cases:
+        want, _, tol, _ = b.want()
+        assert bool(((out.double() - want).abs() <= tol).all())
+        c.close()
+
+
+def test_first_calls_of_a_process_from_threads_with_contexts_of_their_own():
+    run_alone("first_calls_from_threads")
