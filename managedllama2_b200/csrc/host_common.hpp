@@ -20,6 +20,7 @@ struct Ctx {
     void* scratch = nullptr;          // host-buffer entry points stage their vectors here
     size_t scratch_bytes = 0;
     long long launches = 0;
+    bool attention_ready[2][2] = {};  // prefix_attention.cu: kernels of either type and head size may be launched
     long long wait_cycles = 20000000000ll;   // budget of every device-side wait, in SM clock cycles (about ten seconds)
 };
 

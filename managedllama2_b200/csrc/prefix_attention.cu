@@ -1174,13 +1174,13 @@ static bool make_map(CUtensorMap* map, int dtype, const void* base, long long ro
 template <typename T, int kHead>
 static cudaError_t launch_attention(Ctx* ctx, const AttnBatch& p, const AttnPlan& pl, const PrefixMaps& maps)
 {
-    static bool ready[16] = {};  // shared-memory limits are set once per device
+    bool& ready = ctx->attention_ready[std::is_same<T, __half>::value][kHead == 128];  // shared-memory limits are set once
     cudaError_t e = cudaSuccess;
-    if (!ready[ctx->device & 15]) {
+    if (!ready) {
         e = cudaFuncSetAttribute(attention_runs_kernel<T, kHead>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_prefix_kernel<T, kHead>, cudaFuncAttributeMaxDynamicSharedMemorySize, BlockSmem<kHead>::kBytes);
         if (e != cudaSuccess) return e;
-        ready[ctx->device & 15] = true;
+        ready = true;
     }
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
