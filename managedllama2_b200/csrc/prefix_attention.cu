@@ -1216,7 +1216,9 @@ static int check_sizes(const char* what, int n_rows, int n_requests, int prefix,
 {
     if (n_rows < 0 || n_requests < 1 || n_requests > kMaxRequests)
         return fail(ML2_E_INVALID, "%s: n_rows=%d n_requests=%d (1..%d)", what, n_rows, n_requests, kMaxRequests);
-    if (prefix < 0 || max_length < 0) return fail(ML2_E_INVALID, "%s: prefix of %d rows, max_length=%d", what, prefix, max_length);
+    constexpr int kMost = INT32_MAX - 63;  // whole tiles of keys stay below 2^31
+    if (prefix < 0 || max_length < 0 || prefix > kMost || max_length > kMost)
+        return fail(ML2_E_INVALID, "%s: prefix of %d rows, max_length=%d", what, prefix, max_length);
     if (n_heads < 1 || n_kv < 1 || n_heads % n_kv || n_heads > 65536)
         return fail(ML2_E_INVALID, "%s: n_heads=%d must be a multiple of n_kv_heads=%d", what, n_heads, n_kv);
     if (head_size != 64 && head_size != 128) return fail(ML2_E_INVALID, "%s: head_size=%d must be 64 or 128", what, head_size);

@@ -24,3 +24,27 @@ def test_packed_arguments_are_as_long_as_the_struct(name, arguments):
     assert len(packed) == ctypes.sizeof(layout)
     got = layout.from_buffer_copy(packed)
     assert [getattr(got, n) for n in arguments.names] == list(values)
+
+
+def workspace(calls, **change):
+    lib, ctx, _ = calls
+    a = dict(n_rows=1, n_requests=1, prefix=0, max_length=0, n_heads=2, n_kv_heads=2, head_size=64)
+    a.update(change)
+    n = ctypes.c_size_t()
+    rc = lib.ml2_prefix_attention_workspace(ctypes.c_void_p(ctx), *map(ctypes.c_int, a.values()), ctypes.byref(n))
+    return rc, n.value
+
+
+@pytest.mark.parametrize("name", ["prefix", "max_length"])
+def test_prefix_attention_lengths_next_to_the_largest_int(calls, name):  # noqa: F811
+    """Lengths are rounded up to whole tiles of 64 keys: 2^31 - 64 is the largest that can be."""
+    lib, ctx, _ = calls
+    for x in (2**31 - 63, 2**31 - 1):
+        refused(lib, workspace(calls, **{name: x})[0], name)
+    before = 0
+    for x in (100, 2**20, 2**30, 2**31 - 64):
+        rc, n = workspace(calls, **{name: x})
+        assert rc == 0 and before <= n < 1 << 40
+        before = n
+    change = dict(prefix_length=2**31 - 1) if name == "prefix" else dict(max_length=2**31 - 1, table_stride=2**31 - 1, page_size=1)
+    refused(lib, call(lib.ml2_prefix_attention, _lib.PREFIX_ATTENTION, dict(ATTN, ctx=ctx, **change)), name)
