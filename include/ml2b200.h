@@ -174,7 +174,8 @@ typedef struct ml2_block_tables_args {
 int ml2_block_tables(ml2_ctx* ctx, const ml2_block_tables_args* args);
 /* RMS norm of every query and key head (weights of head_size values; both null: no norm), rotation of the first
  * rotary_size values of each head (pairs i, i + rotary_size / 2 as in ml2_rope; angle positions[t] *
- * theta^(-2i / rotary_size), reduced in 64 bits), queries to query_out (may be query), keys and values to the cache rows
+ * theta^(-2i / rotary_size), reduced in 64 bits), queries to query_out (may be query, with its stride;
+ * nothing written may overlap anything else that is read), keys and values to the cache rows
  * slots[t], which must differ from one another. A token with a negative slot is padding: nothing of it is written.
  * Arithmetic in fp32, one rounding to `dtype`. head_size and rotary_size are multiples of 16, head_size at most 256;
  * strides in elements, multiples of 8; pointers 16-byte aligned. */

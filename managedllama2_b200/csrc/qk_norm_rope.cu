@@ -164,6 +164,8 @@ extern "C" int ml2_qk_norm_rope(ml2_ctx* h, const ml2_qk_norm_rope_args* args)
     const long long q_width = (long long)n_heads * head_size, kv_width = (long long)n_kv_heads * head_size;
     if (query_out_stride < q_width || query_stride < q_width || key_stride < kv_width || value_stride < kv_width || cache_stride < kv_width)
         return fail(ML2_E_INVALID, "qk_norm_rope: a row stride is shorter than the row");
+    if (query_out == query && query_out_stride != query_stride && n_tokens > 1)
+        return fail(ML2_E_INVALID, "qk_norm_rope: queries over themselves need one row stride, not %lld and %lld", query_stride, query_out_stride);
     if (cache_rows < 1 || cache_rows > INT32_MAX) return fail(ML2_E_INVALID, "qk_norm_rope: the cache has %lld rows", cache_rows);
     if ((query_out_stride | query_stride | key_stride | value_stride | cache_stride) % 8 || !aligned_to(16, query_out, query, key, value) ||
         !aligned_to(16, key_cache, value_cache) || !aligned_to(16, query_weight, key_weight) || !aligned_to(4, positions, slots))

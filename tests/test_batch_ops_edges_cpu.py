@@ -4,7 +4,7 @@ import ctypes
 import pytest
 
 from managedllama2_b200 import _lib
-from test_batch_ops_cpu import ATTN, call, calls, refused  # noqa: F401  (calls is a fixture)
+from test_batch_ops_cpu import ATTN, P, ROPE, call, calls, refused  # noqa: F401  (calls is a fixture)
 
 
 @pytest.mark.parametrize("scale", [3e38, -2.4e38])
@@ -48,3 +48,11 @@ def test_prefix_attention_lengths_next_to_the_largest_int(calls, name):  # noqa:
         before = n
     change = dict(prefix_length=2**31 - 1) if name == "prefix" else dict(max_length=2**31 - 1, table_stride=2**31 - 1, page_size=1)
     refused(lib, call(lib.ml2_prefix_attention, _lib.PREFIX_ATTENTION, dict(ATTN, ctx=ctx, **change)), name)
+
+
+def test_qk_norm_rope_refuses_queries_over_themselves_with_another_stride(calls):  # noqa: F811
+    """A row's result would lie over a row that another block has still to read."""
+    lib, ctx, _ = calls
+    for strides in ((256, 768), (768, 256)):
+        a = dict(ROPE, ctx=ctx, query=P, query_out=P, query_stride=strides[0], query_out_stride=strides[1])
+        refused(lib, call(lib.ml2_qk_norm_rope, _lib.QK_NORM_ROPE, a), "stride")
