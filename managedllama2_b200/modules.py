@@ -415,7 +415,9 @@ class PrefixAttention(Module):
         if outRows < rows or table.dim() != 2 or table.shape[0] != n:
             raise ValueError("output needs %d rows and table %d; got %d and %s" % (rows, n, outRows, tuple(table.shape)))
         prefix, prefixKeyPtr, prefixValuePtr = (0, kvWidth), 0, 0
-        if prefixKey is not None and prefixKey.shape[0] > 0:
+        if (prefixKey is not None and prefixKey.numel()) or (prefixValue is not None and prefixValue.numel()):
+            if prefixKey is None or prefixValue is None:
+                raise ValueError("prefixKey and prefixValue come together or not at all")
             prefix = _rows(c, "prefixKey", prefixKey, kvWidth, dtype)
             if _rows(c, "prefixValue", prefixValue, kvWidth, dtype) != prefix:
                 raise ValueError("prefixKey and prefixValue must have the same rows and strides")

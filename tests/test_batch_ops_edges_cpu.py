@@ -2,7 +2,9 @@
 import ctypes
 
 import pytest
+import torch
 
+import managedllama2_b200 as ml2
 from managedllama2_b200 import _lib
 from test_batch_ops_cpu import ATTN, P, ROPE, call, calls, refused  # noqa: F401  (calls is a fixture)
 
@@ -56,3 +58,43 @@ def test_qk_norm_rope_refuses_queries_over_themselves_with_another_stride(calls)
     for strides in ((256, 768), (768, 256)):
         a = dict(ROPE, ctx=ctx, query=P, query_out=P, query_stride=strides[0], query_out_stride=strides[1])
         refused(lib, call(lib.ml2_qk_norm_rope, _lib.QK_NORM_ROPE, a), "stride")
+
+
+# ---- the modules' own checks, on CPU tensors: the call into the library is replaced ------------------------------------------------
+@pytest.fixture()
+def modules():
+    lib = ml2.load()
+
+    class Context:
+        _lib, handle, device = lib, ctypes.c_void_p(0), -1  # the device number of CPU tensors
+    cfg = ml2.Config(256, 0, 1, 2, 2, 0, 0)
+    made = [ml2.BlockTables(Context, 16), ml2.QKNormRoPE(Context, cfg), ml2.PrefixAttention(Context, cfg, 16)]
+    calls = []
+    for m in made:
+        m._call = lambda handle, packed: calls.append(packed) or 0
+    return made + [calls]
+
+
+def attention_arguments(**change):
+    def half(*shape):
+        return torch.zeros(*shape, dtype=torch.float16)
+
+    def ints(*shape):
+        return torch.zeros(*shape, dtype=torch.int32)
+    a = dict(output=half(3, 256), query=half(3, 256), prefixKey=half(20, 256), prefixValue=half(20, 256), keyCache=half(64, 256),
+             valueCache=half(64, 256), table=ints(2, 4), lengths=ints(2), queryStart=ints(3), workspace=half(4096), maxLength=40)
+    a.update(change)
+    return a
+
+
+def test_prefix_attention_module_takes_prefix_key_and_value_together(modules):
+    attend, calls = modules[2:]
+    some, none = torch.zeros(20, 256, dtype=torch.float16), torch.zeros(0, 256, dtype=torch.float16)
+    for both in ((some, some), (None, None), (none, none), (none, None), (None, none), (some[:1], some[:1])):
+        attend.Forward(**attention_arguments(prefixKey=both[0], prefixValue=both[1]))
+    assert len(calls) == 6
+    for key, value in ((some, None), (None, some), (none, some), (some, none), (some, some[:5]), (some.view(-1), some),
+                       (some, some.float()), (torch.zeros((), dtype=torch.float16), some)):
+        with pytest.raises(ValueError, match="prefix"):
+            attend.Forward(**attention_arguments(prefixKey=key, prefixValue=value))
+    assert len(calls) == 6
