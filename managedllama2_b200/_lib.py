@@ -63,7 +63,14 @@ class Arguments:
             self.names += names
             self.kinds += kind * len(names)
         # 0P: the end is padded to a pointer's alignment, as the struct's is
-        self.pack = struct.Struct("@" + self.kinds.replace("p", "P").replace("l", "q") + "0P").pack
+        self._pack = struct.Struct("@" + self.kinds.replace("p", "P").replace("l", "q") + "0P").pack
+
+    def pack(self, *values):
+        try:
+            return self._pack(*values)
+        except struct.error as e:
+            wrong = [n for n, k, v in zip(self.names, self.kinds, values) if k == "i" and isinstance(v, int) and not -2**31 <= v < 2**31]
+            raise ValueError("%s: passes 32 bits" % ", ".join(wrong) if wrong else str(e)) from None
 
     def entry(self, function):
         function.argtypes = [ctypes.c_void_p, ctypes.c_char_p]

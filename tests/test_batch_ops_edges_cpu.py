@@ -98,3 +98,18 @@ def test_prefix_attention_module_takes_prefix_key_and_value_together(modules):
         with pytest.raises(ValueError, match="prefix"):
             attend.Forward(**attention_arguments(prefixKey=key, prefixValue=value))
     assert len(calls) == 6
+
+
+@pytest.mark.parametrize("number", [2**31, -2**31 - 1, 2**70])
+def test_modules_refuse_numbers_that_pass_32_bits(modules, number):
+    tables, norm, attend, calls = modules
+    ints = torch.zeros(64, dtype=torch.int32)
+    with pytest.raises(ValueError, match="32 bits"):
+        attend.Forward(**attention_arguments(maxLength=number))
+    with pytest.raises(ValueError, match="32 bits"):
+        tables.Forward(ints[:2], ints[:2], ints[:8].view(2, 4), ints, ints[:1], ints[:2], ints[:1], ints[:3], ints[:8], ints[:8], ints[:2], number)
+    x = torch.zeros(2, 256, dtype=torch.float16)
+    norm.rotarySize = number
+    with pytest.raises(ValueError, match="32 bits"):
+        norm.Forward(x, x, x, x, x, x, None, None, ints[:2], ints[:2])
+    assert not calls
