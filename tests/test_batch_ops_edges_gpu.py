@@ -500,3 +500,27 @@ def first_calls_from_threads():
 
 def test_first_calls_of_a_process_from_threads_with_contexts_of_their_own():
     run_alone("first_calls_from_threads")
+
+
+# ---- beside the operators of one sequence ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("pos", [0, 1, 17, 500, 2047, 4095])
+@pytest.mark.parametrize("head", [64, 128])
+def test_rotation_agrees_with_that_of_one_sequence(ctx, pos, head):
+    """Keys of both meet in one softmax: a prefix that went through a model, own tokens through ``QKNormRoPE``. ``RoPERotation``
+    (and the model's table, by the same expressions) takes the angle in 32 bits: a power and a quotient off by 4 steps of 2^-23
+    and half of one, a product by another half, so the angle by 10 * 2^-24 of itself. Either result is rounded once to fp16."""
+    heads = 4
+    g = torch.Generator(device="cuda").manual_seed(pos + head)
+    x = (torch.randn(2, heads * head, generator=g, device="cuda") * 1.5).half()
+    cfg = ml2.Config(heads * head, 0, 1, heads, heads, 0, 0)
+    kc, vc, out = (torch.zeros(1, heads * head, device="cuda").half() for _ in range(3))
+    ml2.QKNormRoPE(ctx, cfg).Forward(out, kc, vc, x[:1], x[1:], x[1:], None, None, ints([pos]), ints([0]))
+    q, k = x[:1].clone(), torch.zeros(pos + 1, heads * head, device="cuda").half()
+    k[pos] = x[1]
+    ml2.RoPERotation(ctx, cfg).Forward(q, k, heads, head, pos, 0, 10000.0)
+    freq = torch.tensor([10000.0 ** (-2.0 * i / head) for i in range(head // 2)], dtype=torch.float64, device="cuda")
+    for got, one, source in ((out[0], q[0], x[0]), (kc[0], k[pos], x[1])):
+        want, slack = base.rope_want(source[None], None, heads, head, head, ints([pos]), 10000.0, 1e-5)
+        y = source.double().reshape(heads, 2, head // 2).abs().sum(1, keepdim=True).expand(heads, 2, head // 2)
+        bound = (2 * slack[0] + (y * (pos * freq * 10 * 2.0 ** -24)).reshape(-1)) * 1.001 + 2 * (2.0 ** -11 * want[0].abs() * 1.01 + 2.0 ** -25)
+        assert bool(((got.double() - one.double()).abs() <= bound).all())
