@@ -524,3 +524,85 @@ def test_rotation_agrees_with_that_of_one_sequence(ctx, pos, head):
         y = source.double().reshape(heads, 2, head // 2).abs().sum(1, keepdim=True).expand(heads, 2, head // 2)
         bound = (2 * slack[0] + (y * (pos * freq * 10 * 2.0 ** -24)).reshape(-1)) * 1.001 + 2 * (2.0 ** -11 * want[0].abs() * 1.01 + 2.0 ** -25)
         assert bool(((got.double() - one.double()).abs() <= bound).all())
+
+
+# ---- the largest and the odd calls -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("prefix", [0, 40, 1100])
+def test_attention_of_as_many_requests_as_there_may_be(ctx, prefix):
+    lengths, queries = base.ragged(3, 8192, 5, 2)
+    lengths[5000], queries[5000] = 300, 7
+    for r in range(0, 8192, 3):
+        queries[r] = 0
+    b = Batch(prefix, "bf16", 2, 1, 64, 16, prefix, lengths, queries, extra_rows=1)
+    out, z = guarded_call(ctx, b)
+    total = sum(queries)
+    want, lse, tol, tol_lse = b.want()
+    assert bool(((out[:total].double() - want).abs() <= tol).all()) and bool(((z[:total].double() - lse).abs() <= tol_lse).all())
+
+
+@pytest.mark.parametrize("pdl", [False, True])
+def test_tables_of_many_rows_in_a_graph(ctx, pdl):
+    """Two kernels, replayed with other lengths; each replay goes on from the last."""
+    rng = random.Random(5)
+    n, page, width, rows = 300, 16, 40, 20000
+    plain, dev = base.tables_setup(rng, n, page, width, n * width)
+    new = ints([0] * n)
+    a = dict(start=ints([7] * (n + 1)), slots=ints([7] * rows), positions=ints([7] * rows), refused=ints([7] * n))
+    op = ml2.BlockTables(ctx, page)
+
+    def step():
+        op.Forward(dev["lengths"], new, dev["table"], dev["free"], dev["count"], dev["lengths"], dev["count"], a["start"], a["slots"], a["positions"],
+                   a["refused"], 9)
+    new.copy_(dev["lengths"])
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    ctx.set_stream(s.cuda_stream)
+    ctx.set_pdl(pdl)
+    try:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            step()
+    finally:
+        ctx.set_pdl(False)
+        ctx.set_stream(0)
+    for _ in range(4):
+        want = [rng.choice([0, x, min(x + 1, width * page), rng.randint(0, width * page)]) for x in plain.old]
+        new.copy_(ints(want))
+        g.replay()
+        refused, start, slots, positions = plain.step(want, width, rows, 9)
+        torch.cuda.synchronize()
+        assert a["refused"].tolist() == refused and a["start"].tolist() == start
+        assert a["slots"].tolist() == slots and a["positions"].tolist() == positions and dev["lengths"].tolist() == plain.old
+        assert dev["free"].tolist()[:len(plain.free)] == plain.free
+
+
+@pytest.mark.parametrize("prefix,requests", [(300, 40), (1500, 40), (1500, 300)])
+def test_attention_a_row_that_is_not_finite_spoils_itself_alone(ctx, prefix, requests):
+    b = Batch(8, "fp16", 4, 2, 64, 16, prefix, [20] * requests, [1] * requests, extra_rows=2)
+    clean_out, clean_lse = b.check(ctx)
+    b.q[3, 70] = float("nan")
+    b.q[17, 0] = float("inf")
+    b.q[requests:] = float("nan")  # rows behind the last request
+    b.pv[5, 1] = float("inf")      # one value of key head 0
+    out, z = b.call(ctx)
+    spoiled = torch.zeros(requests, 4, dtype=torch.bool, device="cuda")
+    spoiled[3, 1] = spoiled[17, 0] = True
+    assert torch.equal(z[:requests][~spoiled], clean_lse[:requests][~spoiled]) and bool(z[:requests][spoiled].isnan().all())
+    rows, clean = out[:requests].reshape(requests, 4, 64), clean_out[:requests].reshape(requests, 4, 64)
+    assert bool(rows[spoiled].isnan().all())
+    same = (~spoiled)[:, :, None].expand(-1, -1, 64).clone()
+    same[:, :2, 1] = False
+    assert torch.equal(rows[same], clean[same])
+    assert not bool(rows[:, :2, 1].isfinite().any())
+
+
+def test_qk_norm_rope_positions_before_zero_turn_the_other_way(ctx):
+    cfg = ml2.Config(2 * 96, 0, 1, 2, 1, 0, 0)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q, k = (torch.randn(200, w, generator=g, device="cuda").bfloat16() for w in (192, 96))
+    kc, vc = (torch.zeros(200, 96, device="cuda").bfloat16() for _ in range(2))
+    positions, out = ints(list(range(-100, 99)) + [-2**31]), torch.zeros_like(q)
+    ml2.QKNormRoPE(ctx, cfg, 32).Forward(out, kc, vc, q, k, k, None, None, positions, ints(list(range(200))))
+    for got, x, heads in ((out, q, 2), (kc, k, 1)):
+        want, slack = base.rope_want(x, None, heads, 96, 32, positions, 10000.0, 1e-5)
+        base.near(got, want, slack, torch.bfloat16)
