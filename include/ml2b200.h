@@ -193,8 +193,9 @@ int ml2_qk_norm_rope(ml2_ctx* ctx, const ml2_qk_norm_rope_args* args);
  * lengths[r] own tokens (the new ones included) lie in the pages table[r]; row i of `queries` sees all prefix_length rows of
  * the prefix and own tokens 0 .. lengths[r] - queries + i. out[row][head] = softmax(scale q.k) v (out may be query); lse (may be null, fp32
  * [n_rows][n_heads]) = log sum exp(scale q.k). A row that sees nothing, or whose scores are all -inf, gives zeros and
- * -inf. Rows from query_start[n_requests] to n_rows stay as they are. Scores, softmax and sums are fp32; the weights are
- * rounded to `dtype` before their product with the values. Prefix rows and cache rows that no query sees are not used,
+ * -inf. Rows from query_start[n_requests] to n_rows stay as they are. Scores, softmax and sums are fp32; the weights
+ * have 22 bits (fp16) or 16 (bf16) in their product with the values. With prefix_length >= 1024 and n_rows * n_heads /
+ * n_kv_heads > 128 those of the prefix are rounded to `dtype`. Prefix rows and cache rows that no query sees are not used,
  * whatever they hold. max_length bounds lengths[]. head_size 64 or 128; strides in elements, multiples of 8; pointers
  * 16-byte aligned. `workspace` (at least ml2_prefix_attention_workspace bytes for the same sizes) holds partial results: calls that
  * may run at the same time need one each. n_rows, prefix_length and max_length choose the kernels, the arrays on the device

@@ -111,6 +111,27 @@ template <typename T> __device__ __forceinline__ uint32_t not_finite(uint32_t w)
 }
 template <typename T> __device__ __forceinline__ uint32_t times_zero(uint32_t w) { return (not_finite<T>(w) >> 15) * 0x7fffu; }  // 0 or NaN
 
+// A weight as the sum of two 16-bit numbers, 22 bits of it in fp16 and 16 in bf16: the products with the values then lose nothing
+// that the output's own rounding leaves to see (with one, the error against 64 bits was 1.3 times that rounding's, 2.8e-4 against
+// 2.1e-4 in fp16). The first lies below the weight, by cutting off the number before it, so that the second is above 0: a weight
+// times an infinite value is infinite, not 0 times infinity. (Weights below 2^-13 in fp16 may have a second part of 0.)
+template <typename T> __device__ __forceinline__ uint32_t below2(float a, float b)
+{
+    const int x = max(__float_as_int(a) - 1, 0), y = max(__float_as_int(b) - 1, 0);
+    if constexpr (std::is_same<T, __half>::value) {
+        uint32_t w;
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(__int_as_float(y)), "f"(__int_as_float(x)));
+        return w;
+    } else {
+        return __byte_perm(x, y, 0x7632);
+    }
+}
+template <typename T> __device__ __forceinline__ uint32_t rest2(uint32_t w, float a, float b)
+{
+    const float2 f = unpack2<T>(w);
+    return pack2<T>(a - f.x, b - f.y);
+}
+
 // Rows of a request that has `count` queries (or of the prefix, which all see), counted 16 at a time.
 __device__ __forceinline__ int row_tiles(const AttnBatch& p, int count) { return (count * p.group + 15) >> 4; }
 // Key tiles that the 16 rows from row0 on look at: as many as the last of them sees.
@@ -494,8 +515,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
                     __syncwarp();
                 }
             }
-            // weights of at most 2^kSlack, rounded to 16 bits for the product: the same half step the output's own rounding costs
-            const uint32_t pf[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]), pack2<T>(s[1][2], s[1][3])};
+            // both parts of the weights: 16 more products a tile, hidden behind loads in all but the largest calls (own tokens of 1229
+            // queries: 3 % more)
+            const uint32_t pf[4] = {below2<T>(s[0][0], s[0][1]), below2<T>(s[0][2], s[0][3]), below2<T>(s[1][0], s[1][1]), below2<T>(s[1][2], s[1][3])};
+            const uint32_t pr[4] = {rest2<T>(pf[0], s[0][0], s[0][1]), rest2<T>(pf[1], s[0][2], s[0][3]), rest2<T>(pf[2], s[1][0], s[1][1]),
+                                    rest2<T>(pf[3], s[1][2], s[1][3])};
             {
                 const int vr = (lane & 7) + ((lane >> 3) & 1) * 8, vc = lane >> 4;
 #pragma unroll
@@ -504,6 +528,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
                     ldsm4_t(b, vt + vr * kRowBytes + (((2 * d + vc) ^ (vr & 7)) << 4));
                     mma16816<T>(acc[2 * d], pf, b[0], b[1]);
                     mma16816<T>(acc[2 * d + 1], pf, b[2], b[3]);
+                    mma16816<T>(acc[2 * d], pr, b[0], b[1]);
+                    mma16816<T>(acc[2 * d + 1], pr, b[2], b[3]);
                 }
             }
             __syncwarp();  // everybody has read the tile that the next load writes over one turn from now
@@ -536,7 +562,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
 // cut into one contiguous run per CTA, so all CTAs do the same work within one tile and a block's runs ("segments") are
 // joined afterwards. Two streams of a CTA alternate on the tensor core:
 //   S = Q K^T (operands in shared memory, S in TMEM, two of them a stream: one is filled while the other is used),
-//   P = exp2(S - m), rounded to 16 bits, over S in TMEM   (256 threads, half a row each)
+//   P = exp2(S - m), in 16 bits, over S in TMEM           (256 threads, half a row each)
 //   O += P V (P from TMEM, V as it lies: MN-major)
 // With more than 128 rows both streams use each key tile, the first with rows 0..127, the second with 128..255. With fewer,
 // both have the same rows and take the key tiles in turn: then HBM bounds the kernel and eight tiles of 16 KB are under way
@@ -552,6 +578,12 @@ constexpr int kBlockThreads = 608;       // per stream 8 softmax warps and one t
 // blocks / by runs): 1 row of 40 heads, 1024 keys 17.8 / 14.9, 4096 27.0 / 27.9, 8192 38.9 / 41.6; 64 rows of 40 heads, 512 keys
 // 26.2 / 21.7, 1024 28.6 / 28.1, 2048 33.0 / 37.3; 512 rows of 8 heads, 512 keys 23.6 / 22.0, 1024 24.3 / 30.5, 4096 32.2 / 84.4.
 constexpr int kBlockPrefixFewRows = 4096, kBlockPrefix = 1024;
+
+// Up to this many rows of a key head both parts of the weights are multiplied (the second lies behind the first, over S as well):
+// HBM bounds the kernel then (the call of 64 rows of 40 heads behind 4032 keys takes 69 us instead of 67). With more rows the
+// products do: that of 1024 rows of 8 heads behind 16384 keys would take 130 us instead of 114, so the weights are rounded to 16
+// bits, for an error against 64 bits of 2.3e-3 instead of 1.7e-3 in bf16.
+constexpr int kWholeRows = kBlockRows / 2;
 
 struct PrefixMaps {
     CUtensorMap k, v;
@@ -612,7 +644,7 @@ __device__ __forceinline__ bool pair_any(int id, bool flag)
     return any != 0;
 }
 
-template <typename T, int kHead>
+template <typename T, int kHead, bool kWhole>
 __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(const __grid_constant__ AttnBatch p, const __grid_constant__ PrefixMaps maps)
 {
     using S = BlockSmem<kHead>;
@@ -778,7 +810,8 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                         if (leader) {
                             tc_mma_ts(t_o, from, tc_operand_at(v), kShapeO, more);
 #pragma unroll
-                            for (int k = 1; k < kKeyTile / 16; ++k) tc_mma_ts(t_o, from + k * 8, tc_operand_at(v + k * (2048 >> 4)), kShapeO, 1);
+                            for (int k = 1; k < kKeyTile / 16 * (kWhole ? 2 : 1); ++k)
+                                tc_mma_ts(t_o, from + k * 8, tc_operand_at(v + k % (kKeyTile / 16) * (2048 >> 4)), kShapeO, 1);
                             tc_commit(&b_o[s][slot]);
                         }
                         __syncwarp();
@@ -907,15 +940,17 @@ __global__ void __launch_bounds__(kBlockThreads, 1) attention_prefix_kernel(cons
                     }
                     const float ref = m == -INFINITY ? 0.f : -m;
                     const uint64_t ref2 = two(ref, ref);
-                    uint32_t w[16];
+                    uint32_t w[16], w2[kWhole ? 16 : 1];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const float2 y = apart(fma2(add2((uint64_t)x[2 * e + 1] << 32 | x[2 * e], ref2), scale2, lower2));
                         const float a = exp2_fast(y.x), b = exp2_fast(y.y);
                         sum[e & 1] = add2(sum[e & 1], two(a, b));
-                        w[e] = pack2<T>(a, b);
+                        w[e] = kWhole ? below2<T>(a, b) : pack2<T>(a, b);
+                        if constexpr (kWhole) w2[e] = rest2<T>(w[e], a, b);
                     }
                     tmem_st16(t_s + half * 16, w);
+                    if constexpr (kWhole) tmem_st16(t_s + 32 + half * 16, w2);
                     tmem_wait_st();
                 }
                 tc_fence_before();
@@ -1176,9 +1211,11 @@ static cudaError_t launch_attention(Ctx* ctx, const AttnBatch& p, const AttnPlan
 {
     bool& ready = ctx->attention_ready[std::is_same<T, __half>::value][kHead == 128];  // shared-memory limits are set once
     cudaError_t e = cudaSuccess;
+    const auto whole = attention_prefix_kernel<T, kHead, true>, rounded = attention_prefix_kernel<T, kHead, false>;
     if (!ready) {
         e = cudaFuncSetAttribute(attention_runs_kernel<T, kHead>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_prefix_kernel<T, kHead>, cudaFuncAttributeMaxDynamicSharedMemorySize, BlockSmem<kHead>::kBytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(whole, cudaFuncAttributeMaxDynamicSharedMemorySize, BlockSmem<kHead>::kBytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(rounded, cudaFuncAttributeMaxDynamicSharedMemorySize, BlockSmem<kHead>::kBytes);
         if (e != cudaSuccess) return e;
         ready = true;
     }
@@ -1193,7 +1230,7 @@ static cudaError_t launch_attention(Ctx* ctx, const AttnBatch& p, const AttnPlan
         cfg.gridDim = dim3(pl.prefix_ctas);
         cfg.blockDim = dim3(kBlockThreads);
         cfg.dynamicSmemBytes = BlockSmem<kHead>::kBytes;
-        if ((e = cudaLaunchKernelEx(&cfg, attention_prefix_kernel<T, kHead>, p, maps)) != cudaSuccess) return e;
+        if ((e = cudaLaunchKernelEx(&cfg, p.n_rows * p.group <= kWholeRows ? whole : rounded, p, maps)) != cudaSuccess) return e;
         ++ctx->launches;
         cfg.numAttrs = 1;  // what follows starts as this kernel's CTAs leave
     }

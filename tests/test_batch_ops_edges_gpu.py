@@ -606,3 +606,55 @@ def test_qk_norm_rope_positions_before_zero_turn_the_other_way(ctx):
     for got, x, heads in ((out, q, 2), (kc, k, 1)):
         want, slack = base.rope_want(x, None, heads, 96, 32, positions, 10000.0, 1e-5)
         base.near(got, want, slack, torch.bfloat16)
+
+
+# ---- the bits of the weights -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,bits", [("fp16", 22), ("bf16", 16)])
+@pytest.mark.parametrize("prefix,rows,heads", [(0, 128, 1), (0, 300, 2), (300, 40, 2), (1023, 200, 1), (1500, 40, 2), (1100, 128, 1), (4200, 1, 2), (20000, 16, 4)])
+@pytest.mark.parametrize("head", [64, 128])
+def test_attention_small_difference_of_large_weights(ctx, dtype, bits, prefix, rows, heads, head):
+    """Two keys have all of the weight, nearly the same, and opposite values: the output is half the difference of their scores,
+    tanh(x / 2). Each weight, of at most 1, keeps `bits` bits; exponential, sum and quotient are off by 2^-21 together; the
+    output by half a step. Rounded to 16 bits alone the weights were off by up to 2^-12 (fp16) and 2^-9 (bf16)."""
+    own = 2 if prefix else 40
+    b = Batch(1, dtype, heads, 1, head, 16, prefix, [own] * rows, [1] * rows)
+    k, v = (b.pk, b.pv) if prefix else (b.k, b.v)
+    places = (2, 9) if prefix else None  # in one tile: two warps, or blocks, would each have a weight of 1
+    x = torch.arange(1, rows * heads + 1, device="cuda").reshape(rows, heads) / (64.0 * rows * heads)
+    b.q.zero_()
+    b.q.reshape(rows, heads, head)[:, :, 0] = x.to(b.t)
+    x = b.q.reshape(rows, heads, head)[:, :, 0].double()
+    b.q.reshape(rows, heads, head)[:, :, 1] = 1
+    b.k[:], b.v[:] = 0, 0
+    b.k[:, 1] = -100
+    if prefix:
+        k[:], v[:] = 0, 0
+        k[:, 1] = -100
+        k[places[0], 1], v[places[0]] = 0, 1
+        k[places[1], :2], v[places[1]] = torch.tensor([-1.0, 0.0], device="cuda"), -1
+    else:
+        for r in range(rows):
+            first, second = b.rows[r][3], b.rows[r][9]
+            k[first, 1], v[first] = 0, 1
+            k[second, :2], v[second] = torch.tensor([-1.0, 0.0], device="cuda"), -1
+    out, z = b.call(ctx, scale=1.0)
+    want = torch.tanh(x / 2)[:, :, None]
+    off = (out.double().reshape(rows, heads, head) - want).abs()
+    bound = base.step(b.t) * want * 1.01 + 2.0 ** -bits + 2.0 ** -21
+    assert bool((off <= bound).all()), (off / bound).max().item()
+    assert ((z.double() - torch.log1p(torch.exp(-x))).abs().max() <= 2.0 ** -20).item()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("prefix,rows", [(0, 3), (300, 40), (1500, 40), (4200, 1), (1500, 200)])
+def test_attention_an_infinite_value_that_is_seen_is_infinite(ctx, dtype, prefix, rows):
+    """Weights that are all the same, powers of two among them: none has a part that is zero."""
+    b = Batch(2, dtype, 2, 2, 64, 16, prefix, [5] * rows, [1] * rows)
+    b.q.zero_()
+    v, at = (b.pv, prefix // 2) if prefix else (b.v, b.rows[0][2])
+    v[at, 3], v[at, 70] = float("inf"), float("-inf")
+    out, _ = b.call(ctx)
+    seen = slice(None) if prefix else slice(0, 1)
+    assert bool((out[seen, 3] == math.inf).all()) and bool((out[seen, 70] == -math.inf).all())
+    out[seen, 3] = out[seen, 70] = 0
+    assert bool(out.isfinite().all())
