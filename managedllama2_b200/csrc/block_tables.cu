@@ -9,7 +9,7 @@
 // bisection of the sums. A page number that is none of the cache's is reported where it is met; it stays off the free stack,
 // and the table that would have it gets -1. What bounds it is latency: loads of the lengths, the scan's barriers, dependent loads and the store.
 // Where the tokens are many (a step that brings prompts), a second kernel of many CTAs writes the slot map from the finished
-// table: 186000 tokens of 512 requests take 14.7 us, 13 of them the first kernel's; one CTA alone took 150. 64 requests that grow
+// table: 186000 tokens of 512 requests take 15.6 us, 13 of them the first kernel's; one CTA alone took 150. 64 requests that grow
 // by one token take 3.6 us.
 #include "../../include/ml2b200.h"
 

@@ -257,9 +257,9 @@ __device__ __forceinline__ bool settle(const AttnBatch& p, const int* s_base, in
 // cut into runs of the same length, one a warp (without that place runs through short requests took 1.5 times as long). It
 // streams its tiles through a ring of its own (cp.async; the next ones are under way while one is used, across the borders of
 // sequences) and leaves a result for every sequence that it has a part of. 16 rows are all the tensor core's m16 has, so a tile of
-// 16 keys (8 KB at head 128) costs 32 products however few rows are real: with one row a request HBM bounds it (64 requests of 135
-// tokens, 40 heads of 128: 173 MB in 36 us, 4.8 TB/s), with many the instructions and their latency (1229 queries of 8 requests,
-// 32 heads: 53000 tiles in 67 us, the keys read again for every 16 queries).
+// 16 keys (8 KB at head 128) costs 48 products however few rows are real: with one row a request HBM bounds it (64 requests of 135
+// tokens, 40 heads of 128: 173 MB in 37 us, 4.7 TB/s), with many the instructions and their latency (1229 queries of 8 requests,
+// 32 heads: 53000 tiles in 70 us, the keys read again for every 16 queries).
 template <typename T, int kHead>
 __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const __grid_constant__ AttnBatch p)
 {
@@ -270,7 +270,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
     int* s_base = reinterpret_cast<int*>(s_mem + kAttnWarps * kStages * 2 * kTileBytes);  // places before request r; the prefix last
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // after the prefix kernel, which has waited for what comes before both, this one starts beside it
+    // After the prefix kernel this one starts beside it, and reads queries, pages and tables without a wait of its own: every block of
+    // that kernel has come past its own wait, for all that precedes both, before it lets this one start. (It waits for the prefix
+    // kernel at its end.)
     if (!p.prefix_ctas) pdl_wait();
     pdl_launch_dependents();  // every block is resident by the time the join's come, which look up their rows meanwhile
     const int total_rows = min(max(p.query_start[p.n_requests], 0), p.n_rows);
@@ -566,15 +568,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_runs_kernel(const _
 //   O += P V (P from TMEM, V as it lies: MN-major)
 // With more than 128 rows both streams use each key tile, the first with rows 0..127, the second with 128..255. With fewer,
 // both have the same rows and take the key tiles in turn: then HBM bounds the kernel and eight tiles of 16 KB are under way
-// (64 rows of 40 heads, 4032 keys: 83 MB in 22 us, start included). With many rows the products themselves (N = 64 reads its
+// (64 rows of 40 heads, 4032 keys: 83 MB in 25 us from a cold start). With many rows the products themselves (N = 64 reads its
 // operands from shared memory at 47 cycles a product instead of 32) and the instructions of the warps that queue them bound it:
-// 1024 rows of 8 heads, 16384 keys: 69 GFLOP in 78 us, the tensor pipe 55 % active. Without the softmax it takes 12 us less,
-// without seven of eight products 31 us less. S tiles of 128 keys, one a stream, took 100 us.
+// 1024 rows of 8 heads, 16384 keys: 69 GFLOP in 68 to 78 us (of different GPUs), the tensor pipe 55 % active. Without the softmax
+// it took 12 us less, without seven of eight products 31 us less. S tiles of 128 keys, one a stream, were tried when one lane
+// alone ran the code that queues the products (64 samples of 40 heads: 100 us a call instead of 83), and not since.
 constexpr int kBlockRows = 256;
 constexpr int kKeyTile = 64;
 constexpr int kRing = 4;                 // key tiles in shared memory, and value tiles
 constexpr int kBlockThreads = 608;       // per stream 8 softmax warps and one that feeds the tensor core; load warp
-// From which length on the prefix is done by blocks, not by runs, with up to 16 rows of a key head and with more. Measured (us by
+// From which length on the prefix is done by blocks, not by runs, with up to 16 rows of a key head and with more. Measured, at up to
+// 512 rows of a key head (with more the runs' time grows and the blocks' hardly does, so that these are better earlier) (us by
 // blocks / by runs): 1 row of 40 heads, 1024 keys 17.8 / 14.9, 4096 27.0 / 27.9, 8192 38.9 / 41.6; 64 rows of 40 heads, 512 keys
 // 26.2 / 21.7, 1024 28.6 / 28.1, 2048 33.0 / 37.3; 512 rows of 8 heads, 512 keys 23.6 / 22.0, 1024 24.3 / 30.5, 4096 32.2 / 84.4.
 constexpr int kBlockPrefixFewRows = 4096, kBlockPrefix = 1024;

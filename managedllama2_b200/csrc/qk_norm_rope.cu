@@ -5,7 +5,7 @@
 //   (y[i], y[i + h]) -> (y[i] c - y[i + h] s, y[i] s + y[i + h] c),  h = rotary / 2, i < h, angle = pos * theta^(-2 i / rotary)
 //
 // Every element is read once and written once. With many tokens instruction issue is as near as HBM (4032 tokens of 64 / 8 heads
-// of 128: 165 MB in 37 us, 4.5 TB/s, 72 % of the issue slots); with few it is the latency of one launch (one token 2.8 us).
+// of 128: 165 MB in 37 us, 4.5 TB/s, 72 % of the issue slots); with few it is the latency of one launch (one token 2.7 us).
 // The angle is reduced in 64 bits (turns = pos * freq / 2 pi, minus the nearest whole number): in 32 bits a position of
 // 100000 alone leaves an error of 0.004 in the angle. All else is 32-bit arithmetic with one rounding at the store.
 #include "../../include/ml2b200.h"

@@ -339,7 +339,8 @@ class QKNormRoPE(Module):
     """Norm of query and key heads, rotation and cache write of a batch of tokens (``ml2_qk_norm_rope``).
 
     ``query``, ``key`` and ``value`` are [tokens][heads * headSize] and may be columns of one tensor; the caches are
-    [rows][numKVHeads * headSize]. ``queryWeight`` and ``keyWeight`` are None for models without head norms."""
+    [rows][numKVHeads * headSize]. ``queryWeight`` and ``keyWeight`` are None for models without head norms. ``queryOutput`` may be
+    ``query`` (with its strides). Heads of any multiple of 16 up to 256; ``PrefixAttention`` reads those of 64 and 128."""
 
     def __init__(self, cudaContext, config, rotarySize=None):
         super().__init__(cudaContext)
@@ -381,7 +382,9 @@ class PrefixAttention(Module):
     """Attention of a batch that shares a prefix (``ml2_prefix_attention``).
 
     ``prefixKey`` and ``prefixValue`` are the shared rows, [length][numKVHeads * headSize] (a slice of a ``Transformer``'s own
-    caches will do; None: nothing is shared), ``keyCache`` and ``valueCache`` the pages of all requests."""
+    caches will do; None: nothing is shared), ``keyCache`` and ``valueCache`` the pages of all requests. Runs on the stream that the
+    context was given, behind what a ``Transformer`` of the context has queued. Heads of 64 or 128; the config's ``dim`` is
+    taken as numHeads heads of one size, so a model whose heads have another one gets a config of its own here."""
 
     def __init__(self, cudaContext, config, pageSize):
         super().__init__(cudaContext)
