@@ -70,7 +70,7 @@ int ml2_ctx_create(int device, ml2_ctx** out);
 int ml2_ctx_destroy(ml2_ctx* ctx);
 /* The stream of the context's launches. ml2_model_forward moves the context to the model's own stream, where the
  * operators of one sequence follow it; ml2_block_tables, ml2_qk_norm_rope and ml2_prefix_attention come back to the stream
- * set here (outside a capture, behind what the model has queued). */
+ * set here, behind what the model has queued, and the model's next forward comes behind them (outside a capture). */
 int ml2_ctx_set_stream(ml2_ctx* ctx, void* cuda_stream);
 /* Programmatic dependent launch between consecutive operator calls (default off at this level:
  * the reference's semantics are plain stream order). */

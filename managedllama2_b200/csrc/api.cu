@@ -33,22 +33,40 @@ int use_device(const Ctx* ctx)
     return ML2_OK;
 }
 
+// What `to` is given from here on comes behind what `from` has been given so far. Not where either is being captured: a capture
+// cannot wait for what lies outside it.
+static int follow(cudaStream_t to, cudaStream_t from)
+{
+    cudaStreamCaptureStatus of_to = cudaStreamCaptureStatusNone, of_from = cudaStreamCaptureStatusNone;
+    cudaEvent_t queued;
+    cudaError_t e = cudaStreamIsCapturing(to, &of_to);
+    if (e == cudaSuccess) e = cudaStreamIsCapturing(from, &of_from);
+    if (e == cudaSuccess && of_to == cudaStreamCaptureStatusNone && of_from == cudaStreamCaptureStatusNone &&
+        (e = cudaEventCreateWithFlags(&queued, cudaEventDisableTiming)) == cudaSuccess) {
+        e = cudaEventRecord(queued, from);
+        if (e == cudaSuccess) e = cudaStreamWaitEvent(to, queued, 0);
+        cudaEventDestroy(queued);
+    }
+    return e == cudaSuccess ? ML2_OK : fail(ML2_E_CUDA, "order of two streams: %s", cudaGetErrorString(e));
+}
+
 int use_callers_stream(Ctx* ctx)
 {
     if (int rc = use_device(ctx)) return rc;
-    if (ctx->stream == ctx->caller_stream) return ML2_OK;
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    cudaError_t e = cudaStreamIsCapturing(ctx->caller_stream, &capture);
-    if (e == cudaSuccess && capture == cudaStreamCaptureStatusNone) {  // a capture cannot wait for what lies outside it
-        cudaEvent_t queued;
-        if ((e = cudaEventCreateWithFlags(&queued, cudaEventDisableTiming)) == cudaSuccess) {
-            e = cudaEventRecord(queued, ctx->stream);
-            if (e == cudaSuccess) e = cudaStreamWaitEvent(ctx->caller_stream, queued, 0);
-            cudaEventDestroy(queued);
-        }
+    if (ctx->stream != ctx->caller_stream) {
+        if (int rc = follow(ctx->caller_stream, ctx->stream)) return rc;
+        ctx->stream = ctx->caller_stream;
     }
-    if (e != cudaSuccess) return fail(ML2_E_CUDA, "caller's stream: %s", cudaGetErrorString(e));
-    ctx->stream = ctx->caller_stream;
+    ctx->callers_calls = true;
+    return ML2_OK;
+}
+
+int use_model_stream(Ctx* ctx, cudaStream_t stream)
+{
+    if (ctx->callers_calls && ctx->caller_stream != stream)
+        if (int rc = follow(stream, ctx->caller_stream)) return rc;
+    ctx->callers_calls = false;
+    ctx->stream = stream;
     return ML2_OK;
 }
 
@@ -287,8 +305,7 @@ int ml2_ctx_synchronize(ml2_ctx* h)
     if (!h) return fail(ML2_E_INVALID, "null context");
     Ctx* c = reinterpret_cast<Ctx*>(h);
     if (int rc = use_device(c)) return rc;
-    cudaError_t e = cudaStreamSynchronize(c->stream);
-    if (e == cudaSuccess && c->stream != c->caller_stream) e = cudaStreamSynchronize(c->caller_stream);
+    const cudaError_t e = cudaStreamSynchronize(c->stream);
     if (e != cudaSuccess) return fail(ML2_E_CUDA, "synchronize: %s", cudaGetErrorString(e));
     return ML2_OK;
 }
@@ -298,8 +315,7 @@ int ml2_ctx_status(ml2_ctx* h, unsigned* error, unsigned* detail)
     if (!c) return fail(ML2_E_INVALID, "null context");
     if (int rc = use_device(c)) return rc;
     DeviceStatus both[2] = {};
-    cudaError_t e = c->stream != c->caller_stream ? cudaStreamSynchronize(c->caller_stream) : cudaSuccess;
-    if (e == cudaSuccess) e = cudaMemcpyAsync(both, c->status_dev, sizeof(both), cudaMemcpyDeviceToHost, c->stream);
+    cudaError_t e = cudaMemcpyAsync(both, c->status_dev, sizeof(both), cudaMemcpyDeviceToHost, c->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
     const int which = both[0].error ? 0 : 1;  // the other word, if it is set too, is reported by the next call
     const DeviceStatus& st = both[which];

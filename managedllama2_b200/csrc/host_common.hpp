@@ -15,6 +15,7 @@ struct Ctx {
     int sm_count = 0;
     cudaStream_t stream = nullptr;         // of the next launch: the caller's, or a model's own once that has run
     cudaStream_t caller_stream = nullptr;  // what ml2_ctx_set_stream was given last
+    bool callers_calls = false;            // a batched-decoding call has come back to it since a model ran
     bool pdl = false;
     DeviceStatus* status_dev = nullptr;   // [0] waits of a model that ran out, [1] what a batched-decoding operator met
     void* scratch = nullptr;          // host-buffer entry points stage their vectors here
@@ -43,6 +44,8 @@ int use_device(const Ctx* ctx);
 // The same, and the context's launches go to the caller's stream again, behind what a model of the context has queued on its own:
 // a caller's tensors are ordered by the caller's stream.
 int use_callers_stream(Ctx* ctx);
+// The other way: a model's next launches, on its own stream, come behind such calls, which may still read its caches.
+int use_model_stream(Ctx* ctx, cudaStream_t stream);
 int plan_matvec(const Ctx* ctx, Fmt fmt, Epi epi, int rows, int cols, int nmat, MatVecPlan* pl);
 int launch_matvec(Ctx* ctx, Fmt fmt, Epi epi, Pro pro, const MatVecPlan& pl, MatVecParams prm, bool pdl);
 

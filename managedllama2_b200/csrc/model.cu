@@ -1096,7 +1096,7 @@ int ml2_model_forward(ml2_model* h, int pos, int next_pos, int write_token)
     Ctx* ctx = m->ctx;
     if ((rc = use_device(ctx))) return rc;
     if (m->poisoned) return fail(ML2_E_STATE, "forward: an earlier kernel gave up waiting; call ml2_model_reset first");
-    ctx->stream = m->stream;
+    if ((rc = use_model_stream(ctx, m->stream))) return rc;
     m->last_pos = pos;
     if (!m->mega_built && (rc = build_mega(m))) return rc;
     if (m->mega_ok) return forward_mega(m, pos, next_pos, write_token);
@@ -1416,8 +1416,7 @@ int ml2_model_profile(ml2_model* h, int iters, double* avg_us, double* algo_byte
     if (rc) return rc;
     if (iters < 1) return fail(ML2_E_INVALID, "profile: iters=%d", iters);
     Ctx* ctx = m->ctx;
-    if ((rc = use_device(ctx))) return rc;
-    ctx->stream = m->stream;
+    if ((rc = use_device(ctx)) || (rc = use_model_stream(ctx, m->stream))) return rc;
     const ml2_config& c = m->cfg;
     __half* x_save = nullptr;
     ML2_CUDA(cudaMalloc(&x_save, (size_t)c.dim * 2));

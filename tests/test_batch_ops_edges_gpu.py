@@ -658,3 +658,54 @@ def test_attention_an_infinite_value_that_is_seen_is_infinite(ctx, dtype, prefix
     assert bool((out[seen, 3] == math.inf).all()) and bool((out[seen, 70] == -math.inf).all())
     out[seen, 3] = out[seen, 70] = 0
     assert bool(out.isfinite().all())
+
+
+def test_a_model_goes_on_behind_the_operators_that_read_its_cache():
+    """The next prompt overwrites the rows that a call on the caller's stream has still to read."""
+    c = ml2.CudaContext(0)
+    tr = small_model(c)
+    rs = tr.runstate_ptrs()
+
+    class Rows:
+        def __init__(self, at):
+            self.__cuda_array_interface__ = {"shape": (64, 256), "typestr": "<f2", "data": (at, False), "version": 2}
+    b = Batch(12, "fp16", 2, 2, 128, 16, 4, [4, 30, 1], [1, 1, 1])
+    b.pk, b.pv = (torch.as_tensor(Rows(p), device="cuda")[:4] for p in (rs.key_cache, rs.value_cache))
+    for pos in range(4):
+        tr.Forward(pos, pos + 1, False)
+    want, lse = b.call(c)
+    torch.cuda.synchronize()
+    first = b.pk.clone()
+    tr.set_tokens([411, 5, 17, 230])
+    for _ in range(2):
+        busy(torch.cuda.current_stream())
+        out, z = b.call(c)  # behind 20 ms of nothing
+        for pos in range(4):
+            tr.Forward(pos, pos + 1, False)
+        tr.synchronize()
+        torch.cuda.synchronize()
+        assert not torch.equal(b.pk, first)
+        assert torch.equal(out, want) and torch.equal(z, lse)
+        tr.set_tokens([7, 99, 300, 41])
+        for pos in range(4):
+            tr.Forward(pos, pos + 1, False)
+        tr.synchronize()
+        tr.set_tokens([411, 5, 17, 230])
+    assert c.status() == (0, 0)
+    tr.close()
+    c.close()
+
+
+def test_errors_of_operators_that_ran_before_a_model_are_reported():
+    c = ml2.CudaContext(0)
+    tr = small_model(c)
+    b = Batch(4, "fp16", 2, 2, 64, 16, 30, [40, 40], [1, 1])
+    b.table[1, 1] = 10**6
+    busy(torch.cuda.current_stream())
+    b.call(c)
+    tr.Forward(0, 1, False)
+    with pytest.raises(ml2.Ml2Error, match="page of request 1"):
+        c.status()
+    tr.synchronize()
+    tr.close()
+    c.close()
