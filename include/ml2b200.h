@@ -160,7 +160,7 @@ int ml2_argmax(ml2_ctx* ctx, const void* logits, int vocab_size, int* tokens, in
  * query_start[n_requests] to max_tokens are padding: slot -1, position 0. A page number that is none of the cache's stays
  * off the free stack when it is given back, is entered as -1 when it is taken, has slot -1, and is reported.
  * lengths_out and free_count_out may be the arrays lengths and free_count; where they are others, the call can be
- * repeated with the same result. */
+ * repeated with the same result. No other two arrays may overlap. */
 typedef struct ml2_block_tables_args {
     const int *lengths, *new_lengths; /* [n_requests] */
     int *table, *free_pages;          /* [n_requests][table_stride], [n_pages] */

@@ -709,3 +709,43 @@ def test_errors_of_operators_that_ran_before_a_model_are_reported():
     tr.synchronize()
     tr.close()
     c.close()
+
+
+def check_guarded(ctx, b):
+    out, z = guarded_call(ctx, b)
+    total = sum(b.count)
+    want, lse, tol, tol_lse = b.want()
+    assert bool(((out[:total].double() - want).abs() <= tol).all()) and bool(((z[:total].double() - lse).abs() <= tol_lse).all())
+    assert bool((out[total:] == 7.0).all()) and bool((z[total:] == 7.0).all())
+
+
+@pytest.mark.parametrize("heads,kv,prefix,rows", [(65536, 1, 40, 2), (65536, 1, 1100, 2), (65536, 65536, 9, 1), (4096, 16, 1300, 3), (1, 1, 1000003, 3),
+                                                  (2, 1, 1000003, 70)])
+def test_attention_of_many_heads_and_of_a_prefix_of_a_million(ctx, heads, kv, prefix, rows):
+    check_guarded(ctx, Batch(heads + prefix, "bf16", heads, kv, 64, 16, prefix, [20] * rows, [1] * rows, extra_rows=1))
+
+
+@pytest.mark.parametrize("page", [1, 64, 1024])
+def test_attention_of_long_requests(ctx, page):
+    check_guarded(ctx, Batch(page, "fp16", 4, 2, 64, page, 50, [300001, 1, 70000], [3, 1, 40], extra_rows=1))
+
+
+def test_tables_of_half_a_million_tokens_of_a_request(ctx):
+    plain, dev = base.tables_setup(random.Random(3), 3, 1, 600000, 1800000)
+    for new in ([600000, 0, 1], [5, 590001, 2], [0, 0, 600000]):
+        base.tables_step(ctx, plain, dev, new, max(1, sum(max(0, b - a) for a, b in zip(plain.old, new)) + 3), 7)
+
+
+def test_qk_norm_rope_of_many_tokens(ctx):
+    tokens, cfg = 70001, ml2.Config(2 * 16, 0, 1, 2, 1, 0, 0)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q, k = (torch.randn(tokens, w, generator=g, device="cuda").half() for w in (32, 16))
+    w = (1 + torch.randn(16, generator=g, device="cuda") / 8).half()
+    kc, vc = (torch.zeros(tokens + 5, 16, device="cuda").half() for _ in range(2))
+    out, positions = torch.zeros_like(q), torch.arange(tokens, device="cuda", dtype=torch.int32) * 30000
+    slots = torch.randperm(tokens + 5, generator=g, device="cuda")[:tokens].to(torch.int32)
+    ml2.QKNormRoPE(ctx, cfg).Forward(out, kc, vc, q, k, k, w, w, positions, slots)
+    for got, x, heads in ((out, q, 2), (kc[slots.long()], k, 1)):
+        want, slack = base.rope_want(x, w, heads, 16, 16, positions, 10000.0, 1e-5)
+        base.near(got, want, slack, torch.float16)
+    assert torch.equal(vc[slots.long()], k)
